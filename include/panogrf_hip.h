@@ -465,6 +465,54 @@ int pgrf_equirec_to_cube(const float* erp, int N, int H, int W, int C, long long
                          const float* stdv, float* out, long long out_sn, long long out_sh, long long out_sw, long long out_sc,
                          void* stream);
 
+/* ------------------------------------------------------------------ token operators -------- */
+/* Pieces of a transformer block for nets over tokens (the samples of a ray, the patches of a panorama): forward, backward and a form over
+ * a cache.  Element types: every tensor of a call has the one named by `dtype` unless its comment says otherwise; sums, softmax statistics
+ * and norms are float throughout.  Strides are in elements. */
+#define PGRF_DTYPE_F32 0
+#define PGRF_DTYPE_BF16 1
+#define PGRF_DTYPE_F16 2
+
+/* Norms before and after a block, fused with its gate and residual scale:  x' = x + scale * gate (.) Npost(y),  z = Npre(x').
+ * x, y, x_out, z_out [rows, C] contiguous; weights and biases [C], NULL = 1 / 0 (biases are read by PGRF_NORM_LAYER only); gate [rows /
+ * rows_per_gate, C], NULL = 1: row i takes gate row i / rows_per_gate.  y NULL: x' = x (x_out is not written).  Without PGRF_NORM_POST the
+ * norm of y is left out, without PGRF_NORM_PRE z.  stats [rows, 4] float (NULL = not wanted) is what the backward pass needs.  z comes from
+ * the unrounded x'.  x_out may be x or y where no
+ * backward pass follows (it reads both). */
+#define PGRF_NORM_LAYER 1   /* (a - mean) / sqrt(var + eps); without it a / sqrt(mean(a^2) + eps) */
+#define PGRF_NORM_POST 2
+#define PGRF_NORM_PRE 4
+#define PGRF_BLOCK_NORM_MAX_C 8192
+int pgrf_block_norm(const void* x, const void* y, const void* gate, long long rows_per_gate, const void* post_w, const void* post_b,
+                    const void* pre_w, const void* pre_b, int dtype, long long rows, int C, int flags, float scale, float eps, void* x_out,
+                    void* z_out, float* stats, void* stream);
+/* Gradients for upstream dx_out, dz [rows, C] (NULL = zero); x, y, the gate and the weights are the forward's, stats what it wrote.  Any of dx, dy, dgate, dpost_w, dpost_b, dpre_w, dpre_b may be NULL; those
+ * asked for are written, not accumulated (a bias' only with PGRF_NORM_LAYER).  `workspace`: 16-byte aligned scratch of the size the
+ * function below names, read only where a weight's or a shared gate's gradient is asked for. */
+size_t pgrf_block_norm_backward_workspace_bytes(long long rows, int C, long long rows_per_gate);
+int pgrf_block_norm_backward(const void* x, const void* y, const void* gate, long long rows_per_gate, const void* post_w, const void* post_b,
+                             const void* pre_w, const float* stats, const void* dx_out, const void* dz, int dtype, long long rows, int C, int flags,
+                             float scale, void* dx, void* dy, void* dgate, void* dpost_w, void* dpost_b, void* dpre_w, void* dpre_b, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* Rotary positions of queries and keys in one launch: q [B,N,q_heads,D] and k [B,N,k_heads,D] (k_heads 0: none) by the strides of their first
+ * three axes, the channels side by side; q_out, k_out contiguous.  Pair i of the first rotary_dim channels (interleaved: 2i, 2i+1; otherwise
+ * i, i + rotary_dim/2) turns by position * f_i and is multiplied by `magnitude`; channels behind are copied.  f_i = base^(-2i/rotary_dim) and
+ *   PGRF_ROTARY_LINEAR  f_i / factor
+ *   PGRF_ROTARY_NTK     base * factor^(rotary_dim/(rotary_dim-2)) in place of base
+ *   PGRF_ROTARY_PARTS   f_i (t + (1-t)/factor), t = clamp((trained_length f_i / 2 pi - low) / (high - low), 0, 1)
+ * positions: [B,N] by pos_sb (0: shared) and 1, type 0 int32, 1 int64, 2 float, 3 double.  Angles are reduced in double.  backward != 0: the
+ * transpose (the opposite turn), for gradients. */
+#define PGRF_ROTARY_MAX_DIM 256
+#define PGRF_ROTARY_PLAIN 0
+#define PGRF_ROTARY_LINEAR 1
+#define PGRF_ROTARY_NTK 2
+#define PGRF_ROTARY_PARTS 3
+int pgrf_rotary(const void* q, long long q_sb, long long q_sn, long long q_sh, int q_heads, const void* k, long long k_sb, long long k_sn,
+                long long k_sh, int k_heads, const void* positions, int position_type, long long pos_sb, int dtype, int B, int N, int D,
+                int rotary_dim, int interleaved, double base, int scaling, double factor, double trained_length, double low, double high,
+                float magnitude, int backward, void* q_out, void* k_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -153,6 +153,14 @@ SYMBOLS = {
     "pgrf_equirec_to_cube": (C.c_int, [_P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_longlong, C.c_longlong, C.c_longlong, C.c_longlong,
                                        _P, _P, C.c_int, C.c_int, _P, _P, _P, _P, C.c_longlong, C.c_longlong, C.c_longlong,
                                        C.c_longlong, _P]),
+    "pgrf_block_norm": (C.c_int, [_P, _P, _P, C.c_longlong, _P, _P, _P, _P, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_float, C.c_float,
+                                  _P, _P, _P, _P]),
+    "pgrf_block_norm_backward_workspace_bytes": (C.c_size_t, [C.c_longlong, C.c_int, C.c_longlong]),
+    "pgrf_block_norm_backward": (C.c_int, [_P, _P, _P, C.c_longlong, _P, _P, _P, _P, _P, _P, C.c_int, C.c_longlong, C.c_int, C.c_int,
+                                           C.c_float, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
+    "pgrf_rotary": (C.c_int, [_P, C.c_longlong, C.c_longlong, C.c_longlong, C.c_int, _P, C.c_longlong, C.c_longlong, C.c_longlong, C.c_int,
+                              _P, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_double, C.c_int,
+                              C.c_double, C.c_double, C.c_double, C.c_double, C.c_float, C.c_int, _P, _P, _P]),
     "pgrf_render_rays_train": (C.c_int, [C.POINTER(PgrfFrame), _P, _P, C.POINTER(PgrfRenderCfg), _P, C.c_int, _P, _P,
                                          C.POINTER(PgrfPassOut), C.POINTER(PgrfPassOut), _P, _P, _P, C.c_size_t, _P]),
 }

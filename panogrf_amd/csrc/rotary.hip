@@ -1,0 +1,203 @@
+// Rotary positions: the pair i of a head's first `rot` channels is turned by the angle  position * f_i,  f_i = base^(-2i/rot), scaled for long
+// contexts; the gradient is the turn by the opposite angle, so one kernel serves both directions.
+//   half layout: pair i = channels (i, i + rot/2);  interleaved: channels (2i, 2i + 1);  channels behind `rot` are copied
+//
+// The angle of a far position needs more than float: f_i / 2 pi (revolutions by position) comes from the host in double, the product is taken and
+// reduced to a fraction of a revolution in double, and only the fraction goes to the float sine and cosine.  A workgroup forms them once for its
+// tokens in LDS and turns the query and key heads of those tokens with them; what is left is one read and one write of every value, so memory
+// bounds it.
+#include <cmath>
+
+#include "pgrf_experiments.h"
+#include "token_common.h"
+
+namespace pgrf {
+namespace tok {
+
+constexpr int kMaxPairs = PGRF_ROTARY_MAX_DIM / 2;
+
+struct Strided { const void* in; void* out; long long sb, sn, sh; int heads; };   // in: [B,N,heads,D] by strides; out: contiguous
+
+struct RotaryArgs {
+  Strided x[2];
+  const void* pos;
+  long long pos_b;               // stride of the positions' batch axis (0: shared)
+  int pos_kind, B, N, D, rot, tile, interleaved;
+  float sign, magnitude, inv_items, inv_per_head;
+  int items;                     // work items of a token
+  int per_head;                  // work items of a head
+  double rev[kMaxPairs];         // revolutions by position
+};
+
+// n / d for 0 <= n < 2^21 with inv = 1.f / d: n + 0.5 lies at least 0.5 from every multiple of d, which the rounding of the product cannot bridge
+__device__ __forceinline__ int quick_div(int n, float inv) { return (int)(((float)n + 0.5f) * inv); }
+
+enum { kPairs = 0, kHalves = 1, kAnyHalves = 2 };
+
+template <typename T, int V, int HOW>
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
+  extern __shared__ float2 turn[];                   // [tile][rot/2]: cos, sin
+  const int half = a.rot >> 1;
+  const long long tokens = (long long)a.B * a.N, t0 = (long long)blockIdx.x * a.tile;
+  const int here = tokens - t0 < a.tile ? (int)(tokens - t0) : a.tile;
+  for (int i = threadIdx.x; i < here * half; i += 256) {
+    const int k = i / half, pair = i - k * half;
+    const long long tok = t0 + k, b = tok / a.N, at = b * a.pos_b + (tok - b * a.N);
+    const double p = a.pos_kind == 0 ? (double)((const int*)a.pos)[at] : a.pos_kind == 1 ? (double)((const long long*)a.pos)[at]
+                   : a.pos_kind == 2 ? (double)((const float*)a.pos)[at] : ((const double*)a.pos)[at];
+    const double r = p * a.rev[pair];
+    const float f = 2.f * (float)(r - rint(r));
+    float s, c;
+    sincospif(f, &s, &c);
+    turn[i] = make_float2(c * a.magnitude, s * a.magnitude * a.sign);
+  }
+  __syncthreads();
+  const int total = here * a.items;
+  for (int it = threadIdx.x; it < total; it += 256) {
+    const int k = quick_div(it, a.inv_items), rem = it - k * a.items;
+    int head = quick_div(rem, a.inv_per_head);
+    const int j = rem - head * a.per_head;
+    const long long tok = t0 + k, b = tok / a.N, n = tok - b * a.N;
+    const int which = head >= a.x[0].heads ? 1 : 0;
+    const Strided& x = a.x[which];
+    if (which) head -= a.x[0].heads;
+    const T* in = (const T*)x.in + b * x.sb + n * x.sn + head * x.sh;
+    T* out = (T*)x.out + (tok * x.heads + head) * a.D;
+    const float2* cs = turn + k * half;
+    if constexpr (HOW == kHalves) {                  // an item = V pairs (two vectors), or a vector behind `rot`
+      const int np = half / V;
+      if (j < np) {
+        const int c0 = j * V;
+        const Vec<T, V> u = load_vec<T, V>(in + c0), w = load_vec<T, V>(in + c0 + half);
+        Vec<T, V> ou, ow;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float2 q = cs[c0 + e];
+          const float p = (float)u.e[e], r = (float)w.e[e];
+          ou.e[e] = (T)(p * q.x - r * q.y);
+          ow.e[e] = (T)(r * q.x + p * q.y);
+        }
+        store_vec<T, V>(out + c0, ou);
+        store_vec<T, V>(out + c0 + half, ow);
+      } else {
+        const int c0 = a.rot + (j - np) * V;
+        store_vec<T, V>(out + c0, load_vec<T, V>(in + c0));
+      }
+    } else {                                         // an item = V neighbouring channels
+      const int c0 = j * V;
+      const Vec<T, V> u = load_vec<T, V>(in + c0);
+      Vec<T, V> o = u;
+      if constexpr (HOW == kPairs) {
+#pragma unroll
+        for (int e = 0; e + 1 < V; e += 2)
+          if (c0 + e < a.rot) {
+            const float2 q = cs[(c0 + e) >> 1];
+            const float p = (float)u.e[e], r = (float)u.e[e + 1];
+            o.e[e] = (T)(p * q.x - r * q.y);
+            o.e[e + 1] = (T)(r * q.x + p * q.y);
+          }
+        if constexpr (V == 1) {
+          if (c0 < a.rot) {
+            const float2 q = cs[c0 >> 1];
+            const float p = (float)u.e[0], r = (float)in[c0 ^ 1];
+            o.e[0] = (T)((c0 & 1) ? p * q.x + r * q.y : p * q.x - r * q.y);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const int c = c0 + e;
+          if (c < a.rot) {
+            const bool low = c < half;
+            const float2 q = cs[low ? c : c - half];
+            const float p = (float)u.e[e], r = (float)in[low ? c + half : c - half];
+            o.e[e] = (T)(low ? p * q.x - r * q.y : p * q.x + r * q.y);
+          }
+        }
+      }
+      store_vec<T, V>(out + c0, o);
+    }
+  }
+}
+
+template <typename T>
+static void launch_rotary(const RotaryArgs& a, bool vec, dim3 grid, size_t lds, hipStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  if (a.interleaved) {
+    if (vec) hipLaunchKernelGGL((rotary_kernel<T, V, kPairs>), grid, dim3(256), lds, s, a);
+    else hipLaunchKernelGGL((rotary_kernel<T, 1, kPairs>), grid, dim3(256), lds, s, a);
+  } else if (vec && (a.rot / 2) % V == 0) {
+    hipLaunchKernelGGL((rotary_kernel<T, V, kHalves>), grid, dim3(256), lds, s, a);
+  } else if (vec) {
+    hipLaunchKernelGGL((rotary_kernel<T, V, kAnyHalves>), grid, dim3(256), lds, s, a);
+  } else {
+    hipLaunchKernelGGL((rotary_kernel<T, 1, kAnyHalves>), grid, dim3(256), lds, s, a);
+  }
+}
+
+}  // namespace tok
+}  // namespace pgrf
+
+using namespace pgrf;
+using namespace pgrf::tok;
+
+extern "C" int pgrf_rotary(const void* q, long long q_sb, long long q_sn, long long q_sh, int q_heads, const void* k, long long k_sb, long long k_sn,
+                           long long k_sh, int k_heads, const void* positions, int position_type, long long pos_sb, int dtype, int B, int N, int D,
+                           int rotary_dim, int interleaved, double base, int scaling, double factor, double trained_length, double low, double high,
+                           float magnitude, int backward, void* q_out, void* k_out, void* stream) {
+  const char* who = "pgrf_rotary";
+  if (!dtype_ok(dtype)) return set_error(PGRF_ERR_UNSUPPORTED, "%s: dtype %d (PGRF_DTYPE_F32 | BF16 | F16)", who, dtype);
+  if (B < 0 || N < 0 || q_heads < 1 || k_heads < 0 || D < 2) return set_error(PGRF_ERR_ARG, "%s: bad sizes B=%d N=%d heads=%d,%d D=%d", who, B, N, q_heads, k_heads, D);
+  if (rotary_dim < 2 || (rotary_dim & 1) || rotary_dim > D || rotary_dim > PGRF_ROTARY_MAX_DIM)
+    return set_error(PGRF_ERR_UNSUPPORTED, "%s: rotary_dim=%d (even, at most the head's %d channels and %d)", who, rotary_dim, D, PGRF_ROTARY_MAX_DIM);
+  if ((long long)(q_heads + (long long)k_heads) * D > (1 << 20)) return set_error(PGRF_ERR_UNSUPPORTED, "%s: over 2^20 channels by token", who);
+  if (position_type < 0 || position_type > 3) return set_error(PGRF_ERR_ARG, "%s: position_type %d", who, position_type);
+  if (!(base > 0) || !std::isfinite(base)) return set_error(PGRF_ERR_ARG, "%s: base must be positive", who);
+  if (scaling < PGRF_ROTARY_PLAIN || scaling > PGRF_ROTARY_PARTS) return set_error(PGRF_ERR_ARG, "%s: scaling %d", who, scaling);
+  if (scaling != PGRF_ROTARY_PLAIN && !(factor > 0 && std::isfinite(factor))) return set_error(PGRF_ERR_ARG, "%s: factor must be positive", who);
+  if (scaling == PGRF_ROTARY_NTK && rotary_dim < 4) return set_error(PGRF_ERR_UNSUPPORTED, "%s: this scaling needs rotary_dim of 4 at least", who);
+  if (scaling == PGRF_ROTARY_PARTS && !(trained_length > 0 && high > low)) return set_error(PGRF_ERR_ARG, "%s: scaling by parts needs trained_length > 0 and high > low", who);
+  if ((long long)B * N == 0) return PGRF_OK;
+  if (!q || !q_out || !positions || (k_heads && (!k || !k_out))) return set_error(PGRF_ERR_ARG, "%s: null pointer", who);
+  RotaryArgs a = {};
+  a.x[0] = {q, q_out, q_sb, q_sn, q_sh, q_heads};
+  a.x[1] = {k, k_out, k_sb, k_sn, k_sh, k_heads};
+  a.pos = positions; a.pos_b = pos_sb; a.pos_kind = position_type;
+  a.B = B; a.N = N; a.D = D; a.rot = rotary_dim; a.interleaved = interleaved ? 1 : 0;
+  a.sign = backward ? -1.f : 1.f; a.magnitude = magnitude;
+  const double pi2 = 6.283185307179586476925286766559, bs = scaling == PGRF_ROTARY_NTK ? base * std::pow(factor, rotary_dim / (rotary_dim - 2.0)) : base;
+  const double step = -2.0 * std::log2(bs) / rotary_dim;
+  for (int i = 0; i < rotary_dim / 2; ++i) {
+    double f = std::exp2(step * i);
+    if (scaling == PGRF_ROTARY_LINEAR) f /= factor;
+    if (scaling == PGRF_ROTARY_PARTS) {
+      double keep = (trained_length * f / pi2 - low) / (high - low);
+      keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
+      f = f * (keep + (1 - keep) / factor);
+    }
+    a.rev[i] = f / pi2;
+  }
+  const int V = 16 / (int)dtype_bytes(dtype);
+  bool vec = D % V == 0 && aligned16(q) && aligned16(q_out) && !((q_sb | q_sn | q_sh) % V);
+  if (k_heads) vec = vec && aligned16(k) && aligned16(k_out) && !((k_sb | k_sn | k_sh) % V);
+  const int step_v = vec ? V : 1;
+  const bool halves = !interleaved && vec && (rotary_dim / 2) % V == 0;
+  a.per_head = halves ? rotary_dim / 2 / V + (D - rotary_dim) / V : D / step_v;
+  a.items = (q_heads + k_heads) * a.per_head;
+  a.inv_items = 1.f / a.items;
+  a.inv_per_head = 1.f / a.per_head;
+  // Tokens of a workgroup: about eight items per thread, as long as over a thousand workgroups remain, and 32 KB of sines at most
+  const long long tokens = (long long)B * N;
+  long long tile = 2048 / a.items;
+  if (tile > tokens / 1024) tile = tokens / 1024;
+  if (tile > 4096 / (rotary_dim / 2)) tile = 4096 / (rotary_dim / 2);
+  a.tile = tile < 1 ? 1 : (int)tile;
+  const long long grid = (tokens + a.tile - 1) / a.tile;
+  if (grid > 0x7fffffffll) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tokens", who);
+  const size_t lds = (size_t)a.tile * (rotary_dim / 2) * sizeof(float2);
+  if (dtype == PGRF_DTYPE_F32) launch_rotary<float>(a, vec, dim3((unsigned)grid), lds, (hipStream_t)stream);
+  else if (dtype == PGRF_DTYPE_BF16) launch_rotary<bf16>(a, vec, dim3((unsigned)grid), lds, (hipStream_t)stream);
+  else launch_rotary<f16>(a, vec, dim3((unsigned)grid), lds, (hipStream_t)stream);
+  PGRF_TOK_LAUNCHED(who);
+  return PGRF_OK;
+}

@@ -1,0 +1,70 @@
+"""What the token operators refuse, on the host: no kernel is launched here."""
+import ctypes as C
+
+import pytest
+import torch
+
+from panogrf_amd._lib import PgrfError, lib
+
+PTR = 1 << 20        # an address no kernel ever sees: every call below ends in the checks before it
+
+
+def norm_c(dtype=0, rows=4, channels=8, flags=6, rpg=4, x=PTR, y=PTR, gate=None, x_out=PTR, z=PTR, stats=None):
+    return lib.pgrf_block_norm(x, y, gate, rpg, None, None, None, None, dtype, rows, channels, flags, 1.0, 1e-6, x_out, z, stats, None)
+
+
+@pytest.mark.parametrize('kw,code', [(dict(dtype=3), -3), (dict(dtype=-1), -3), (dict(channels=0), -3), (dict(channels=8193), -3), (dict(rows=-1), -1),
+                                     (dict(flags=8), -1), (dict(y=None), -1), (dict(y=None, flags=0), -1), (dict(gate=PTR, rpg=3), -1), (dict(gate=PTR, rpg=0), -1),
+                                     (dict(x=None), -1), (dict(x_out=None), -1), (dict(z=None), -1), (dict(stats=PTR + 4), -1)])
+def test_block_norm_entry(kw, code):
+    assert norm_c(**kw) == code and b'pgrf_block_norm' in lib.pgrf_last_error()
+
+
+def test_block_norm_entries_without_rows():
+    assert norm_c(rows=0) == 0
+    n = lib.pgrf_block_norm_backward_workspace_bytes(100, 64, 10)
+    assert n >= 64 * 5 * 4
+    args = lambda ws, size: (PTR, PTR, PTR, 10, None, None, None, PTR, PTR, PTR, 0, 100, 64, 6, 1.0, PTR, PTR, PTR, PTR, None, PTR, None, ws, size, None)
+    assert lib.pgrf_block_norm_backward(*args(None, 0)) == -1 and b'workspace' in lib.pgrf_last_error()
+    assert lib.pgrf_block_norm_backward(*args(PTR, 64)) == -1
+    assert lib.pgrf_block_norm_backward(PTR, PTR, None, 1, None, None, None, PTR, PTR, PTR, 0, 100, 64, 6, 1.0, PTR, PTR, PTR, None, None, None, None, None, 0, None) == -1
+
+
+@pytest.mark.parametrize('kw', [dict(y=torch.zeros(2, 3, 7)), dict(gate=torch.ones(8)), dict(y=torch.zeros(2, 3, 8), gate=torch.ones(3, 8)),
+                                dict(y=torch.zeros(2, 3, 8), gate=torch.ones(7)), dict(kind='group'), dict(post_weight=torch.ones(8)), dict(pre=False),
+                                dict(pre_weight=torch.ones(7)), dict(pre_bias=torch.ones(8)), dict(y=torch.zeros(2, 3, 8).half()),
+                                dict(y=torch.zeros(2, 3, 8), post=False, post_weight=torch.ones(8)), dict()])
+def test_block_norm(kw):
+    from panogrf_amd.block_norm import block_norm
+    with pytest.raises(PgrfError):          # (the last: a CPU tensor)
+        block_norm(torch.zeros(2, 3, 8), **kw)
+
+
+def test_block_norm_types():
+    from panogrf_amd.block_norm import block_norm
+    for x in (torch.zeros(2, 8).double(), torch.zeros(2, 8).int(), torch.zeros(()), torch.zeros(2, 8193), torch.zeros(2, 0), None):
+        with pytest.raises(PgrfError):
+            block_norm(x)
+
+
+@pytest.mark.parametrize('kw,code', [(dict(dtype=5), -3), (dict(D=1), -1), (dict(rot=3), -3), (dict(rot=0), -3), (dict(rot=18), -3), (dict(D=512, rot=258), -3),
+                                     (dict(hq=0), -1), (dict(hk=-1), -1), (dict(kind=4), -1), (dict(base=0.0), -1), (dict(base=float('nan')), -1),
+                                     (dict(scaling=4), -1), (dict(scaling=1, factor=0.0), -1), (dict(scaling=2, rot=2, factor=2.0), -3),
+                                     (dict(scaling=3, factor=2.0, low=4.0, high=4.0), -1), (dict(q=None), -1), (dict(hk=1, k=None), -1), (dict(hq=1 << 17), -3)])
+def test_rotary_entry(kw, code):
+    a = dict(q=PTR, hq=1, k=PTR, hk=0, kind=0, dtype=0, D=16, rot=16, base=1e4, scaling=0, factor=1.0, low=1.0, high=32.0)
+    a.update(kw)
+    rc = lib.pgrf_rotary(a['q'], 16, 16, 16, a['hq'], a['k'], 16, 16, 16, a['hk'], PTR, a['kind'], 0, a['dtype'], 2, 3, a['D'], a['rot'], 0, a['base'],
+                         a['scaling'], a['factor'], 4096.0, a['low'], a['high'], 1.0, 0, PTR, PTR, None)
+    assert rc == code and b'pgrf_rotary' in lib.pgrf_last_error()
+
+
+@pytest.mark.parametrize('kw', [dict(rotary_dim=3), dict(rotary_dim=18), dict(rotary_dim=0), dict(layout='quarter'), dict(scaling='cubic'),
+                                dict(positions=torch.arange(4)), dict(positions=torch.arange(3).half()), dict(positions=torch.zeros(3, 3)), dict(positions=None),
+                                dict(k=torch.zeros(2, 4, 1, 16)), dict(k=torch.zeros(2, 3, 1, 8)), dict(k=torch.zeros(2, 3, 1, 16).half()),
+                                dict(k=torch.zeros(2, 3, 0, 16)), dict()])
+def test_rotary(kw):
+    from panogrf_amd.rotary import rotary
+    kw = dict(k=None, positions=torch.arange(3)) | kw
+    with pytest.raises(PgrfError):          # (the last: a CPU tensor)
+        rotary(torch.zeros(2, 3, 4, 16), kw.pop('k'), kw.pop('positions'), **kw)
