@@ -513,6 +513,33 @@ int pgrf_rotary(const void* q, long long q_sb, long long q_sn, long long q_sh, i
                 int rotary_dim, int interleaved, double base, int scaling, double factor, double trained_length, double low, double high,
                 float magnitude, int backward, void* q_out, void* k_out, void* stream);
 
+/* Differential attention: out = (softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v, per head.
+ * q [B,N,H,2,D], k [B,M,Hk,2,D], v [B,M,Hk,2D] by strides (channels side by side; rows 16-byte aligned: every stride a multiple of 16 bytes), D 32, 64
+ * or 128, H a multiple of Hk (head h reads key head h / (H/Hk)).  A query sees the keys j < M (j < lengths[b] where given, clamped to [0,M]) whose
+ * mask byte is not 0 and, with `causal`, j <= i + (M or lengths[b]) - N: the last query stands at the last key.  A query that sees no key gives 0 and
+ * has no gradient.  Values of keys nobody sees are not used, whatever they hold. */
+typedef struct PgrfDiffAttn {
+  const void *q, *k, *v;
+  const void* lam;             /* [H], float with lam_f32, else the tensors' type */
+  const unsigned char* key_mask; /* [B,M] by mask_sb, NULL: every key */
+  const int* lengths;          /* [B] device, NULL: M (forward only) */
+  void* out;                   /* [B,N,H,2D] contiguous */
+  float* lse;                  /* [B,H,2,N] and */
+  float* maps_out;             /* [B,N,H,2,2D]: what the backward pass needs, both NULL = not wanted */
+  void* workspace;             /* >= pgrf_diff_attention_workspace_bytes(), 16-byte aligned */
+  size_t workspace_bytes;
+  long long q_sb, q_sn, q_sh, q_sm, k_sb, k_sn, k_sh, k_sm, v_sb, v_sn, v_sh, mask_sb;   /* strides; *_sm: between the two maps */
+  int dtype, lam_f32, B, N, M, H, Hk, D, causal;
+  float scale;                 /* > 0 */
+} PgrfDiffAttn;
+size_t pgrf_diff_attention_workspace_bytes(int dtype, int B, int N, int M, int H, int Hk, int D);
+int pgrf_diff_attention(const PgrfDiffAttn* a, void* stream);
+/* Gradients for upstream dout [B,N,H,2D] (contiguous): dq [B,N,H,2,D], dk [B,M,Hk,2,D], dv [B,M,Hk,2D] contiguous and dlam [H] of lam's type; any may be
+ * NULL (dk and dv only together).  `a` as in the forward call, with what it wrote to lse and maps_out (`out` is not read); workspace >=
+ * pgrf_diff_attention_backward_workspace_bytes().  No atomics: gradients do not depend on scheduling. */
+size_t pgrf_diff_attention_backward_workspace_bytes(int dtype, int B, int N, int M, int H, int Hk, int D);
+int pgrf_diff_attention_backward(const PgrfDiffAttn* a, const void* dout, void* dq, void* dk, void* dv, void* dlam, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

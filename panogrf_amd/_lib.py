@@ -52,6 +52,13 @@ class PgrfRenderCfg(C.Structure):
                 ("use_vis_coarse", C.c_int), ("use_vis_fine", C.c_int), ("precision", C.c_int)]
 
 
+class PgrfDiffAttn(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "lam", "key_mask", "lengths", "out", "lse", "maps_out", "workspace")] + \
+               [("workspace_bytes", C.c_size_t)] + \
+               [(n, C.c_longlong) for n in ("q_sb", "q_sn", "q_sh", "q_sm", "k_sb", "k_sn", "k_sh", "k_sm", "v_sb", "v_sn", "v_sh", "mask_sb")] + \
+               [(n, C.c_int) for n in ("dtype", "lam_f32", "B", "N", "M", "H", "Hk", "D", "causal")] + [("scale", C.c_float)]
+
+
 ABI_VERSION = 5      # PGRF_ABI_VERSION of include/panogrf_hip.h (struct layouts below)
 
 # every symbol include/panogrf_hip.h declares: name -> (restype, argtypes)
@@ -161,6 +168,10 @@ SYMBOLS = {
     "pgrf_rotary": (C.c_int, [_P, C.c_longlong, C.c_longlong, C.c_longlong, C.c_int, _P, C.c_longlong, C.c_longlong, C.c_longlong, C.c_int,
                               _P, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_double, C.c_int,
                               C.c_double, C.c_double, C.c_double, C.c_double, C.c_float, C.c_int, _P, _P, _P]),
+    "pgrf_diff_attention_workspace_bytes": (C.c_size_t, [C.c_int] * 7),
+    "pgrf_diff_attention": (C.c_int, [C.POINTER(PgrfDiffAttn), _P]),
+    "pgrf_diff_attention_backward_workspace_bytes": (C.c_size_t, [C.c_int] * 7),
+    "pgrf_diff_attention_backward": (C.c_int, [C.POINTER(PgrfDiffAttn), _P, _P, _P, _P, _P, _P]),
     "pgrf_render_rays_train": (C.c_int, [C.POINTER(PgrfFrame), _P, _P, C.POINTER(PgrfRenderCfg), _P, C.c_int, _P, _P,
                                          C.POINTER(PgrfPassOut), C.POINTER(PgrfPassOut), _P, _P, _P, C.c_size_t, _P]),
 }

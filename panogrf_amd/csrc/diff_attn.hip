@@ -1,0 +1,136 @@
+// C entries of the differential attention: checks, the cut of the work, and the choice of the kernels (diff_attn.h).
+#include "pgrf_experiments.h"
+#include "diff_attn.h"
+
+namespace pgrf {
+namespace tok {
+
+#define PGRF_DA_DECL(T, D)                                                                       \
+  int launch_da_fwd_##T##_##D(const DiffArgs& a, int waves, unsigned grid, hipStream_t s);       \
+  int launch_da_bwd_##T##_##D(const DiffArgs& a, int row_waves, unsigned row_grid, int key_waves, unsigned key_grid, hipStream_t s);
+#define PGRF_DA_ALL(X) X(0, 32) X(0, 64) X(0, 128) X(1, 32) X(1, 64) X(1, 128) X(2, 32) X(2, 64) X(2, 128)
+PGRF_DA_ALL(PGRF_DA_DECL)
+
+static int waves_for(long long rows) { return rows > 64 ? 4 : rows > 32 ? 2 : 1; }
+
+// The key axis is cut where the rows alone leave the chip idle: a share is at least 128 keys, and there are about as many workgroups as the chip holds at a time
+// (one of four waves per CU, five of a single wave, whose two buffers take 32 KB)
+static int splits_for(int B, int Hk, long long rows, int M, int* waves) {
+  *waves = waves_for(rows);
+  const long long groups = (long long)B * Hk * ((rows + *waves * 32 - 1) / (*waves * 32));
+  const long long want = *waves == 1 ? 1280 : 512, most = M / 128;
+  long long s = (want + groups - 1) / groups;
+  if (groups * 2 > want) s = 1;
+  if (s > most) s = most;
+  if (s > 128) s = 128;
+  return s < 1 ? 1 : (int)s;
+}
+
+static int check(const PgrfDiffAttn* p, const char* who, bool backward) {
+  if (!p) return set_error(PGRF_ERR_ARG, "%s: null arguments", who);
+  if (!dtype_ok(p->dtype)) return set_error(PGRF_ERR_UNSUPPORTED, "%s: dtype %d (PGRF_DTYPE_F32 | BF16 | F16)", who, p->dtype);
+  if (p->D != 32 && p->D != 64 && p->D != 128) return set_error(PGRF_ERR_UNSUPPORTED, "%s: D=%d (32, 64 or 128)", who, p->D);
+  if (p->B < 0 || p->N < 0 || p->M < 1 || p->H < 1 || p->Hk < 1 || p->H % p->Hk)
+    return set_error(PGRF_ERR_ARG, "%s: bad sizes B=%d N=%d M=%d H=%d Hk=%d (H a multiple of Hk, M at least 1)", who, p->B, p->N, p->M, p->H, p->Hk);
+  if (!(p->scale > 0.f) || p->scale > 1e30f) return set_error(PGRF_ERR_ARG, "%s: scale must be positive", who);
+  if ((long long)p->N * (p->H / p->Hk) > 0x3fffffff || (long long)p->B * p->N > 0x3fffffff || p->M > 0x3fffffff)
+    return set_error(PGRF_ERR_UNSUPPORTED, "%s: over 2^30 rows", who);
+  if ((long long)p->B * p->H * (((long long)p->N + 31) / 32 + 1) > 0xffffff || (long long)p->B * p->Hk * (((long long)p->M + 31) / 32) > 0x7fffffff)
+    return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tiles", who);
+  if ((long long)p->B * p->N == 0) return PGRF_OK;
+  if (!p->q || !p->k || !p->v || !p->lam) return set_error(PGRF_ERR_ARG, "%s: null q / k / v / lam", who);
+  const long long per = 16 / (long long)dtype_bytes(p->dtype);
+  if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) ||
+      (p->q_sb | p->q_sn | p->q_sh | p->q_sm | p->k_sb | p->k_sn | p->k_sh | p->k_sm | p->v_sb | p->v_sn | p->v_sh) % per)
+    return set_error(PGRF_ERR_ARG, "%s: q, k, v: addresses and strides must be multiples of 16 bytes", who);
+  if (backward && (!p->lse || !p->maps_out)) return set_error(PGRF_ERR_ARG, "%s: null lse / maps_out", who);
+  if (backward && p->lengths) return set_error(PGRF_ERR_UNSUPPORTED, "%s: lengths have no backward pass (use key_mask)", who);
+  if (!backward && !p->out) return set_error(PGRF_ERR_ARG, "%s: null out", who);
+  if (!p->lse != !p->maps_out) return set_error(PGRF_ERR_ARG, "%s: lse and maps_out go together", who);
+  if ((p->maps_out && !aligned16(p->maps_out)) || (p->out && !aligned16(p->out))) return set_error(PGRF_ERR_ARG, "%s: out / maps_out must be 16-byte aligned", who);
+  return PGRF_OK;
+}
+
+static DiffArgs args_of(const PgrfDiffAttn* p) {
+  DiffArgs a = {};
+  a.q = p->q; a.k = p->k; a.v = p->v; a.lam = p->lam;
+  a.q_sb = p->q_sb; a.q_sn = p->q_sn; a.q_sh = p->q_sh; a.q_sm = p->q_sm;
+  a.k_sb = p->k_sb; a.k_sn = p->k_sn; a.k_sh = p->k_sh; a.k_sm = p->k_sm;
+  a.v_sb = p->v_sb; a.v_sn = p->v_sn; a.v_sh = p->v_sh;
+  a.mask = p->key_mask; a.mask_sb = p->mask_sb; a.lengths = p->lengths;
+  a.B = p->B; a.N = p->N; a.M = p->M; a.H = p->H; a.Hk = p->Hk; a.G = p->H / p->Hk; a.causal = p->causal ? 1 : 0; a.lam_f32 = p->lam_f32 ? 1 : 0;
+  a.scale = p->scale; a.c = p->scale * kLog2e;
+  a.out = p->out; a.lse = p->lse; a.o12 = p->maps_out; a.splits = 1;
+  return a;
+}
+
+}  // namespace tok
+}  // namespace pgrf
+
+using namespace pgrf;
+using namespace pgrf::tok;
+
+extern "C" {
+
+size_t pgrf_diff_attention_workspace_bytes(int, int B, int N, int M, int H, int Hk, int D) {
+  if (B < 1 || N < 1 || M < 1 || H < 1 || Hk < 1 || H % Hk || D < 1) return 0;
+  int waves;
+  const long long rows = (long long)N * (H / Hk);
+  const int s = splits_for(B, Hk, rows, M, &waves);
+  return s > 1 ? (size_t)s * B * Hk * rows * (4 * D + 4) * sizeof(float) : 0;
+}
+
+int pgrf_diff_attention(const PgrfDiffAttn* p, void* stream) {
+  const char* who = "pgrf_diff_attention";
+  int rc = check(p, who, false);
+  if (rc) return rc;
+  if ((long long)p->B * p->N == 0) return PGRF_OK;
+  DiffArgs a = args_of(p);
+  int waves;
+  const long long rows = (long long)a.N * a.G;
+  a.splits = splits_for(a.B, a.Hk, rows, a.M, &waves);
+  if (a.splits > 1) {
+    const size_t need = pgrf_diff_attention_workspace_bytes(p->dtype, p->B, p->N, p->M, p->H, p->Hk, p->D);
+    if (!p->workspace || !aligned16(p->workspace) || p->workspace_bytes < need)
+      return set_error(PGRF_ERR_ARG, "%s: workspace too small or not 16-byte aligned (%zu < %zu bytes)", who, p->workspace_bytes, need);
+    a.part_o = (float*)p->workspace;
+    a.part_ml = a.part_o + (size_t)a.splits * a.B * a.Hk * rows * 4 * p->D;
+  }
+  const long long grid = (long long)a.B * a.Hk * ((rows + waves * 32 - 1) / (waves * 32)) * a.splits;
+  if (grid > 0x7fffffffll) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tiles", who);
+#define PGRF_DA_FWD(T, D_) \
+  if (p->dtype == T && p->D == D_) return launch_da_fwd_##T##_##D_(a, waves, (unsigned)grid, (hipStream_t)stream);
+  PGRF_DA_ALL(PGRF_DA_FWD)
+  return set_error(PGRF_ERR_UNSUPPORTED, "%s: no kernel", who);
+}
+
+size_t pgrf_diff_attention_backward_workspace_bytes(int, int B, int N, int M, int H, int Hk, int D) {
+  if (B < 1 || N < 1 || M < 1 || H < 1 || Hk < 1 || D < 1) return 0;
+  return (size_t)B * H * N * 3 * sizeof(float);
+}
+
+int pgrf_diff_attention_backward(const PgrfDiffAttn* p, const void* dout, void* dq, void* dk, void* dv, void* dlam, void* stream) {
+  const char* who = "pgrf_diff_attention_backward";
+  int rc = check(p, who, true);
+  if (rc) return rc;
+  if (!dk != !dv) return set_error(PGRF_ERR_ARG, "%s: dk and dv go together", who);
+  if ((long long)p->B * p->N == 0) return set_error(PGRF_ERR_ARG, "%s: no rows: the gradients are 0", who);
+  if (!dout || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return set_error(PGRF_ERR_ARG, "%s: dout null, or a tensor not 16-byte aligned", who);
+  const size_t need = pgrf_diff_attention_backward_workspace_bytes(p->dtype, p->B, p->N, p->M, p->H, p->Hk, p->D);
+  if (!p->workspace || !aligned16(p->workspace) || p->workspace_bytes < need)
+    return set_error(PGRF_ERR_ARG, "%s: workspace too small or not 16-byte aligned (%zu < %zu bytes)", who, p->workspace_bytes, need);
+  DiffArgs a = args_of(p);
+  a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv; a.dlam = dlam;
+  a.delta = (float*)p->workspace;
+  a.dlam_rows = a.delta + (size_t)a.B * a.H * 2 * a.N;
+  const long long rows = (long long)a.N * a.G;
+  const int rw = waves_for(rows), kw = waves_for(a.M);
+  const long long rg = (long long)a.B * a.Hk * ((rows + rw * 32 - 1) / (rw * 32)), kg = (long long)a.B * a.Hk * (((long long)a.M + kw * 32 - 1) / (kw * 32));
+  if (rg > 0x7fffffffll || kg > 0x7fffffffll) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tiles", who);
+#define PGRF_DA_BWD(T, D_) \
+  if (p->dtype == T && p->D == D_) return launch_da_bwd_##T##_##D_(a, rw, (unsigned)rg, kw, (unsigned)kg, (hipStream_t)stream);
+  PGRF_DA_ALL(PGRF_DA_BWD)
+  return set_error(PGRF_ERR_UNSUPPORTED, "%s: no kernel", who);
+}
+
+}  // extern "C"

@@ -68,3 +68,62 @@ def test_rotary(kw):
     kw = dict(k=None, positions=torch.arange(3)) | kw
     with pytest.raises(PgrfError):          # (the last: a CPU tensor)
         rotary(torch.zeros(2, 3, 4, 16), kw.pop('k'), kw.pop('positions'), **kw)
+
+
+def attn(**kw):
+    from panogrf_amd._lib import PgrfDiffAttn
+    a = PgrfDiffAttn(q=PTR, k=PTR, v=PTR, lam=PTR, out=PTR, dtype=1, B=2, N=3, M=4, H=4, Hk=2, D=64, scale=0.1)
+    for n in ('q_sb', 'q_sn', 'q_sh', 'q_sm', 'k_sb', 'k_sn', 'k_sh', 'k_sm', 'v_sb', 'v_sn', 'v_sh'):
+        setattr(a, n, 64)
+    for n, x in kw.items():
+        setattr(a, n, x)
+    return a
+
+
+BAD = [(dict(dtype=3), -3), (dict(D=48), -3), (dict(D=256), -3), (dict(M=0), -1), (dict(H=3), -1), (dict(Hk=0), -1), (dict(N=-1), -1), (dict(scale=0.0), -1),
+       (dict(scale=-1.0), -1), (dict(scale=float('nan')), -1), (dict(q=None), -1), (dict(v=None), -1), (dict(lam=None), -1), (dict(q=PTR + 8), -1),
+       (dict(k_sn=63), -1), (dict(q_sm=4), -1), (dict(lse=PTR), -1), (dict(N=1 << 30), -3)]
+
+
+@pytest.mark.parametrize('kw,code', BAD + [(dict(out=None), -1), (dict(N=1, M=100000, B=1), -1)])       # (the last: a cut key axis without a workspace)
+def test_diff_attention_entry(kw, code):
+    assert lib.pgrf_diff_attention(C.byref(attn(**kw)), None) == code and b'pgrf_diff_attention' in lib.pgrf_last_error()
+
+
+@pytest.mark.parametrize('kw,code', [b for b in BAD if 'lse' not in b[0]] + [(dict(lse=None, maps_out=None), -1), (dict(lengths=PTR), -3), (dict(B=0), -1)])
+def test_diff_attention_backward_entry(kw, code):
+    a = attn(**{**dict(lse=PTR, maps_out=PTR), **kw})
+    assert lib.pgrf_diff_attention_backward(C.byref(a), PTR, PTR, PTR, PTR, PTR, None) == code
+
+
+def test_diff_attention_backward_arguments():
+    a = attn(lse=PTR, maps_out=PTR)
+    assert lib.pgrf_diff_attention_backward(C.byref(a), PTR, PTR, PTR, None, PTR, None) == -1          # dk without dv
+    assert lib.pgrf_diff_attention_backward(C.byref(a), None, PTR, PTR, PTR, PTR, None) == -1
+    assert lib.pgrf_diff_attention_backward(C.byref(a), PTR, PTR, PTR, PTR, PTR, None) == -1 and b'workspace' in lib.pgrf_last_error()
+    assert lib.pgrf_diff_attention(None, None) == -1
+    assert lib.pgrf_diff_attention(C.byref(attn(B=0)), None) == 0
+
+
+Q, K, V, L = torch.zeros(2, 3, 4, 2, 32), torch.zeros(2, 5, 2, 2, 32), torch.zeros(2, 5, 2, 64), torch.zeros(4)
+
+
+@pytest.mark.parametrize('a,kw', [((Q[..., :24], K, V, L), {}), ((Q, K[..., :16], V, L), {}), ((Q, K, V[..., :32], L), {}), ((Q, K, V, L[:3]), {}), ((Q, K[:, :4], V, L), {}),
+                                  ((Q, K[:1], V, L), {}), ((Q[:, :, :3], K, V, L[:3]), {}), ((Q.half(), K, V, L), {}), ((Q.double(), K.double(), V.double(), L), {}),
+                                  ((Q, K, V, L.half()), {}), ((Q, K, V, None), {}), ((Q.flatten(-2), K, V, L), {}), ((Q, K, V, L), dict(scale=0.0)),
+                                  ((Q, K, V, L), dict(key_mask=torch.ones(2, 5))), ((Q, K, V, L), dict(key_mask=torch.ones(2, 4) > 0)),
+                                  ((Q, K, V, L), dict(key_mask=torch.ones(2, 3, 5) > 0)), ((Q, K, V, L), {})])
+def test_diff_attention(a, kw):
+    from panogrf_amd.attention import diff_attention
+    with pytest.raises(PgrfError):          # (the last: CPU tensors)
+        diff_attention(*a, **kw)
+
+
+@pytest.mark.parametrize('n', [torch.tensor([1, 2]), torch.tensor([1], dtype=torch.int32), None, torch.tensor([1.0, 2.0]), torch.tensor([1, 2], dtype=torch.int32)])
+def test_diff_attention_cached(n):
+    from panogrf_amd.attention import diff_attention_cached
+    with pytest.raises(PgrfError):
+        diff_attention_cached(Q, K, V, L, n)
+    with pytest.raises(PgrfError, match='gradients|GPU|lengths'):
+        diff_attention_cached(Q.requires_grad_(True), K, V, L, n)
+    Q.requires_grad_(False)

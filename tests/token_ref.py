@@ -93,3 +93,82 @@ def block_norm(x, y, gate, pw, pb, qw, qb, kind, scale, eps, post, pre, dx1, dz,
     out['grad_pw'], out['grad_pb'] = column(du * hy, edu * hy.abs() + du.abs() * ehy), column(du, edu)
     out['grad_gate_all'] = (scale * dh * u, scale * (edh * u.abs() + dh.abs() * eu) + chain * U * (scale * dh * u).abs())
     return out
+
+
+def diff_attention(q, k, v, lam, see, scale, dout=None, dtype=None):
+    """Values and gradients in 64 bits with first-order bounds: {name: (value, bound)}.  see [B, N, M] bool.
+
+    A product of D values of the type is exact in float, so a score is off by (D + 8) U of its magnitudes (and the power of two behind it by U of the score); a map's value p by
+    that much relative to itself, and by the row sum's chain of at most M / 16 + 64 additions.  For the product with v, p is rounded to the type (half a step; in f16
+    not below 2^-25, as the row's largest value is at least 1 when it is rounded); the score gradients and p1 - lam p2 likewise in the backward pass.  A sum over n values adds
+    (n / 16 + 64) U of their magnitudes: sixteen places of a matrix instruction are added as one."""
+    q, k, v, lam = (t.detach().double() for t in (q, k, v, lam))
+    B, N, H, _, D = q.shape
+    M, Hk = k.shape[1], k.shape[2]
+    G = H // Hk
+    half = HALF[dtype]
+    inner = 0.0 if dtype == torch.float32 else half
+    # below the smallest normal float, 2^-126, a value (and a product with a factor of up to 2^6) keeps fewer bits or none: a map of scores 200 apart has such values
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -120
+    chain = lambda n: (n / 16 + 64) * U
+    q = q.view(B, N, Hk, G, 2, D).permute(0, 2, 3, 4, 1, 5)                        # [B, Hk, G, 2, N, D]
+    k = k.permute(0, 2, 3, 1, 4).unsqueeze(2)                                      # [B, Hk, 1, 2, M, D]
+    keep = see.any(1)[:, None, None, :, None]
+    k, v = k.where(keep[:, :, :, None], torch.zeros((), dtype=torch.float64, device=k.device)), v.permute(0, 2, 1, 3).unsqueeze(2).where(keep, torch.zeros((), dtype=torch.float64, device=v.device))
+    lam = lam.view(Hk, G, 1, 1)
+    s = torch.matmul(q, k.transpose(-1, -2)) * scale
+    es = torch.matmul(q.abs(), k.abs().transpose(-1, -2)) * scale * (D + 8) * U
+    ok = see[:, None, None, None]
+    s = s.masked_fill(~ok, -float('inf'))
+    top = s.amax(-1, keepdim=True)
+    top = torch.where(top == -float('inf'), torch.zeros_like(top), top)
+    p = torch.exp(s - top)
+    tot = p.sum(-1, keepdim=True)
+    p = p / torch.where(tot == 0, torch.ones_like(tot), tot)
+    es = torch.where(ok, es + 4 * U * (1 + s.abs()), torch.zeros_like(s))
+    ep = p * (es + (p * es).sum(-1, keepdim=True) + chain(M)) + 2.0 ** -126 * ok   # error of p, unrounded
+    o = torch.matmul(p, v.unsqueeze(3))                                            # [B, Hk, G, 2, N, 2D]
+    va = v.abs().unsqueeze(3)
+    eo = torch.matmul(ep + p * (inner + chain(M)) + tiny * ok, va)
+    out = o[:, :, :, 0] - lam * o[:, :, :, 1]
+    e = eo[:, :, :, 0] + lam.abs() * eo[:, :, :, 1]
+    back = lambda t: t.permute(0, 3, 1, 2, 4).reshape(B, N, H, -1)
+    room = 1e-300 + (6e-8 if dtype == torch.float16 else 0.0)
+    done = lambda t, err: (t, half * t.abs() + err * (1 + half) + room)
+    res = {'out': done(back(out), back(e))}
+    if dout is None:
+        return res
+    do = dout.detach().double().view(B, N, Hk, G, 2 * D).permute(0, 2, 3, 1, 4)    # [B, Hk, G, N, 2D]
+    g = torch.matmul(do, v.transpose(-1, -2))
+    eg = torch.matmul(do.abs(), v.abs().transpose(-1, -2)) * chain(2 * D)
+    delta = (do.unsqueeze(3) * o).sum(-1, keepdim=True)
+    ed = (do.abs().unsqueeze(3) * (eo + o.abs() * chain(2 * D))).sum(-1, keepdim=True)
+    sign = torch.stack([torch.ones_like(lam), -lam], 2)                            # [Hk, G, 2, 1, 1]
+    ds = sign * p * (g.unsqueeze(3) - delta)
+    eds = sign.abs() * (p * (eg.unsqueeze(3) + ed) + ep * (g.unsqueeze(3) - delta).abs())
+    eds = eds + inner * ds.abs() + 4 * U * ds.abs() + tiny * ok
+    dq = scale * torch.matmul(ds, k)
+    edq = scale * torch.matmul(eds + chain(M) * ds.abs(), k.abs())
+    dk = scale * torch.matmul(ds.transpose(-1, -2), q).sum(2)                      # [B, Hk, 2, M, D]
+    edk = scale * torch.matmul((eds + chain(N * G) * ds.abs()).transpose(-1, -2), q.abs()).sum(2)
+    pc = p[:, :, :, 0] - lam * p[:, :, :, 1]
+    epc = ep[:, :, :, 0] + lam.abs() * ep[:, :, :, 1] + (inner + 2 * U) * pc.abs() + 2 * U * p.sum(3) + tiny * ok[:, :, :, 0]
+    dv = torch.matmul(pc.transpose(-1, -2), do).sum(2)
+    edv = torch.matmul((epc + chain(N * G) * pc.abs()).transpose(-1, -2), do.abs()).sum(2)
+    t = p[:, :, :, 1] * g
+    dlam = -t.sum((0, 3, 4)).reshape(H)
+    edl = (ep[:, :, :, 1] * g.abs() + p[:, :, :, 1] * eg + chain(M + B * N) * t.abs()).sum((0, 3, 4)).reshape(H)
+    res['q'] = done(dq.permute(0, 4, 1, 2, 3, 5).reshape(B, N, H, 2, D), edq.permute(0, 4, 1, 2, 3, 5).reshape(B, N, H, 2, D))
+    res['k'] = done(dk.permute(0, 3, 1, 2, 4), edk.permute(0, 3, 1, 2, 4))
+    res['v'] = done(dv.permute(0, 2, 1, 3), edv.permute(0, 2, 1, 3))
+    res['lam'] = (dlam, edl)
+    return res
+
+
+def may_see(B, N, M, causal, mask=None, lengths=None, device='cuda'):
+    i, j = torch.arange(N, device=device).view(1, N, 1), torch.arange(M, device=device).view(1, 1, M)
+    end = torch.full((B, 1, 1), M, device=device) if lengths is None else lengths.clamp(0, M).view(B, 1, 1).long()
+    see = (j < end).expand(B, N, M)
+    if causal:
+        see = see & (j <= i + end - N)
+    return see if mask is None else see & mask[:, None]
