@@ -13,9 +13,10 @@ from ._token import alike, dtype_code, on_device, on_gpu, ptr, require
 
 
 def _aligned(t):
-    """A tensor whose last axis is side by side and whose rows start at multiples of 16 bytes: t itself where it is one."""
+    """A tensor whose last axis is side by side and whose rows start at multiples of 16 bytes, with tokens and maps at most 2^22 values apart: t itself where it is one."""
     per = 16 // t.element_size()
-    if t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(s % per == 0 or n == 1 for s, n in zip(t.stride()[:-1], t.shape[:-1])):
+    if t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(s % per == 0 or n == 1 for s, n in zip(t.stride()[:-1], t.shape[:-1])) and \
+            all(t.stride(i) <= 1 << 22 for i in (1, 3) if i < t.dim() - 1 and t.shape[i] > 1):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()

@@ -73,19 +73,28 @@ struct Tile {
       return v;
     }
   }
-  // rows [r0, r0 + R) of a strided matrix into the tile, without registers; rows from `end` on repeat the last one (they are masked).  Two halves of
-  // D values, `sm` apart.
+  // Brings R rows of a strided matrix (two halves of D values, `sm` apart) into a tile, without registers.  What a lane fetches in a tile is fixed: step i of its wave
+  // is row `row(i)`, value `val(i)`; only the uniform base moves from tile to tile.
   template <int R, int NW>
-  static __device__ __forceinline__ void load(char* t, const T* src, long long sn, long long sm, int r0, int end, int wave, int lane) {
-    static_assert(R * kChunks % 64 == 0, "whole waves");
-#pragma unroll
-    for (int i = wave; i < R * kChunks / 64; i += NW) {
-      const int slot = i * 64 + lane, r = slot / kChunks, c = (slot % kChunks) ^ turn(r), e = c * kPer;
-      const int g = r0 + r < end ? r0 + r : end - 1;
-      const T* p = src + g * sn + (e >= D ? sm : 0) + (e % D);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)(t + i * 1024), 16, 0, 0);
+  struct Loader {
+    static constexpr int kSteps = R * kChunks / 64 / NW, kRowsPer = 64 * NW / kChunks;   // rows between a lane's steps
+    static_assert(R * kChunks % (64 * NW) == 0 && kRowsPer * kChunks == 64 * NW, "whole waves, whole rows");
+    int row0, sn, sm;
+    __device__ Loader(long long sn_, long long sm_, int tid) : row0(tid / kChunks), sn((int)sn_), sm((int)sm_) {}
+    __device__ __forceinline__ int val(int i, int tid) const {
+      const int e = ((tid % kChunks) ^ turn(row0 + i * kRowsPer)) * kPer;
+      return e >= D ? e - D + sm : e;
     }
-  }
+    // base: the tile's first row; rows from `rows` on repeat the last one (they are masked)
+    __device__ __forceinline__ void operator()(char* t, const T* base, int rows, int tid, int wave) const {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int r = row0 + i * kRowsPer, g = min(r, rows - 1);
+        const char* p = (const char*)base + (unsigned)((g * sn + val(i, tid)) * (int)sizeof(T));
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)(t + (i * NW + wave) * 1024), 16, 0, 0);
+      }
+    }
+  };
   // rows whose bit is not set in `keep` are set to zero
   template <int R, int THREADS>
   static __device__ __forceinline__ void clear(char* t, unsigned long long keep, int tid) {
@@ -172,110 +181,167 @@ __device__ __forceinline__ unsigned long long keys_seen(const unsigned char* mas
   return __ballot(in);
 }
 
+// Bit row_of(i, 0): whether value i of a lane, key row_of(i, h) of its block, counts for a row whose last key is `last` keys behind the block's first
+__device__ __forceinline__ unsigned keys_of_lane(unsigned seen32, int last, int h) {
+  const unsigned upto = last >= 31 ? ~0u : last < 0 ? 0u : (2u << last) - 1;
+  return (seen32 & upto) >> (4 * h);
+}
+
 // ---------------------------------------------------------------------------------------------------------------- forward
+// MPW: maps of a wave.  Up to D = 64 a wave keeps the sums of both maps of its 32 rows (128 registers), and every fragment of v serves two products.  At
+// D = 128 two waves share 32 rows, one map each, and meet at the end.
 template <typename T, int D, int NW> struct FwdShape {
-  static constexpr int KT = sizeof(T) == 4 || D == 128 || NW == 1 ? 32 : 64;  // keys of a tile: two tiles of k and v in at most 128 KB
+  static constexpr int MPW = D == 128 && NW > 1 ? 1 : 2;
+  static constexpr int KT = 32;                                                // keys of a block
 };
 
+// Scores of a block: S^T of MPW maps
+template <typename T, int D, int MPW>
+__device__ __forceinline__ void scores(f32x16 (&s)[MPW], const char* kt, const typename Frag8<T>::type (&qf)[MPW][D / 16], int map0, int lane) {
+#pragma unroll
+  for (int m = 0; m < MPW; ++m) s[m] = zero16();
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+    for (int m = 0; m < MPW; ++m) s[m] = mma(Tile<T, D>::row(kt, lane & 31, (map0 + m) * D + 16 * i + 8 * (lane >> 5)), qf[m][i], s[m]);
+}
+
+__device__ __forceinline__ float top_of(const f32x16& s) {
+  float t = s[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) t = fmaxf(t, s[i]);
+  return t;
+}
+__device__ __forceinline__ float with_other_half(float t) {                    // the larger of lane and lane ^ 32
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(t), __float_as_uint(t), false, false);
+  return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+
+// One pass over the keys in blocks of 32, three blocks in work at a time: while block j goes through its exponentials, the matrix pipe forms the scores of
+// block j + 1 and adds block j - 1 times its values.  None of the three waits for another, and they stand in one stretch of code without a branch, so that a
+// wave by itself keeps both pipes busy (measured on this card: 24 products of 32x32x16, 96 FMAs and 32 exponentials take 471 ns side by side, 386 + 312 one
+// after the other); masks and a new maximum are dealt with in front of it.
+#define PGRF_DA_WEAVE_FWD
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, 1) void diff_attn_fwd(DiffArgs a) {
+__global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_fwd(DiffArgs a) {
   using TL = Tile<T, D>;
   using F = typename Frag8<T>::type;
-  constexpr int KT = FwdShape<T, D, NW>::KT, NK = D / 16, NC = 2 * D / 32;
-  constexpr unsigned long long kAll = KT == 64 ? ~0ull : (1ull << KT) - 1;
-  __shared__ __attribute__((aligned(16))) char kt[2][KT * TL::kRow];
-  __shared__ __attribute__((aligned(16))) char vt[2][KT * TL::kRow];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int rows = a.N * a.G, tiles = (rows + NW * 32 - 1) / (NW * 32);
+  using Sh = FwdShape<T, D, NW>;
+  constexpr int KT = Sh::KT, MPW = Sh::MPW, NK = D / 16, NC = 2 * D / 32, RW = NW * MPW / 2;   // RW: groups of 32 rows in the workgroup
+  constexpr int kTile = KT * TL::kRow;
+  __shared__ __attribute__((aligned(16))) char tiles_lds[4 * kTile];             // two blocks of k, two of v
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int group = MPW == 2 ? wave : wave >> 1, map0 = MPW == 2 ? 0 : wave & 1;
+  const int rows = a.N * a.G, tiles = (rows + RW * 32 - 1) / (RW * 32);
   unsigned id = by_xcd(blockIdx.x, gridDim.x);
   const int split = id % a.splits;
   id /= a.splits;
   const int tile = tiles - 1 - (int)(id % tiles);                              // (causal: the longest rows first)
   const int bh = id / tiles, b = bh / a.Hk, hk = bh % a.Hk;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.M) : a.M;
-  const int r0 = (tile * NW + wave) * 32, r = r0 + (lane & 31), rc = min(r, rows - 1);
+  const int r0 = (tile * RW + group) * 32, r = r0 + (lane & 31), rc = min(r, rows - 1);
   const int n = rc / a.G, head = hk * a.G + rc % a.G;
-  // the last key a row sees, of the first and of the last row of the wave, and of the workgroup's last row
+  // the last key a row sees, of the wave's first row, and of the workgroup's last row
   const int off = len - a.N;
   const int lim = r >= rows ? -1 : a.causal ? min(n + off, len - 1) : len - 1;
   const int lim_lo = r0 + 31 >= rows ? -1 : a.causal ? min(r0 / a.G + off, len - 1) : len - 1;
-  const int lim_hi = r0 >= rows ? -1 : a.causal ? min(min(r0 + 31, rows - 1) / a.G + off, len - 1) : len - 1;
-  const int wg_hi = a.causal ? min(min((tile + 1) * NW * 32 - 1, rows - 1) / a.G + off, len - 1) : len - 1;
+  const int wg_hi = a.causal ? min(min((tile + 1) * RW * 32 - 1, rows - 1) / a.G + off, len - 1) : len - 1;
   const int all = (wg_hi + KT) / KT, per = (max(all, 0) + a.splits - 1) / a.splits;
   const int t0 = split * per, t1 = min(all, t0 + per);
 
-  const T* q = (const T*)a.q + b * a.q_sb + n * a.q_sn + head * a.q_sh + 8 * h;
-  F qf[2][NK];
+  const T* q = (const T*)a.q + b * a.q_sb + n * a.q_sn + head * a.q_sh + map0 * a.q_sm + 8 * h;
+  F qf[MPW][NK];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int m = 0; m < MPW; ++m)
 #pragma unroll
     for (int s = 0; s < NK; ++s) qf[m][s] = load8<T>(q + m * a.q_sm + 16 * s);
 
   const T* k = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
   const T* v = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
   const unsigned char* mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+  const typename TL::template Loader<KT, NW> lk(a.k_sn, a.k_sm, tid), lv(a.v_sn, D, tid);
+  auto ktile = [&](int t) { return tiles_lds + (t & 1) * kTile; };
+  auto vtile = [&](int t) { return tiles_lds + 2 * kTile + (t & 1) * kTile; };
+  auto fetch_k = [&](int t) { lk(ktile(t), k + (long long)t * KT * a.k_sn, len - t * KT, tid, wave); };
+  auto fetch_v = [&](int t) { lv(vtile(t), v + (long long)t * KT * a.v_sn, len - t * KT, tid, wave); };
 
-  f32x16 o[2][NC];
-  float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  f32x16 o[MPW][NC], s[MPW];
+  F p[MPW][2];
+  float mx[MPW], l[MPW], top[MPW];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int m = 0; m < MPW; ++m) {
+    mx[m] = -INFINITY;
+    l[m] = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) o[m][c] = zero16();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[m][i][j] = (T)0.f;
+  }
+  auto add_block = [&](const char* vt) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const F vf = TL::col(vt, 16 * i, 32 * c, lane);
+#pragma unroll
+        for (int m = 0; m < MPW; ++m) o[m][c] = mma(vf, p[m][i], o[m][c]);
+      }
+  };
 
   if (t0 < t1) {
-    TL::template load<KT, NW>(kt[0], k, a.k_sn, a.k_sm, t0 * KT, len, wave, lane);
-    TL::template load<KT, NW>(vt[0], v, a.v_sn, D, t0 * KT, len, wave, lane);
-  }
-  for (int t = t0; t < t1; ++t) {
-    const int cur = (t - t0) & 1, k0 = t * KT;
-    const unsigned long long seen = keys_seen<KT>(mask, k0, len, lane);
-    __syncthreads();                                                           // tile t has come; nobody reads the other buffer any more
-    if (t + 1 < t1) {
-      TL::template load<KT, NW>(kt[cur ^ 1], k, a.k_sn, a.k_sm, k0 + KT, len, wave, lane);
-      TL::template load<KT, NW>(vt[cur ^ 1], v, a.v_sn, D, k0 + KT, len, wave, lane);
-    }
-    if (seen == 0) continue;
-    if (seen != kAll) {                                                        // what stands in masked values may be anything, and 0 * NaN is NaN
-      TL::template clear<KT, NW * 64>(vt[cur], seen, threadIdx.x);
-      __syncthreads();
-    }
-    if (lim_hi < k0) continue;
+    fetch_k(t0);
+    for (int i = tid; i < kTile / 16; i += NW * 64) *(float4*)(vtile(t0 - 1) + i * 16) = make_float4(0.f, 0.f, 0.f, 0.f);   // (its probabilities are 0)
+    unsigned seen = ~0u;
+    __syncthreads();
+    if (t0 + 1 < t1) fetch_k(t0 + 1);
+    scores<T, D, MPW>(s, ktile(t0), qf, map0, lane);
 #pragma unroll
-    for (int kb = 0; kb < KT; kb += 32) {
-      if (lim_hi < k0 + kb) break;
-      const unsigned seen32 = (unsigned)(seen >> kb);
-      f32x16 s[2];
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        s[m] = zero16();
-#pragma unroll
-        for (int i = 0; i < NK; ++i) s[m] = mma(TL::row(kt[cur], kb + (lane & 31), m * D + 16 * i + 8 * h), qf[m][i], s[m]);
+    for (int m = 0; m < MPW; ++m) top[m] = top_of(s[m]);
+    for (int t = t0; t < t1; ++t) {
+      const int k0 = t * KT;
+      const unsigned before = seen;
+      seen = ~0u;
+      if (mask || k0 + KT > len) seen = (unsigned)keys_seen<KT>(mask, k0, len, lane);
+      __syncthreads();                                                         // k of t + 1 and v of t - 1 have come; nobody reads k of t or v of t - 2 any more
+      if (t + 2 < t1) fetch_k(t + 2);
+      if (before != ~0u) {                                                     // what stands in masked values may be anything, and 0 * NaN is NaN
+        TL::template clear<KT, NW * 64>(vtile(t - 1), before, tid);
+        __syncthreads();
       }
-      if (seen32 != ~0u || k0 + kb + 31 > lim_lo) {
+      fetch_v(t);
+      if (seen != ~0u || k0 + 31 > lim_lo) {
+        const unsigned ok = keys_of_lane(seen, lim - k0, h);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = row_of(i, h);
-          const bool ok = ((seen32 >> key) & 1) && k0 + kb + key <= lim;
-          s[0][i] = ok ? s[0][i] : -INFINITY;
-          s[1][i] = ok ? s[1][i] : -INFINITY;
+        for (int m = 0; m < MPW; ++m) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[m][i] = (ok >> row_of(i, 0)) & 1 ? s[m][i] : -INFINITY;
+          top[m] = top_of(s[m]);
         }
       }
+      // The running maximum follows only where a row outgrew it by 2^8, and by a whole power of two: sums and values stay in range, and what was rounded before
+      // scales without another rounding
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        float top = s[m][0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[m][i]);
-        top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c;
-        // the running maximum follows only where a row outgrew it by 2^8: sums and values stay in range, and the result does not change
-        if (__any(top > mx[m] + 8.f)) {
-          const float now = fmaxf(mx[m], top), f = now == -INFINITY ? 1.f : exp2f(mx[m] - now);
-          mx[m] = now;
+      for (int m = 0; m < MPW; ++m) {
+        const float up = with_other_half(top[m]) * a.c;
+        if (__any(up > mx[m] + 8.f)) {
+          const float grow = fmaxf(ceilf(up - mx[m]), 0.f), f = mx[m] == -INFINITY ? 1.f : ldexpf(1.f, -(int)fminf(grow, 1000.f));
+          mx[m] = mx[m] == -INFINITY ? up : mx[m] + grow;
           l[m] *= f;
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
+          for (int c = 0; c < NC; ++c) o[m][c] *= f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[m][c][i] *= f;
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[m][i][j] = (T)((float)p[m][i][j] * f);
         }
+      }
+      f32x16 next[MPW];
+      scores<T, D, MPW>(next, ktile(t + 1), qf, map0, lane);                   // (behind the last block: of whatever stands there, and unused)
+      add_block(vtile(t - 1));
+#pragma unroll
+      for (int m = 0; m < MPW; ++m) {
         const float base = mx[m] == -INFINITY ? 0.f : mx[m];
         float sum = 0.f;
 #pragma unroll
@@ -284,56 +350,90 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_fwd(DiffArgs a) {
           sum += s[m][i];
         }
         l[m] += sum;
-      }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const F p0 = pack<T>(s[0], i), p1 = pack<T>(s[1], i);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const F vf = TL::col(vt[cur], kb + 16 * i, 32 * c, lane);
-          o[0][c] = mma(vf, p0, o[0][c]);
-          o[1][c] = mma(vf, p1, o[1][c]);
-        }
+        for (int i = 0; i < 2; ++i) p[m][i] = pack<T>(s[m], i);
+        s[m] = next[m];
+        top[m] = top_of(s[m]);
       }
+      PGRF_DA_WEAVE_FWD
     }
+    __syncthreads();
+    if (seen != ~0u) {
+      TL::template clear<KT, NW * 64>(vtile(t1 - 1), seen, tid);
+      __syncthreads();
+    }
+    add_block(vtile(t1 - 1));
   }
 #pragma unroll
-  for (int m = 0; m < 2; ++m) l[m] += __shfl_xor(l[m], 32, 64);
-  if (r >= rows) return;
+  for (int m = 0; m < MPW; ++m) l[m] += __shfl_xor(l[m], 32, 64);
+  const bool live = r < rows;
   if (a.splits > 1) {
+    if (!live) return;
     const long long at = ((long long)split * a.B * a.Hk + bh) * rows + r;
-    float* po = a.part_o + at * 4 * D;
+    float* po = a.part_o + at * 4 * D + map0 * 2 * D + 4 * h;
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < MPW; ++m) {
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          store4<float>(po + m * 2 * D + 32 * c + 8 * g + 4 * h, o[m][c][4 * g], o[m][c][4 * g + 1], o[m][c][4 * g + 2], o[m][c][4 * g + 3]);
-    if (h == 0) *(float4*)(a.part_ml + at * 4) = make_float4(mx[0], l[0], mx[1], l[1]);
+          store4<float>(po + m * 2 * D + 32 * c + 8 * g, o[m][c][4 * g], o[m][c][4 * g + 1], o[m][c][4 * g + 2], o[m][c][4 * g + 3]);
+      if (h == 0) *(float2*)(a.part_ml + at * 4 + 2 * (map0 + m)) = make_float2(mx[m], l[m]);
+    }
     return;
   }
-  const float lam = lam_of<T>(a, head), i0 = l[0] > 0.f ? 1.f / l[0] : l[0], i1 = l[1] > 0.f ? 1.f / l[1] : l[1];   // (a NaN stays one)
+  const float lam = lam_of<T>(a, head);
   const long long at = ((long long)b * a.N + n) * a.H + head;
-  T* out = (T*)a.out + at * 2 * D + 4 * h;
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
+  for (int m = 0; m < MPW; ++m) {
+    const float inv = l[m] > 0.f ? 1.f / l[m] : l[m];                          // (a NaN stays one)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      float u[4], w[4];
+    for (int c = 0; c < NC; ++c) o[m][c] *= inv;
+    if (a.o12 && live) {
+      float* oo = a.o12 + at * 4 * D + (map0 + m) * 2 * D + 4 * h;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) { u[j] = o[0][c][4 * g + j] * i0; w[j] = o[1][c][4 * g + j] * i1; }
-      store4<T>(out + 32 * c + 8 * g, u[0] - lam * w[0], u[1] - lam * w[1], u[2] - lam * w[2], u[3] - lam * w[3]);
-      if (a.o12) {
-        float* oo = a.o12 + at * 4 * D + 4 * h + 32 * c + 8 * g;
-        store4<float>(oo, u[0], u[1], u[2], u[3]);
-        store4<float>(oo + 2 * D, w[0], w[1], w[2], w[3]);
-      }
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) store4<float>(oo + 32 * c + 8 * g, o[m][c][4 * g], o[m][c][4 * g + 1], o[m][c][4 * g + 2], o[m][c][4 * g + 3]);
+      if (h == 0) a.lse[(((long long)b * a.H + head) * 2 + map0 + m) * a.N + n] = l[m] == 0.f ? INFINITY : mx[m] + log2f(l[m]);
     }
-  if (a.lse && h == 0) {
-    float* e = a.lse + ((long long)b * a.H + head) * 2 * a.N + n;
-    e[0] = l[0] == 0.f ? INFINITY : mx[0] + log2f(l[0]);
-    e[a.N] = l[1] == 0.f ? INFINITY : mx[1] + log2f(l[1]);
+  }
+  T* out = (T*)a.out + at * 2 * D + 4 * h;
+  if constexpr (MPW == 1) {
+    // the second map's waves hand their values over through LDS, as many column blocks at a time as the tiles' room holds
+    constexpr int kFit = 4 * kTile / (RW * 64 * 64), kAt = kFit < NC ? kFit : NC;
+    static_assert(kAt >= 1 && NC % kAt == 0, "");
+    float* room = (float*)tiles_lds + group * kAt * 16 * 64 + lane;
+    for (int c0 = 0; c0 < NC; c0 += kAt) {
+      __syncthreads();                                                         // (also: the tiles are read)
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (map0 == 1 && c >= c0 && c < c0 + kAt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) room[((c - c0) * 16 + i) * 64] = o[0][c][i];
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (map0 == 0 && live && c >= c0 && c < c0 + kAt)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float u[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j] = o[0][c][4 * g + j] - lam * room[((c - c0) * 16 + 4 * g + j) * 64];
+            store4<T>(out + 32 * c + 8 * g, u[0], u[1], u[2], u[3]);
+          }
+    }
+  } else {
+    if (!live) return;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = o[0][c][4 * g + j] - lam * o[MPW - 1][c][4 * g + j];
+        store4<T>(out + 32 * c + 8 * g, u[0], u[1], u[2], u[3]);
+      }
   }
 }
 
@@ -390,7 +490,7 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_dq(DiffArgs a) {
   constexpr unsigned long long kAll = (1ull << KT) - 1;
   __shared__ __attribute__((aligned(16))) char kt[2][KT * TL::kRow];
   __shared__ __attribute__((aligned(16))) char vt[2][KT * TL::kRow];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int rows = a.N * a.G, tiles = (rows + NW * 32 - 1) / (NW * 32);
   const unsigned id = by_xcd(blockIdx.x, gridDim.x);
   const int tile = tiles - 1 - (int)(id % tiles);
@@ -440,18 +540,18 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_dq(DiffArgs a) {
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int c = 0; c < NC; ++c) dq[m][c] = zero16();
-  if (t1 > 0) {
-    TL::template load<KT, NW>(kt[0], k, a.k_sn, a.k_sm, 0, len, wave, lane);
-    TL::template load<KT, NW>(vt[0], v, a.v_sn, D, 0, len, wave, lane);
-  }
+  const typename TL::template Loader<KT, NW> lk(a.k_sn, a.k_sm, threadIdx.x), lv(a.v_sn, D, threadIdx.x);
+  auto fetch = [&](int t, int buf) {
+    lk(kt[buf], k + (long long)t * KT * a.k_sn, len - t * KT, threadIdx.x, wave);
+    lv(vt[buf], v + (long long)t * KT * a.v_sn, len - t * KT, threadIdx.x, wave);
+  };
+  if (t1 > 0) fetch(0, 0);
   for (int t = 0; t < t1; ++t) {
     const int cur = t & 1, k0 = t * KT;
-    const unsigned long long seen = keys_seen<KT>(mask, k0, len, lane);
+    unsigned long long seen = kAll;
+    if (mask || k0 + KT > len) seen = keys_seen<KT>(mask, k0, len, lane);
     __syncthreads();
-    if (t + 1 < t1) {
-      TL::template load<KT, NW>(kt[cur ^ 1], k, a.k_sn, a.k_sm, k0 + KT, len, wave, lane);
-      TL::template load<KT, NW>(vt[cur ^ 1], v, a.v_sn, D, k0 + KT, len, wave, lane);
-    }
+    if (t + 1 < t1) fetch(t + 1, cur ^ 1);
     if (seen == 0) continue;
     if (seen != kAll) {
       TL::template clear<KT, NW * 64>(kt[cur], seen, threadIdx.x);
@@ -469,14 +569,13 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_dq(DiffArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) g = mma(TL::row(vt[cur], lane & 31, 16 * i + 8 * h), gf[i], g);
     const bool part = (unsigned)seen != ~0u || k0 + 31 > lim_lo;
+    const unsigned ok = part ? keys_of_lane((unsigned)seen, lim - k0, h) : 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float p0 = __builtin_amdgcn_exp2f(fmaf(s[0][i], a.c, -lse[0])), p1 = __builtin_amdgcn_exp2f(fmaf(s[1][i], a.c, -lse[1]));
       if (part) {
-        const int key = row_of(i, h);
-        const bool ok = (((unsigned)seen >> key) & 1) && k0 + key <= lim;
-        p0 = ok ? p0 : 0.f;
-        p1 = ok ? p1 : 0.f;
+        p0 = (ok >> row_of(i, 0)) & 1 ? p0 : 0.f;
+        p1 = (ok >> row_of(i, 0)) & 1 ? p1 : 0.f;
       }
       dlam = fmaf(p1, g[i], dlam);
       s[0][i] = p0 * (g[i] - delta[0]);
@@ -514,7 +613,7 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_dkv(DiffArgs a) {
   __shared__ __attribute__((aligned(16))) char qt[2][QT * TL::kRow];
   __shared__ __attribute__((aligned(16))) char gt[2][QT * TL::kRow];
   __shared__ __attribute__((aligned(16))) float stat[2][4][QT];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int tiles = (a.M + NW * 32 - 1) / (NW * 32);
   const unsigned id = by_xcd(blockIdx.x, gridDim.x);
   const int tile = (int)(id % tiles), bh = id / tiles, b = bh / a.Hk, hk = bh % a.Hk;
@@ -540,10 +639,11 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_dkv(DiffArgs a) {
 
   // queries that see the workgroup's first key, in tiles, of each head that shares it
   const int first = a.causal ? max(0, tile * NW * 32 - off) / QT : 0, nq = (a.N + QT - 1) / QT - first, total = max(nq, 0) * a.G;
+  const typename TL::template Loader<QT, NW> lq(a.q_sn, a.q_sm, threadIdx.x), lg((long long)a.H * 2 * D, D, threadIdx.x);
   auto fetch = [&](int i, int buf) {
     const int head = hk * a.G + i / nq, n0 = (first + i % nq) * QT;
-    TL::template load<QT, NW>(qt[buf], (const T*)a.q + b * a.q_sb + head * a.q_sh, a.q_sn, a.q_sm, n0, a.N, wave, lane);
-    TL::template load<QT, NW>(gt[buf], (const T*)a.dout + ((long long)b * a.N * a.H + head) * 2 * D, (long long)a.H * 2 * D, D, n0, a.N, wave, lane);
+    lq(qt[buf], (const T*)a.q + b * a.q_sb + head * a.q_sh + n0 * a.q_sn, a.N - n0, threadIdx.x, wave);
+    lg(gt[buf], (const T*)a.dout + (((long long)b * a.N + n0) * a.H + head) * 2 * D, a.N - n0, threadIdx.x, wave);
     const long long st = ((long long)b * a.H + head) * 2 * a.N;
     for (int w = wave; w < 2; w += NW) {                                        // lse of both maps, then delta of both: 32 values each
       const float* src = (w == 0 ? a.lse : a.delta) + st + (long long)h * a.N + min(n0 + (lane & 31), a.N - 1);

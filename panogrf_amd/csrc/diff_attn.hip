@@ -13,17 +13,23 @@ PGRF_DA_ALL(PGRF_DA_DECL)
 
 static int waves_for(long long rows) { return rows > 64 ? 4 : rows > 32 ? 2 : 1; }
 
-// The key axis is cut where the rows alone leave the chip idle: a share is at least 128 keys, and there are about as many workgroups as the chip holds at a time
-// (one of four waves per CU, five of a single wave, whose two buffers take 32 KB)
-static int splits_for(int B, int Hk, long long rows, int M, int* waves) {
-  *waves = waves_for(rows);
-  const long long groups = (long long)B * Hk * ((rows + *waves * 32 - 1) / (*waves * 32));
-  const long long want = *waves == 1 ? 1280 : 512, most = M / 128;
+// The forward kernel's waves and their rows: at D = 128 two waves share 32 rows, except where one wave is all there is
+struct FwdCut { int waves, rows, splits; };
+static FwdCut cut_fwd(int B, int Hk, long long rows, int M, int D) {
+  FwdCut f;
+  f.waves = waves_for(rows);
+  if (D == 128 && f.waves > 1) f.waves *= 2;
+  f.rows = D == 128 && f.waves > 1 ? f.waves * 16 : f.waves * 32;
+  const long long groups = (long long)B * Hk * ((rows + f.rows - 1) / f.rows);
+  // The key axis is cut where the rows alone leave the chip idle: a share is at least 128 keys, and there are about as many workgroups as the chip holds at a time
+  // (two of four waves per CU, five of a single wave, whose two buffers take 32 KB)
+  const long long want = f.waves == 1 ? 1280 : 512, most = M / 128;
   long long s = (want + groups - 1) / groups;
   if (groups * 2 > want) s = 1;
   if (s > most) s = most;
   if (s > 128) s = 128;
-  return s < 1 ? 1 : (int)s;
+  f.splits = s < 1 ? 1 : (int)s;
+  return f;
 }
 
 static int check(const PgrfDiffAttn* p, const char* who, bool backward) {
@@ -43,6 +49,10 @@ static int check(const PgrfDiffAttn* p, const char* who, bool backward) {
   if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) ||
       (p->q_sb | p->q_sn | p->q_sh | p->q_sm | p->k_sb | p->k_sn | p->k_sh | p->k_sm | p->v_sb | p->v_sn | p->v_sh) % per)
     return set_error(PGRF_ERR_ARG, "%s: q, k, v: addresses and strides must be multiples of 16 bytes", who);
+  // (what a tile's lanes add to its base has to fit 32 bits)
+  if (p->q_sn > (1 << 22) || p->q_sm > (1 << 22) || p->k_sn > (1 << 22) || p->k_sm > (1 << 22) || p->v_sn > (1 << 22) || p->q_sn < 0 || p->q_sm < 0 || p->k_sn < 0 || p->k_sm < 0 ||
+      p->v_sn < 0 || (long long)p->H * 2 * p->D > (1 << 22))
+    return set_error(PGRF_ERR_UNSUPPORTED, "%s: a stride between tokens or maps is negative or over 2^22 values", who);
   if (backward && (!p->lse || !p->maps_out)) return set_error(PGRF_ERR_ARG, "%s: null lse / maps_out", who);
   if (backward && p->lengths) return set_error(PGRF_ERR_UNSUPPORTED, "%s: lengths have no backward pass (use key_mask)", who);
   if (!backward && !p->out) return set_error(PGRF_ERR_ARG, "%s: null out", who);
@@ -74,9 +84,8 @@ extern "C" {
 
 size_t pgrf_diff_attention_workspace_bytes(int, int B, int N, int M, int H, int Hk, int D) {
   if (B < 1 || N < 1 || M < 1 || H < 1 || Hk < 1 || H % Hk || D < 1) return 0;
-  int waves;
   const long long rows = (long long)N * (H / Hk);
-  const int s = splits_for(B, Hk, rows, M, &waves);
+  const int s = cut_fwd(B, Hk, rows, M, D).splits;
   return s > 1 ? (size_t)s * B * Hk * rows * (4 * D + 4) * sizeof(float) : 0;
 }
 
@@ -86,9 +95,9 @@ int pgrf_diff_attention(const PgrfDiffAttn* p, void* stream) {
   if (rc) return rc;
   if ((long long)p->B * p->N == 0) return PGRF_OK;
   DiffArgs a = args_of(p);
-  int waves;
   const long long rows = (long long)a.N * a.G;
-  a.splits = splits_for(a.B, a.Hk, rows, a.M, &waves);
+  const FwdCut cut = cut_fwd(a.B, a.Hk, rows, a.M, p->D);
+  a.splits = cut.splits;
   if (a.splits > 1) {
     const size_t need = pgrf_diff_attention_workspace_bytes(p->dtype, p->B, p->N, p->M, p->H, p->Hk, p->D);
     if (!p->workspace || !aligned16(p->workspace) || p->workspace_bytes < need)
@@ -96,10 +105,10 @@ int pgrf_diff_attention(const PgrfDiffAttn* p, void* stream) {
     a.part_o = (float*)p->workspace;
     a.part_ml = a.part_o + (size_t)a.splits * a.B * a.Hk * rows * 4 * p->D;
   }
-  const long long grid = (long long)a.B * a.Hk * ((rows + waves * 32 - 1) / (waves * 32)) * a.splits;
+  const long long grid = (long long)a.B * a.Hk * ((rows + cut.rows - 1) / cut.rows) * a.splits;
   if (grid > 0x7fffffffll) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tiles", who);
 #define PGRF_DA_FWD(T, D_) \
-  if (p->dtype == T && p->D == D_) return launch_da_fwd_##T##_##D_(a, waves, (unsigned)grid, (hipStream_t)stream);
+  if (p->dtype == T && p->D == D_) return launch_da_fwd_##T##_##D_(a, cut.waves, (unsigned)grid, (hipStream_t)stream);
   PGRF_DA_ALL(PGRF_DA_FWD)
   return set_error(PGRF_ERR_UNSUPPORTED, "%s: no kernel", who);
 }

@@ -20,7 +20,8 @@ using DaT = f16;
 int PGRF_DA_NAME(launch_da_fwd)(const DiffArgs& a, int waves, unsigned grid, hipStream_t s) {
   if (waves == 1) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 1>), dim3(grid), dim3(64), 0, s, a);
   else if (waves == 2) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 2>), dim3(grid), dim3(128), 0, s, a);
-  else hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 4>), dim3(grid), dim3(256), 0, s, a);
+  else if (waves == 4) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 4>), dim3(grid), dim3(256), 0, s, a);
+  else if constexpr (PGRF_DA_D == 128) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 8>), dim3(grid), dim3(512), 0, s, a);
   PGRF_TOK_LAUNCHED("pgrf_diff_attention");
   if (a.splits > 1) {
     const long long rows = (long long)a.B * a.Hk * a.N * a.G, per = 256 / (2 * PGRF_DA_D);
