@@ -120,7 +120,7 @@ struct DiffArgs {
   // backward
   const void* dout;               // [B,N,H,2D] contiguous
   float* delta;                   // [B,H,2,N]: dout . o_i
-  float* dlam_rows;               // [B,H,N]
+  float* dlam_part;               // [B*Hk][units][G]: shares of -dlam, by wave of the dq kernel (G a power of two up to 32) or by token
   void *dq, *dk, *dv, *dlam;
 };
 
@@ -173,6 +173,23 @@ __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d)
   store_vec<T, 4>(p, v);
 }
 
+// Products 0 .. N - 1 in this order, the fragment of each read AHEAD products before it, and a share of other work behind each.  Left to itself the compiler reads
+// each fragment right before its product, waits for it, and puts the other work behind all of them; the fences keep it to this order.
+template <typename F, int N, int AHEAD, class Read, class Product, class Work>
+__device__ __forceinline__ void weave(Read read, Product product, Work work) {
+  F f[AHEAD + 1];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) f[i] = read(i);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i + AHEAD < N) f[(i + AHEAD) % (AHEAD + 1)] = read(i + AHEAD);
+    product(i, f[i % (AHEAD + 1)]);
+    work(i);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // Which keys of the R keys from k0 any query may see: bit r = key k0 + r (uniform over the workgroup)
 template <int R>
 __device__ __forceinline__ unsigned long long keys_seen(const unsigned char* mask, int k0, int len, int lane) {
@@ -191,7 +208,8 @@ __device__ __forceinline__ unsigned keys_of_lane(unsigned seen32, int last, int 
 // MPW: maps of a wave.  Up to D = 64 a wave keeps the sums of both maps of its 32 rows (128 registers), and every fragment of v serves two products.  At
 // D = 128 two waves share 32 rows, one map each, and meet at the end.
 template <typename T, int D, int NW> struct FwdShape {
-  static constexpr int MPW = D == 128 && NW > 1 ? 1 : 2;
+  static_assert(D < 128 || NW > 1, "a pair of waves at D = 128");
+  static constexpr int MPW = D == 128 ? 1 : 2;
   static constexpr int KT = 32;                                                // keys of a block
 };
 
@@ -221,7 +239,6 @@ __device__ __forceinline__ float with_other_half(float t) {                    /
 // block j + 1 and adds block j - 1 times its values.  None of the three waits for another, and they stand in one stretch of code without a branch, so that a
 // wave by itself keeps both pipes busy (measured on this card: 24 products of 32x32x16, 96 FMAs and 32 exponentials take 471 ns side by side, 386 + 312 one
 // after the other); masks and a new maximum are dealt with in front of it.
-#define PGRF_DA_WEAVE_FWD
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_fwd(DiffArgs a) {
   using TL = Tile<T, D>;
@@ -338,24 +355,46 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_fwd(DiffArgs 
         }
       }
       f32x16 next[MPW];
-      scores<T, D, MPW>(next, ktile(t + 1), qf, map0, lane);                   // (behind the last block: of whatever stands there, and unused)
-      add_block(vtile(t - 1));
+      const char *kn = ktile(t + 1), *vb = vtile(t - 1);                       // (behind the last block: scores of whatever stands there, unused)
+      float base[MPW], sum[MPW];
+      F pn[MPW][2];
 #pragma unroll
       for (int m = 0; m < MPW; ++m) {
-        const float base = mx[m] == -INFINITY ? 0.f : mx[m];
-        float sum = 0.f;
+        next[m] = zero16();
+        base[m] = mx[m] == -INFINITY ? 0.f : mx[m];
+        sum[m] = 0.f;
+      }
+      constexpr int NS = NK * MPW, NA = 2 * NC, NP = NS + NA;                   // fragments of k, of v; every one of v serves MPW products
+      weave<F, NP, 3>(
+          [&](int i) {
+            return i < NS ? TL::row(kn, lane & 31, (map0 + i % MPW) * D + 16 * (i / MPW) + 8 * h) : TL::col(vb, 16 * ((i - NS) / NC), 32 * ((i - NS) % NC), lane);
+          },
+          [&](int i, const F& f) {
+            if (i < NS) {
+              next[i % MPW] = mma(f, qf[i % MPW][i / MPW], next[i % MPW]);
+            } else {
+              const int c = (i - NS) % NC;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[m][i] = __builtin_amdgcn_exp2f(fmaf(s[m][i], a.c, -base));
-          sum += s[m][i];
-        }
-        l[m] += sum;
+              for (int m = 0; m < MPW; ++m) o[m][c] = mma(f, p[m][(i - NS) / NC], o[m][c]);
+            }
+          },
+          [&](int i) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) p[m][i] = pack<T>(s[m], i);
+            for (int x = 16 * MPW * i / NP; x < 16 * MPW * (i + 1) / NP; ++x) {
+              const int m = x / 16, e = x % 16;
+              const float w = __builtin_amdgcn_exp2f(fmaf(s[m][e], a.c, -base[m]));
+              sum[m] += w;
+              pn[m][e / 8][e % 8] = (T)w;
+            }
+          });
+#pragma unroll
+      for (int m = 0; m < MPW; ++m) {
+        l[m] += sum[m];
+        p[m][0] = pn[m][0];
+        p[m][1] = pn[m][1];
         s[m] = next[m];
         top[m] = top_of(s[m]);
       }
-      PGRF_DA_WEAVE_FWD
     }
     __syncthreads();
     if (seen != ~0u) {
@@ -480,17 +519,29 @@ __global__ __launch_bounds__(256) void diff_attn_join(DiffArgs a) {
 // With G = dout v^T and delta_i = dout . o_i:  dS1 = A1 (G - delta1), dS2 = -lam A2 (G - delta2), dq_i = scale dS_i k_i, dk_i = scale dS_i^T q_i,
 // dv = (A1 - lam A2)^T dout, dlam = -sum A2 G.  A and G are formed again from q, k, v, dout and the saved log sums, twice: once by rows (dq, delta,
 // dlam) and once by keys (dk, dv), 14 instead of 10 products of N M D, so that no two workgroups add to one value and gradients do not depend on scheduling.
-template <typename T, int D> struct BwdShape { static constexpr int KT = 32; };
+//
+// Both kernels weave three blocks as the forward kernel does (scores and G of block j + 1, probabilities of block j, products of block j - 1); float does not, as
+// its products take eight times as long and hide the rest by themselves.
+template <typename T> struct BwdShape {
+  static constexpr bool kWeave = sizeof(T) == 2;
+  static constexpr int kLate = kWeave ? 1 : 0;                                 // blocks between a block's scores and its last use
+};
+
+// Bit row_of(i, 0): whether value i of a lane, row row_of(i, h) of its block, is one of rows lo .. hi
+__device__ __forceinline__ unsigned rows_of_lane(int lo, int hi, int h) {
+  const unsigned upto = hi >= 31 ? ~0u : hi < 0 ? 0u : (2u << hi) - 1, below = lo > 31 ? ~0u : lo <= 0 ? 0u : (1u << lo) - 1;
+  return (upto & ~below) >> (4 * h);
+}
 
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, 1) void diff_attn_dq(DiffArgs a) {
+__global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dq(DiffArgs a) {
   using TL = Tile<T, D>;
   using F = typename Frag8<T>::type;
-  constexpr int KT = BwdShape<T, D>::KT, NK = D / 16, NV = 2 * D / 16, NC = D / 32;
-  constexpr unsigned long long kAll = (1ull << KT) - 1;
-  __shared__ __attribute__((aligned(16))) char kt[2][KT * TL::kRow];
-  __shared__ __attribute__((aligned(16))) char vt[2][KT * TL::kRow];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  constexpr bool kWeave = BwdShape<T>::kWeave;
+  constexpr int KT = 32, NK = D / 16, NV = 2 * D / 16, NC = D / 32, KR = kWeave ? 4 : 2;   // KR: blocks of k in LDS
+  constexpr int kTile = KT * TL::kRow;
+  __shared__ __attribute__((aligned(16))) char tiles_lds[(KR + 2) * kTile];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int rows = a.N * a.G, tiles = (rows + NW * 32 - 1) / (NW * 32);
   const unsigned id = by_xcd(blockIdx.x, gridDim.x);
   const int tile = tiles - 1 - (int)(id % tiles);
@@ -501,7 +552,6 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_dq(DiffArgs a) {
   const int off = len - a.N;
   const int lim = r >= rows ? -1 : a.causal ? min(n + off, len - 1) : len - 1;
   const int lim_lo = r0 + 31 >= rows ? -1 : a.causal ? min(r0 / a.G + off, len - 1) : len - 1;
-  const int lim_hi = r0 >= rows ? -1 : a.causal ? min(min(r0 + 31, rows - 1) / a.G + off, len - 1) : len - 1;
   const int wg_hi = a.causal ? min(min((tile + 1) * NW * 32 - 1, rows - 1) / a.G + off, len - 1) : len - 1;
   const int t1 = max((wg_hi + KT) / KT, 0);
   const long long at = ((long long)b * a.N + n) * a.H + head;
@@ -522,98 +572,182 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_dq(DiffArgs a) {
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
 #pragma unroll
-      for (int s = 0; s < NV; ++s)
+      for (int s = 0; s < NV; ++s) {
+        const Frag8<float>::type e = load8<float>(oo + m * 2 * D + 16 * s);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) delta[m] = fmaf((float)gf[s][j], oo[m * 2 * D + 16 * s + j], delta[m]);
+        for (int j = 0; j < 8; ++j) delta[m] = fmaf((float)gf[s][j], e[j], delta[m]);
+      }
       delta[m] += __shfl_xor(delta[m], 32, 64);
       lse[m] = a.lse[st + m * a.N];
       if (h == 0 && r < rows) a.delta[st + m * a.N] = delta[m];
     }
   }
-  const float lam = lam_of<T>(a, head);
   const T* k = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
   const T* v = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
   const unsigned char* mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
-  f32x16 dq[2][NC];
+  f32x16 dq[2][NC], s[2], g;
+  F ds[2][2];
   float dlam = 0.f;
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int m = 0; m < 2; ++m) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) dq[m][c] = zero16();
-  const typename TL::template Loader<KT, NW> lk(a.k_sn, a.k_sm, threadIdx.x), lv(a.v_sn, D, threadIdx.x);
-  auto fetch = [&](int t, int buf) {
-    lk(kt[buf], k + (long long)t * KT * a.k_sn, len - t * KT, threadIdx.x, wave);
-    lv(vt[buf], v + (long long)t * KT * a.v_sn, len - t * KT, threadIdx.x, wave);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ds[m][i][j] = (T)0.f;
+  }
+  const typename TL::template Loader<KT, NW> lk(a.k_sn, a.k_sm, tid), lv(a.v_sn, D, tid);
+  auto ktile = [&](int t) { return tiles_lds + (t & (KR - 1)) * kTile; };
+  auto vtile = [&](int t) { return tiles_lds + (KR + (t & 1)) * kTile; };
+  auto fetch = [&](int t) {
+    lk(ktile(t), k + (long long)t * KT * a.k_sn, len - t * KT, tid, wave);
+    lv(vtile(t), v + (long long)t * KT * a.v_sn, len - t * KT, tid, wave);
   };
-  if (t1 > 0) fetch(0, 0);
-  for (int t = 0; t < t1; ++t) {
-    const int cur = t & 1, k0 = t * KT;
-    unsigned long long seen = kAll;
-    if (mask || k0 + KT > len) seen = keys_seen<KT>(mask, k0, len, lane);
-    __syncthreads();
-    if (t + 1 < t1) fetch(t + 1, cur ^ 1);
-    if (seen == 0) continue;
-    if (seen != kAll) {
-      TL::template clear<KT, NW * 64>(kt[cur], seen, threadIdx.x);
-      TL::template clear<KT, NW * 64>(vt[cur], seen, threadIdx.x);
-      __syncthreads();
+  auto seen_of = [&](int t) { return mask || t * KT + KT > len ? (unsigned)keys_seen<KT>(mask, t * KT, len, lane) : ~0u; };
+  auto form = [&](f32x16 (&s_)[2], f32x16& g_, int t) {
+    scores<T, D, 2>(s_, ktile(t), qf, 0, lane);
+    g_ = zero16();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) g_ = mma(TL::row(vtile(t), lane & 31, 16 * i + 8 * h), gf[i], g_);
+  };
+  auto hide = [&](unsigned seen, int t) {                                      // masked keys of block t: their probability becomes 0
+    if (seen != ~0u || t * KT + 31 > lim_lo) {
+      const unsigned ok = keys_of_lane(seen, lim - t * KT, h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) s[m][i] = (ok >> row_of(i, 0)) & 1 ? s[m][i] : -INFINITY;
     }
-    if (lim_hi < k0) continue;
-    f32x16 s[2], g = zero16();
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      s[m] = zero16();
-#pragma unroll
-      for (int i = 0; i < NK; ++i) s[m] = mma(TL::row(kt[cur], lane & 31, m * D + 16 * i + 8 * h), qf[m][i], s[m]);
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) g = mma(TL::row(vt[cur], lane & 31, 16 * i + 8 * h), gf[i], g);
-    const bool part = (unsigned)seen != ~0u || k0 + 31 > lim_lo;
-    const unsigned ok = part ? keys_of_lane((unsigned)seen, lim - k0, h) : 0;
+  };
+  auto turn = [&]() {                                                          // scores to score gradients (the second map's without its -lam)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float p0 = __builtin_amdgcn_exp2f(fmaf(s[0][i], a.c, -lse[0])), p1 = __builtin_amdgcn_exp2f(fmaf(s[1][i], a.c, -lse[1]));
-      if (part) {
-        p0 = (ok >> row_of(i, 0)) & 1 ? p0 : 0.f;
-        p1 = (ok >> row_of(i, 0)) & 1 ? p1 : 0.f;
-      }
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[0][i], a.c, -lse[0])), p1 = __builtin_amdgcn_exp2f(fmaf(s[1][i], a.c, -lse[1]));
       dlam = fmaf(p1, g[i], dlam);
       s[0][i] = p0 * (g[i] - delta[0]);
-      s[1][i] = p1 * (g[i] - delta[1]) * -lam;
+      s[1][i] = p1 * (g[i] - delta[1]);
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const F ds = pack<T>(s[m], i);
+      for (int i = 0; i < 2; ++i) ds[m][i] = pack<T>(s[m], i);
+  };
+  auto add = [&](int t) {
 #pragma unroll
-        for (int c = 0; c < NC; ++c) dq[m][c] = mma(TL::col(kt[cur], 16 * i, m * D + 32 * c, lane), ds, dq[m][c]);
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) dq[m][c] = mma(TL::col(ktile(t), 16 * i, m * D + 32 * c, lane), ds[m][i], dq[m][c]);
+  };
+  auto clean = [&](unsigned seen, int t) {                                     // what stands in masked keys may be anything, and 0 * NaN is NaN
+    if (seen != ~0u) {
+      TL::template clear<KT, NW * 64>(ktile(t), seen, tid);
+      TL::template clear<KT, NW * 64>(vtile(t), seen, tid);
+      __syncthreads();
+    }
+  };
+  if (t1 > 0) {
+    fetch(0);
+    unsigned seen = seen_of(0);
+    if constexpr (kWeave)
+      for (int i = tid; i < kTile / 16; i += NW * 64) *(float4*)(ktile(-1) + i * 16) = make_float4(0.f, 0.f, 0.f, 0.f);   // (its score gradients are 0)
+    __syncthreads();
+    if (t1 > 1) fetch(1);
+    clean(seen, 0);
+    if constexpr (kWeave) {
+      form(s, g, 0);
+      for (int t = 0; t < t1; ++t) {
+        const unsigned next = t + 1 < t1 ? seen_of(t + 1) : ~0u;
+        __syncthreads();                                                       // block t + 1 has come; nobody reads k of t - 2 or v of t any more
+        if (t + 2 < t1) fetch(t + 2);
+        clean(next, t + 1);
+        hide(seen, t);
+        f32x16 s2[2] = {zero16(), zero16()}, g2 = zero16();
+        const char *kn = ktile(t + 1), *vn = vtile(t + 1), *kb = ktile(t - 1);   // (behind the last block: whatever stands there, unused)
+        F dn[2][2];
+        constexpr int NS = 2 * NK, NG = NS + NV, NP = NG + 4 * NC;
+        weave<F, NP, 3>(
+            [&](int i) {
+              return i < NS ? TL::row(kn, lane & 31, (i & 1) * D + 16 * (i / 2) + 8 * h) : i < NG ? TL::row(vn, lane & 31, 16 * (i - NS) + 8 * h)
+                                                                                        : TL::col(kb, 16 * ((i - NG) / (2 * NC)), 32 * ((i - NG) % (2 * NC)), lane);
+            },
+            [&](int i, const F& f) {
+              if (i < NS) s2[i & 1] = mma(f, qf[i & 1][i / 2], s2[i & 1]);
+              else if (i < NG) g2 = mma(f, gf[i - NS], g2);
+              else {
+                const int c = (i - NG) % (2 * NC);
+                dq[c / NC][c % NC] = mma(f, ds[c / NC][(i - NG) / (2 * NC)], dq[c / NC][c % NC]);
+              }
+            },
+            [&](int i) {
+#pragma unroll
+              for (int x = 16 * i / NP; x < 16 * (i + 1) / NP; ++x) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[0][x], a.c, -lse[0])), p1 = __builtin_amdgcn_exp2f(fmaf(s[1][x], a.c, -lse[1]));
+                dlam = fmaf(p1, g[x], dlam);
+                dn[0][x / 8][x % 8] = (T)(p0 * (g[x] - delta[0]));
+                dn[1][x / 8][x % 8] = (T)(p1 * (g[x] - delta[1]));
+              }
+            });
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          ds[m][0] = dn[m][0];
+          ds[m][1] = dn[m][1];
+          s[m] = s2[m];
+        }
+        asm volatile("" : "+v"(g2));                                           // (or its products are moved behind the others, to where they are used)
+        g = g2;
+        seen = next;
       }
+      add(t1 - 1);
+    } else {
+      for (int t = 0; t < t1; ++t) {
+        form(s, g, t);
+        hide(seen, t);
+        turn();
+        add(t);
+        if (t + 1 < t1) {
+          seen = seen_of(t + 1);
+          __syncthreads();
+          if (t + 2 < t1) fetch(t + 2);
+          clean(seen, t + 1);
+        }
+      }
+    }
   }
   dlam += __shfl_xor(dlam, 32, 64);
-  if (r >= rows) return;
-  if (a.dq) {
+  if (r >= rows) dlam = 0.f;
+  if ((a.G & (a.G - 1)) == 0 && a.G <= 32) {                                   // one value for each head of the wave
+    for (int o = 16; o >= a.G; o >>= 1) dlam += __shfl_xor(dlam, o, 64);
+    if (lane < a.G) a.dlam_part[((long long)bh * tiles * NW + tile * NW + wave) * a.G + lane] = dlam;
+  } else if (r < rows && h == 0) {
+    a.dlam_part[(long long)bh * rows + r] = dlam;
+  }
+  if (r < rows && a.dq) {
     T* out = (T*)a.dq + at * 2 * D + 4 * h;
+    const float f[2] = {a.scale, -lam_of<T>(a, head) * a.scale};
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          store4<T>(out + m * D + 32 * c + 8 * g, dq[m][c][4 * g] * a.scale, dq[m][c][4 * g + 1] * a.scale, dq[m][c][4 * g + 2] * a.scale, dq[m][c][4 * g + 3] * a.scale);
+        for (int u = 0; u < 4; ++u)
+          store4<T>(out + m * D + 32 * c + 8 * u, dq[m][c][4 * u] * f[m], dq[m][c][4 * u + 1] * f[m], dq[m][c][4 * u + 2] * f[m], dq[m][c][4 * u + 3] * f[m]);
   }
-  if (h == 0) a.dlam_rows[((long long)b * a.H + head) * a.N + n] = dlam;
 }
 
-template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, 1) void diff_attn_dkv(DiffArgs a) {
+// DK, DV: which of the two this launch forms.  At D = 128 their sums and the keys' own values do not fit a wave's registers together, and the scores are formed twice.
+template <typename T, int D, int NW, bool DK, bool DV>
+__global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dkv(DiffArgs a) {
   using TL = Tile<T, D>;
   using F = typename Frag8<T>::type;
-  constexpr int QT = BwdShape<T, D>::KT, NK = D / 16, NV = 2 * D / 16, NC = D / 32, ND = 2 * D / 32;
-  __shared__ __attribute__((aligned(16))) char qt[2][QT * TL::kRow];
-  __shared__ __attribute__((aligned(16))) char gt[2][QT * TL::kRow];
-  __shared__ __attribute__((aligned(16))) float stat[2][4][QT];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  constexpr bool kWeave = BwdShape<T>::kWeave;
+  constexpr int QT = 32, NK = D / 16, NV = DK ? 2 * D / 16 : 1, NC = DK ? D / 32 : 1, ND = DV ? 2 * D / 32 : 1, R = kWeave ? 4 : 2;   // R: blocks in LDS
+  constexpr int kTile = QT * TL::kRow;
+  __shared__ __attribute__((aligned(16))) char tiles_lds[2 * R * kTile];
+  __shared__ __attribute__((aligned(16))) float stat[R][4][QT];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int tiles = (a.M + NW * 32 - 1) / (NW * 32);
   const unsigned id = by_xcd(blockIdx.x, gridDim.x);
   const int tile = (int)(id % tiles), bh = id / tiles, b = bh / a.Hk, hk = bh % a.Hk;
@@ -627,113 +761,227 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_dkv(DiffArgs a) {
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int s = 0; s < NK; ++s) kf[m][s] = load8<T>(k + m * a.k_sm + 16 * s);
+  if constexpr (DK)
 #pragma unroll
-  for (int s = 0; s < NV; ++s) vf[s] = load8<T>(v + 16 * s);
-  f32x16 dk[2][NC], dv[ND];
+    for (int s = 0; s < NV; ++s) vf[s] = load8<T>(v + 16 * s);
+  f32x16 dk[2][NC], dv[ND], s[2], g;
+  F ds[2][2], pc[2];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int m = 0; m < 2; ++m) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) dk[m][c] = zero16();
 #pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { ds[m][i][j] = (T)0.f; pc[i][j] = (T)0.f; }
+  }
+#pragma unroll
   for (int c = 0; c < ND; ++c) dv[c] = zero16();
 
-  // queries that see the workgroup's first key, in tiles, of each head that shares it
-  const int first = a.causal ? max(0, tile * NW * 32 - off) / QT : 0, nq = (a.N + QT - 1) / QT - first, total = max(nq, 0) * a.G;
-  const typename TL::template Loader<QT, NW> lq(a.q_sn, a.q_sm, threadIdx.x), lg((long long)a.H * 2 * D, D, threadIdx.x);
-  auto fetch = [&](int i, int buf) {
-    const int head = hk * a.G + i / nq, n0 = (first + i % nq) * QT;
-    lq(qt[buf], (const T*)a.q + b * a.q_sb + head * a.q_sh + n0 * a.q_sn, a.N - n0, threadIdx.x, wave);
-    lg(gt[buf], (const T*)a.dout + (((long long)b * a.N + n0) * a.H + head) * 2 * D, a.N - n0, threadIdx.x, wave);
+  // the blocks: queries that see the workgroup's first key, of each head that shares it
+  const int first = a.causal ? max(0, tile * NW * 32 - off) / QT : 0, nq = max((a.N + QT - 1) / QT - first, 0), total = nq * a.G;
+  auto qtile = [&](int t) { return tiles_lds + (t & (R - 1)) * kTile; };
+  auto gtile = [&](int t) { return tiles_lds + (R + (t & (R - 1))) * kTile; };
+  const typename TL::template Loader<QT, NW> lq(a.q_sn, a.q_sm, tid), lg((long long)a.H * 2 * D, D, tid);
+  int to_head = hk * a.G, to_n = first * QT;                                   // what the next fetch brings
+  auto fetch = [&](int t) {
+    const int head = to_head, n0 = to_n;
+    to_n += QT;
+    if (to_n >= a.N) { to_n = first * QT; ++to_head; }
+    lq(qtile(t), (const T*)a.q + b * a.q_sb + head * a.q_sh + n0 * a.q_sn, a.N - n0, tid, wave);
+    lg(gtile(t), (const T*)a.dout + (((long long)b * a.N + n0) * a.H + head) * 2 * D, a.N - n0, tid, wave);
     const long long st = ((long long)b * a.H + head) * 2 * a.N;
-    for (int w = wave; w < 2; w += NW) {                                        // lse of both maps, then delta of both: 32 values each
+    for (int w = wave; w < 2; w += NW) {                                       // lse of both maps, then delta of both: 32 values each
       const float* src = (w == 0 ? a.lse : a.delta) + st + (long long)h * a.N + min(n0 + (lane & 31), a.N - 1);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)(&stat[buf][2 * w][0]), 4, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)(&stat[t & (R - 1)][2 * w][0]), 4, 0, 0);
     }
   };
-  if (total > 0) fetch(0, 0);
-  for (int i = 0; i < total; ++i) {
-    const int cur = i & 1, n0 = (first + i % nq) * QT;
-    const float lam = lam_of<T>(a, hk * a.G + i / nq);
-    __syncthreads();
-    if (i + 1 < total) fetch(i + 1, cur ^ 1);
-    if (a.causal && n0 + QT - 1 + off < k0) continue;                           // (this wave's keys lie behind all of them)
-    f32x16 s[2], g = zero16();
+  auto form = [&](f32x16 (&s_)[2], f32x16& g_, int t) {
+    scores<T, D, 2>(s_, qtile(t), kf, 0, lane);
+    if constexpr (DK) {
+      g_ = zero16();
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      s[m] = zero16();
-#pragma unroll
-      for (int j = 0; j < NK; ++j) s[m] = mma(TL::row(qt[cur], lane & 31, m * D + 16 * j + 8 * h), kf[m][j], s[m]);
+      for (int i = 0; i < NV; ++i) g_ = mma(TL::row(gtile(t), lane & 31, 16 * i + 8 * h), vf[i], g_);
     }
+  };
+  auto hide = [&](int n0) {                                                    // queries behind the last, and those that do not see the lane's key
+    if (n0 + QT > a.N || (a.causal && k0 + 31 > n0 + off)) {
+      const unsigned ok = rows_of_lane(a.causal ? key - off - n0 : 0, a.N - 1 - n0, h);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) g = mma(TL::row(gt[cur], lane & 31, 16 * j + 8 * h), vf[j], g);
-    const bool part = n0 + QT > a.N || (a.causal && k0 + 31 > n0 + off);
-    f32x16 pc;
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) s[m][i] = (ok >> row_of(i, 0)) & 1 ? s[m][i] : -INFINITY;
+    }
+  };
+  auto turn = [&](int t, float lam) {                                          // (the second map's score gradients with lam, without the sign)
+    const float(*e)[QT] = stat[t & (R - 1)];
+    f32x16 p;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const float4 e0 = *(const float4*)&stat[cur][0][8 * u + 4 * h], e1 = *(const float4*)&stat[cur][1][8 * u + 4 * h];
-      const float4 d0 = *(const float4*)&stat[cur][2][8 * u + 4 * h], d1 = *(const float4*)&stat[cur][3][8 * u + 4 * h];
-      const float E0[4] = {e0.x, e0.y, e0.z, e0.w}, E1[4] = {e1.x, e1.y, e1.z, e1.w}, D0[4] = {d0.x, d0.y, d0.z, d0.w}, D1[4] = {d1.x, d1.y, d1.z, d1.w};
+      typedef float f4 __attribute__((ext_vector_type(4)));
+      const int at = 8 * u + 4 * h;
+      const f4 e0 = *(const f4*)&e[0][at], e1 = *(const f4*)&e[1][at], d0 = *(const f4*)&e[2][at], d1 = *(const f4*)&e[3][at];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int x = 4 * u + j;
-        float p0 = __builtin_amdgcn_exp2f(fmaf(s[0][x], a.c, -E0[j])), p1 = __builtin_amdgcn_exp2f(fmaf(s[1][x], a.c, -E1[j]));
-        if (part) {
-          const int n = n0 + 8 * u + 4 * h + j;
-          const bool ok = n < a.N && (!a.causal || key <= n + off);
-          p0 = ok ? p0 : 0.f;
-          p1 = ok ? p1 : 0.f;
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[0][x], a.c, -e0[j])), p1 = __builtin_amdgcn_exp2f(fmaf(s[1][x], a.c, -e1[j])) * lam;
+        p[x] = p0 - p1;
+        if constexpr (DK) {
+          s[0][x] = p0 * (g[x] - d0[j]);
+          s[1][x] = p1 * (g[x] - d1[j]);
         }
-        pc[x] = fmaf(-lam, p1, p0);
-        s[0][x] = p0 * (g[x] - D0[j]);
-        s[1][x] = p1 * (g[x] - D1[j]) * -lam;
       }
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const F p = pack<T>(pc, j);
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (DV) pc[i] = pack<T>(p, i);
+      if constexpr (DK) {
+        ds[0][i] = pack<T>(s[0], i);
+        ds[1][i] = pack<T>(s[1], i);
+      }
+    }
+  };
+  auto add = [&](int t) {
 #pragma unroll
-      for (int c = 0; c < ND; ++c) dv[c] = mma(TL::col(gt[cur], 16 * j, 32 * c, lane), p, dv[c]);
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (DV)
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const F ds = pack<T>(s[m], j);
+        for (int c = 0; c < ND; ++c) dv[c] = mma(TL::col(gtile(t), 16 * i, 32 * c, lane), pc[i], dv[c]);
+      if constexpr (DK)
 #pragma unroll
-        for (int c = 0; c < NC; ++c) dk[m][c] = mma(TL::col(qt[cur], 16 * j, m * D + 32 * c, lane), ds, dk[m][c]);
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int c = 0; c < NC; ++c) dk[m][c] = mma(TL::col(qtile(t), 16 * i, m * D + 32 * c, lane), ds[m][i], dk[m][c]);
+    }
+  };
+  if (total > 0) {
+    fetch(0);
+    if constexpr (kWeave)
+      for (int i = tid; i < kTile / 16; i += NW * 64) {                        // (block -1: its probabilities and score gradients are 0)
+        *(float4*)(qtile(-1) + i * 16) = make_float4(0.f, 0.f, 0.f, 0.f);
+        *(float4*)(gtile(-1) + i * 16) = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    __syncthreads();
+    if (total > 1) fetch(1);
+    int head = hk * a.G, n0 = first * QT;
+    float lam = lam_of<T>(a, head);
+    auto step = [&]() {
+      n0 += QT;
+      if (n0 >= a.N && head + 1 < (hk + 1) * a.G) { n0 = first * QT; lam = lam_of<T>(a, ++head); }
+    };
+    if constexpr (kWeave) {
+      form(s, g, 0);
+      for (int t = 0; t < total; ++t) {
+        __syncthreads();                                                       // block t + 1 has come; nobody reads block t - 2 any more
+        if (t + 2 < total) fetch(t + 2);
+        hide(n0);
+        const float lam_t = lam;
+        step();
+        f32x16 s2[2] = {zero16(), zero16()}, g2 = zero16();
+        const char *qn = qtile(t + 1), *gn = gtile(t + 1), *qb = qtile(t - 1), *gb = gtile(t - 1);   // (behind the last block: whatever stands there, unused)
+        const float(*e)[QT] = stat[t & (R - 1)];
+        typedef float f4 __attribute__((ext_vector_type(4)));
+        f4 st[4];
+        F dn[2][2], pn[2];
+        constexpr int NS = 2 * NK, NG = NS + (DK ? NV : 0), NDV = NG + (DV ? 2 * ND : 0), NP = NDV + (DK ? 4 * NC : 0);
+        weave<F, NP, 3>(
+            [&](int i) {
+              return i < NS    ? TL::row(qn, lane & 31, (i & 1) * D + 16 * (i / 2) + 8 * h)
+                     : i < NG  ? TL::row(gn, lane & 31, 16 * (i - NS) + 8 * h)
+                     : i < NDV ? TL::col(gb, 16 * ((i - NG) / ND), 32 * ((i - NG) % ND), lane)
+                               : TL::col(qb, 16 * ((i - NDV) / (2 * NC)), 32 * ((i - NDV) % (2 * NC)), lane);
+            },
+            [&](int i, const F& f) {
+              if (i < NS) s2[i & 1] = mma(f, kf[i & 1][i / 2], s2[i & 1]);
+              else if (i < NG) g2 = mma(f, vf[i - NS], g2);
+              else if (i < NDV) dv[(i - NG) % ND] = mma(f, pc[(i - NG) / ND], dv[(i - NG) % ND]);
+              else {
+                const int c = (i - NDV) % (2 * NC);
+                dk[c / NC][c % NC] = mma(f, ds[c / NC][(i - NDV) / (2 * NC)], dk[c / NC][c % NC]);
+              }
+            },
+            [&](int i) {
+#pragma unroll
+              for (int x = 16 * i / NP; x < 16 * (i + 1) / NP; ++x) {
+                if (x % 4 == 0)
+#pragma unroll
+                  for (int y = 0; y < (DK ? 4 : 2); ++y) st[y] = *(const f4*)&e[y][2 * x + 4 * h];
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[0][x], a.c, -st[0][x % 4])), p1 = __builtin_amdgcn_exp2f(fmaf(s[1][x], a.c, -st[1][x % 4])) * lam_t;
+                if constexpr (DV) pn[x / 8][x % 8] = (T)(p0 - p1);
+                if constexpr (DK) {
+                  dn[0][x / 8][x % 8] = (T)(p0 * (g[x] - st[2][x % 4]));
+                  dn[1][x / 8][x % 8] = (T)(p1 * (g[x] - st[3][x % 4]));
+                }
+              }
+            });
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          if constexpr (DV) pc[m] = pn[m];
+          if constexpr (DK) {
+            ds[m][0] = dn[m][0];
+            ds[m][1] = dn[m][1];
+          }
+          s[m] = s2[m];
+        }
+        if constexpr (DK) {
+          asm volatile("" : "+v"(g2));                                         // (or its products are moved behind the others, to where they are used)
+          g = g2;
+        }
+      }
+      add(total - 1);
+    } else {
+      for (int t = 0; t < total; ++t) {
+        form(s, g, t);
+        hide(n0);
+        turn(t, lam);
+        add(t);
+        step();
+        if (t + 1 < total) {
+          __syncthreads();
+          if (t + 2 < total) fetch(t + 2);
+        }
       }
     }
   }
   if (key >= a.M) return;
   // (a key nobody sees has gradient 0; what its lanes hold came of values that may be anything, and stayed in their own columns)
   const long long at = (((long long)b * a.M + key) * a.Hk + hk) * 2 * D + 4 * h;
+  auto put = [&](T* to, const f32x16& x, float f) {
 #pragma unroll
-  for (int c = 0; c < ND; ++c)
+    for (int u = 0; u < 4; ++u)
+      store4<T>(to + 8 * u, seen ? x[4 * u] * f : 0.f, seen ? x[4 * u + 1] * f : 0.f, seen ? x[4 * u + 2] * f : 0.f, seen ? x[4 * u + 3] * f : 0.f);
+  };
+  if constexpr (DV)
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-      store4<T>((T*)a.dv + at + 32 * c + 8 * g, seen ? dv[c][4 * g] : 0.f, seen ? dv[c][4 * g + 1] : 0.f, seen ? dv[c][4 * g + 2] : 0.f, seen ? dv[c][4 * g + 3] : 0.f);
+    for (int c = 0; c < ND; ++c) put((T*)a.dv + at + 32 * c, dv[c], 1.f);
+  if constexpr (DK)
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        store4<T>((T*)a.dk + at + m * D + 32 * c + 8 * g, seen ? dk[m][c][4 * g] * a.scale : 0.f, seen ? dk[m][c][4 * g + 1] * a.scale : 0.f,
-                  seen ? dk[m][c][4 * g + 2] * a.scale : 0.f, seen ? dk[m][c][4 * g + 3] * a.scale : 0.f);
+      for (int c = 0; c < NC; ++c) put((T*)a.dk + at + m * D + 32 * c, dk[m][c], m ? -a.scale : a.scale);
 }
 
-// dlam[h] = - the sum of its rows' shares, in a fixed order
+// dlam[h] = - the sum of what the waves (or rows) left for it, in a fixed order
 template <typename T>
-__global__ __launch_bounds__(1024) void diff_attn_dlam(DiffArgs a) {
+__global__ __launch_bounds__(1024) void diff_attn_dlam(DiffArgs a, int units) {
   __shared__ float s[16];
-  const int head = blockIdx.x;
-  float v = 0.f;
-  for (int i = threadIdx.x; i < a.B * a.N; i += 1024) v += a.dlam_rows[((long long)(i / a.N) * a.H + head) * a.N + i % a.N];
-  v = group_sum<64>(v);
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+  const int head = blockIdx.x, hk = head / a.G, u = head % a.G;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  const long long all = (long long)a.B * units;
+  auto at = [&](long long i) { return a.dlam_part[((i / units * a.Hk + hk) * units + i % units) * a.G + u]; };
+  long long i = threadIdx.x;
+  for (; i + 3 * 1024 < all; i += 4 * 1024)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += at(i + j * 1024);
+  for (; i < all; i += 1024) v[0] += at(i);
+  const float w = group_sum<64>((v[0] + v[1]) + (v[2] + v[3]));
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = w;
   __syncthreads();
   if (threadIdx.x == 0) {
-    float w = 0.f;
-    for (int i = 0; i < 16; ++i) w += s[i];
-    if (a.lam_f32) ((float*)a.dlam)[head] = -w;
-    else ((T*)a.dlam)[head] = (T)-w;
+    float t = 0.f;
+    for (int j = 0; j < 16; ++j) t += s[j];
+    if (a.lam_f32) ((float*)a.dlam)[head] = -t;
+    else ((T*)a.dlam)[head] = (T)-t;
   }
 }
 

@@ -7,23 +7,23 @@ namespace tok {
 
 #define PGRF_DA_DECL(T, D)                                                                       \
   int launch_da_fwd_##T##_##D(const DiffArgs& a, int waves, unsigned grid, hipStream_t s);       \
-  int launch_da_bwd_##T##_##D(const DiffArgs& a, int row_waves, unsigned row_grid, int key_waves, unsigned key_grid, hipStream_t s);
+  int launch_da_bwd_##T##_##D(const DiffArgs& a, int row_waves, unsigned row_grid, int units, int key_waves, unsigned key_grid, hipStream_t s);
 #define PGRF_DA_ALL(X) X(0, 32) X(0, 64) X(0, 128) X(1, 32) X(1, 64) X(1, 128) X(2, 32) X(2, 64) X(2, 128)
 PGRF_DA_ALL(PGRF_DA_DECL)
 
 static int waves_for(long long rows) { return rows > 64 ? 4 : rows > 32 ? 2 : 1; }
 
-// The forward kernel's waves and their rows: at D = 128 two waves share 32 rows, except where one wave is all there is
+// The forward kernel's waves and their rows: at D = 128 two waves share 32 rows (and float's values leave no room for eight)
 struct FwdCut { int waves, rows, splits; };
-static FwdCut cut_fwd(int B, int Hk, long long rows, int M, int D) {
+static FwdCut cut_fwd(int dtype, int B, int Hk, long long rows, int M, int D) {
   FwdCut f;
   f.waves = waves_for(rows);
-  if (D == 128 && f.waves > 1) f.waves *= 2;
-  f.rows = D == 128 && f.waves > 1 ? f.waves * 16 : f.waves * 32;
+  if (D == 128) f.waves = f.waves == 4 && dtype == PGRF_DTYPE_F32 ? 4 : 2 * f.waves;
+  f.rows = D == 128 ? f.waves * 16 : f.waves * 32;
   const long long groups = (long long)B * Hk * ((rows + f.rows - 1) / f.rows);
   // The key axis is cut where the rows alone leave the chip idle: a share is at least 128 keys, and there are about as many workgroups as the chip holds at a time
   // (two of four waves per CU, five of a single wave, whose two buffers take 32 KB)
-  const long long want = f.waves == 1 ? 1280 : 512, most = M / 128;
+  const long long want = rows <= 32 ? 1280 : 512, most = M / 128;
   long long s = (want + groups - 1) / groups;
   if (groups * 2 > want) s = 1;
   if (s > most) s = most;
@@ -82,10 +82,10 @@ using namespace pgrf::tok;
 
 extern "C" {
 
-size_t pgrf_diff_attention_workspace_bytes(int, int B, int N, int M, int H, int Hk, int D) {
+size_t pgrf_diff_attention_workspace_bytes(int dtype, int B, int N, int M, int H, int Hk, int D) {
   if (B < 1 || N < 1 || M < 1 || H < 1 || Hk < 1 || H % Hk || D < 1) return 0;
   const long long rows = (long long)N * (H / Hk);
-  const int s = cut_fwd(B, Hk, rows, M, D).splits;
+  const int s = cut_fwd(dtype, B, Hk, rows, M, D).splits;
   return s > 1 ? (size_t)s * B * Hk * rows * (4 * D + 4) * sizeof(float) : 0;
 }
 
@@ -96,7 +96,7 @@ int pgrf_diff_attention(const PgrfDiffAttn* p, void* stream) {
   if ((long long)p->B * p->N == 0) return PGRF_OK;
   DiffArgs a = args_of(p);
   const long long rows = (long long)a.N * a.G;
-  const FwdCut cut = cut_fwd(a.B, a.Hk, rows, a.M, p->D);
+  const FwdCut cut = cut_fwd(p->dtype, a.B, a.Hk, rows, a.M, p->D);
   a.splits = cut.splits;
   if (a.splits > 1) {
     const size_t need = pgrf_diff_attention_workspace_bytes(p->dtype, p->B, p->N, p->M, p->H, p->Hk, p->D);
@@ -115,7 +115,7 @@ int pgrf_diff_attention(const PgrfDiffAttn* p, void* stream) {
 
 size_t pgrf_diff_attention_backward_workspace_bytes(int, int B, int N, int M, int H, int Hk, int D) {
   if (B < 1 || N < 1 || M < 1 || H < 1 || Hk < 1 || D < 1) return 0;
-  return (size_t)B * H * N * 3 * sizeof(float);
+  return (size_t)B * H * ((size_t)N * 3 + 4) * sizeof(float);
 }
 
 int pgrf_diff_attention_backward(const PgrfDiffAttn* p, const void* dout, void* dq, void* dk, void* dv, void* dlam, void* stream) {
@@ -131,13 +131,15 @@ int pgrf_diff_attention_backward(const PgrfDiffAttn* p, const void* dout, void* 
   DiffArgs a = args_of(p);
   a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv; a.dlam = dlam;
   a.delta = (float*)p->workspace;
-  a.dlam_rows = a.delta + (size_t)a.B * a.H * 2 * a.N;
+  a.dlam_part = a.delta + (size_t)a.B * a.H * 2 * a.N;
   const long long rows = (long long)a.N * a.G;
   const int rw = waves_for(rows), kw = waves_for(a.M);
+  // (a wave's shares of dlam: G for 32 rows, rounded up to whole workgroups of at most four waves; fewer than N + 4 of each head)
+  const int units = (a.G & (a.G - 1)) == 0 && a.G <= 32 ? (int)((rows + rw * 32 - 1) / (rw * 32) * rw) : a.N;
   const long long rg = (long long)a.B * a.Hk * ((rows + rw * 32 - 1) / (rw * 32)), kg = (long long)a.B * a.Hk * (((long long)a.M + kw * 32 - 1) / (kw * 32));
   if (rg > 0x7fffffffll || kg > 0x7fffffffll) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tiles", who);
 #define PGRF_DA_BWD(T, D_) \
-  if (p->dtype == T && p->D == D_) return launch_da_bwd_##T##_##D_(a, rw, (unsigned)rg, kw, (unsigned)kg, (hipStream_t)stream);
+  if (p->dtype == T && p->D == D_) return launch_da_bwd_##T##_##D_(a, rw, (unsigned)rg, units, kw, (unsigned)kg, (hipStream_t)stream);
   PGRF_DA_ALL(PGRF_DA_BWD)
   return set_error(PGRF_ERR_UNSUPPORTED, "%s: no kernel", who);
 }

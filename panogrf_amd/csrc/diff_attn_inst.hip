@@ -1,4 +1,4 @@
-// The differential attention kernels of one element type and head width (-DPGRF_DA_TYPE, -DPGRF_DA_D), and their launches.
+// The differential attention kernels of one direction, element type and head width (-DPGRF_DA_BWD, -DPGRF_DA_TYPE, -DPGRF_DA_D), and their launches.
 #include "pgrf_experiments.h"
 #include "diff_attn.h"
 
@@ -17,38 +17,55 @@ using DaT = f16;
 #define PGRF_DA_NAME1(a, b, c) PGRF_DA_NAME2(a, b, c)
 #define PGRF_DA_NAME(f) PGRF_DA_NAME1(f, PGRF_DA_TYPE, PGRF_DA_D)
 
+#if !PGRF_DA_BWD
 int PGRF_DA_NAME(launch_da_fwd)(const DiffArgs& a, int waves, unsigned grid, hipStream_t s) {
-  if (waves == 1) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 1>), dim3(grid), dim3(64), 0, s, a);
-  else if (waves == 2) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 2>), dim3(grid), dim3(128), 0, s, a);
-  else if (waves == 4) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 4>), dim3(grid), dim3(256), 0, s, a);
-  else if constexpr (PGRF_DA_D == 128) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 8>), dim3(grid), dim3(512), 0, s, a);
-  PGRF_TOK_LAUNCHED("pgrf_diff_attention");
+  const char* who = "pgrf_diff_attention";
+  if constexpr (PGRF_DA_D < 128)
+    if (waves == 1) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 1>), dim3(grid), dim3(64), 0, s, a);
+  if (waves == 2) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 2>), dim3(grid), dim3(128), 0, s, a);
+  if (waves == 4) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 4>), dim3(grid), dim3(256), 0, s, a);
+  if constexpr (PGRF_DA_D == 128 && sizeof(DaT) == 2)
+    if (waves == 8) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 8>), dim3(grid), dim3(512), 0, s, a);
+  PGRF_TOK_LAUNCHED(who);
   if (a.splits > 1) {
     const long long rows = (long long)a.B * a.Hk * a.N * a.G, per = 256 / (2 * PGRF_DA_D);
     hipLaunchKernelGGL((diff_attn_join<DaT, PGRF_DA_D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, a);
-    PGRF_TOK_LAUNCHED("pgrf_diff_attention");
+    PGRF_TOK_LAUNCHED(who);
   }
   return PGRF_OK;
 }
 
-int PGRF_DA_NAME(launch_da_bwd)(const DiffArgs& a, int row_waves, unsigned row_grid, int key_waves, unsigned key_grid, hipStream_t s) {
+#else
+template <int NW>
+static void launch_dkv(const DiffArgs& a, unsigned grid, hipStream_t s) {
+  if constexpr (PGRF_DA_D == 128) {
+    hipLaunchKernelGGL((diff_attn_dkv<DaT, PGRF_DA_D, NW, false, true>), dim3(grid), dim3(NW * 64), 0, s, a);
+    hipLaunchKernelGGL((diff_attn_dkv<DaT, PGRF_DA_D, NW, true, false>), dim3(grid), dim3(NW * 64), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((diff_attn_dkv<DaT, PGRF_DA_D, NW, true, true>), dim3(grid), dim3(NW * 64), 0, s, a);
+  }
+}
+
+int PGRF_DA_NAME(launch_da_bwd)(const DiffArgs& a, int row_waves, unsigned row_grid, int units, int key_waves, unsigned key_grid, hipStream_t s) {
   const char* who = "pgrf_diff_attention_backward";
   if (row_waves == 1) hipLaunchKernelGGL((diff_attn_dq<DaT, PGRF_DA_D, 1>), dim3(row_grid), dim3(64), 0, s, a);
   else if (row_waves == 2) hipLaunchKernelGGL((diff_attn_dq<DaT, PGRF_DA_D, 2>), dim3(row_grid), dim3(128), 0, s, a);
   else hipLaunchKernelGGL((diff_attn_dq<DaT, PGRF_DA_D, 4>), dim3(row_grid), dim3(256), 0, s, a);
   PGRF_TOK_LAUNCHED(who);
   if (a.dlam) {
-    hipLaunchKernelGGL((diff_attn_dlam<DaT>), dim3(a.H), dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((diff_attn_dlam<DaT>), dim3(a.H), dim3(1024), 0, s, a, units);
     PGRF_TOK_LAUNCHED(who);
   }
   if (a.dk) {
-    if (key_waves == 1) hipLaunchKernelGGL((diff_attn_dkv<DaT, PGRF_DA_D, 1>), dim3(key_grid), dim3(64), 0, s, a);
-    else if (key_waves == 2) hipLaunchKernelGGL((diff_attn_dkv<DaT, PGRF_DA_D, 2>), dim3(key_grid), dim3(128), 0, s, a);
-    else hipLaunchKernelGGL((diff_attn_dkv<DaT, PGRF_DA_D, 4>), dim3(key_grid), dim3(256), 0, s, a);
+    if (key_waves == 1) launch_dkv<1>(a, key_grid, s);
+    else if (key_waves == 2) launch_dkv<2>(a, key_grid, s);
+    else launch_dkv<4>(a, key_grid, s);
     PGRF_TOK_LAUNCHED(who);
   }
   return PGRF_OK;
 }
+
+#endif
 
 }  // namespace tok
 }  // namespace pgrf
