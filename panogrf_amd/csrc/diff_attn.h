@@ -36,40 +36,50 @@ struct Tile {
   static constexpr int kRow = 2 * D * (int)sizeof(T), kChunks = kRow / 16, kPer = 16 / (int)sizeof(T);
   using F = typename Frag8<T>::type;
   static __device__ __forceinline__ int turn(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
-  static __device__ __forceinline__ const char* at(const char* t, int r, int c) { return t + r * kRow + ((c ^ turn(r)) << 4); }
-
-  // 8 values from value e (a multiple of 8) of row r
-  static __device__ __forceinline__ F row(const char* t, int r, int e) {
+  // Where a lane reads: what the places of its fragments have that depends on the lane, so that a read is one of these, the tile, and a constant.
+  struct Lane {
+    int row[4], col[4];
+    __device__ explicit Lane(int lane) {
+      const int r = lane & 31, h = lane >> 5;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if constexpr (sizeof(T) == 2) {
+          row[x] = r * kRow + (((2 * x + h) ^ turn(r)) << 4);
+          // ds_read_b64_tr: the 16 lanes of a group hand in 4 rows x 16 values (4 values each) and each gets a column of 4
+          const int i = lane & 15, rr = 4 * h + (i >> 2), c = 4 * (x & 1) + ((lane & 16) >> 3) + ((i & 3) >> 1);
+          col[x] = rr * kRow + ((c ^ turn(rr)) << 4) + (i & 1) * 8;
+        } else {
+          row[x] = r * kRow + (((4 * (x >> 1) + 2 * h + (x & 1)) ^ turn(r)) << 4);
+          const int rr = 4 * h + x;
+          col[x] = rr * kRow + (((r >> 2) ^ turn(rr)) << 4) + (r & 3) * 4;
+        }
+      }
+    }
+  };
+  // 8 values, 16 q + 8 h .. + 7, of row `lane & 31`
+  static __device__ __forceinline__ F row(const char* t, const Lane& l, int q) {
     if constexpr (sizeof(T) == 2) {
-      return *(const F*)at(t, r, e / 8);
+      return *(const F*)(t + l.row[q & 3] + (q >> 2) * 128);
     } else {
       typedef float f4 __attribute__((ext_vector_type(4)));
-      const f4 lo = *(const f4*)at(t, r, e / 4), hi = *(const f4*)at(t, r, e / 4 + 1);
+      const f4 lo = *(const f4*)(t + l.row[2 * (q & 1)] + (q >> 1) * 128), hi = *(const f4*)(t + l.row[2 * (q & 1) + 1] + (q >> 1) * 128);
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
-  // the transposed fragment: value e0 + (lane & 31) of rows r0 + 4 h + {0..3, 8..11}, h = lane >> 5
-  static __device__ __forceinline__ F col(const char* t, int r0, int e0, int lane) {
-    const int h = lane >> 5;
+  // the transposed fragment: value 32 c + (lane & 31) of rows 16 s + 4 h + {0..3, 8..11}
+  static __device__ __forceinline__ F col(const char* t, const Lane& l, int s, int c) {
     if constexpr (sizeof(T) == 2) {
-      // ds_read_b64_tr: the 16 lanes of a group hand in 4 rows x 16 values (4 values each) and each gets a column of 4
       typedef short s4 __attribute__((ext_vector_type(4)));
       typedef short s8 __attribute__((ext_vector_type(8)));
-      const int i = lane & 15, e = e0 + (lane & 16) + (i & 3) * 4, r = r0 + 4 * h + (i >> 2);
-      const char* p = at(t, r, e / 8) + (i & 1) * 8;
-      const char* q = at(t, r + 8, e / 8) + (i & 1) * 8;
+      const char* p = t + l.col[c & 1] + s * 16 * kRow + (c >> 1) * 128;
       const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(__attribute__((address_space(3))) char*)p);
-      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(__attribute__((address_space(3))) char*)q);
+      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(__attribute__((address_space(3))) char*)(p + 8 * kRow));
       const s8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
       return __builtin_bit_cast(F, v);
     } else {
-      const int e = e0 + (lane & 31);
       F v;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int r = r0 + 4 * h + (j & 3) + (j >> 2) * 8;
-        v[j] = *(const float*)(at(t, r, e / 4) + (e & 3) * 4);
-      }
+      for (int j = 0; j < 8; ++j) v[j] = *(const float*)(t + l.col[j & 3] + (16 * s + 8 * (j >> 2)) * kRow + c * 128);
       return v;
     }
   }
@@ -207,21 +217,28 @@ __device__ __forceinline__ unsigned keys_of_lane(unsigned seen32, int last, int 
 // ---------------------------------------------------------------------------------------------------------------- forward
 // MPW: maps of a wave.  Up to D = 64 a wave keeps the sums of both maps of its 32 rows (128 registers), and every fragment of v serves two products.  At
 // D = 128 two waves share 32 rows, one map each, and meet at the end.
+#ifndef PGRF_DA_WEAVE
+#define PGRF_DA_WEAVE(T, D, NW) (sizeof(T) == 4)
+#define PGRF_DA_MINW 2
+#endif
 template <typename T, int D, int NW> struct FwdShape {
   static_assert(D < 128 || NW > 1, "a pair of waves at D = 128");
   static constexpr int MPW = D == 128 ? 1 : 2;
   static constexpr int KT = 32;                                                // keys of a block
+  static constexpr bool kWeave = PGRF_DA_WEAVE(T, D, NW);
+  static constexpr int kTileKeys = kWeave || sizeof(T) == 4 || NW * MPW < 4 * 2 ? 32 : D == 32 ? 64 : 64;      // keys between barriers
+  static constexpr int kMinWaves = kWeave ? (NW + 3) / 4 : sizeof(T) == 2 && NW > 1 ? PGRF_DA_MINW : (NW + 3) / 4;
 };
 
 // Scores of a block: S^T of MPW maps
 template <typename T, int D, int MPW>
-__device__ __forceinline__ void scores(f32x16 (&s)[MPW], const char* kt, const typename Frag8<T>::type (&qf)[MPW][D / 16], int map0, int lane) {
+__device__ __forceinline__ void scores(f32x16 (&s)[MPW], const char* kt, const typename Frag8<T>::type (&qf)[MPW][D / 16], int map0, const typename Tile<T, D>::Lane& at) {
 #pragma unroll
   for (int m = 0; m < MPW; ++m) s[m] = zero16();
 #pragma unroll
   for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-    for (int m = 0; m < MPW; ++m) s[m] = mma(Tile<T, D>::row(kt, lane & 31, (map0 + m) * D + 16 * i + 8 * (lane >> 5)), qf[m][i], s[m]);
+    for (int m = 0; m < MPW; ++m) s[m] = mma(Tile<T, D>::row(kt, at, (map0 + m) * (D / 16) + i), qf[m][i], s[m]);
 }
 
 __device__ __forceinline__ float top_of(const f32x16& s) {
@@ -240,14 +257,16 @@ __device__ __forceinline__ float with_other_half(float t) {                    /
 // wave by itself keeps both pipes busy (measured on this card: 24 products of 32x32x16, 96 FMAs and 32 exponentials take 471 ns side by side, 386 + 312 one
 // after the other); masks and a new maximum are dealt with in front of it.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_fwd(DiffArgs a) {
+__global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff_attn_fwd(DiffArgs a) {
   using TL = Tile<T, D>;
   using F = typename Frag8<T>::type;
   using Sh = FwdShape<T, D, NW>;
   constexpr int KT = Sh::KT, MPW = Sh::MPW, NK = D / 16, NC = 2 * D / 32, RW = NW * MPW / 2;   // RW: groups of 32 rows in the workgroup
   constexpr int kTile = KT * TL::kRow;
-  __shared__ __attribute__((aligned(16))) char tiles_lds[4 * kTile];             // two blocks of k, two of v
+  constexpr int BT = Sh::kTileKeys / KT;                                         // blocks between barriers
+  __shared__ __attribute__((aligned(16))) char tiles_lds[4 * BT * kTile];        // two tiles of k, two of v
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const typename TL::Lane at(lane);
   const int group = MPW == 2 ? wave : wave >> 1, map0 = MPW == 2 ? 0 : wave & 1;
   const int rows = a.N * a.G, tiles = (rows + RW * 32 - 1) / (RW * 32);
   unsigned id = by_xcd(blockIdx.x, gridDim.x);
@@ -258,13 +277,14 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_fwd(DiffArgs 
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.M) : a.M;
   const int r0 = (tile * RW + group) * 32, r = r0 + (lane & 31), rc = min(r, rows - 1);
   const int n = rc / a.G, head = hk * a.G + rc % a.G;
-  // the last key a row sees, of the wave's first row, and of the workgroup's last row
+  // the last key a row sees, of the wave's first and last row, and of the workgroup's last row
   const int off = len - a.N;
   const int lim = r >= rows ? -1 : a.causal ? min(n + off, len - 1) : len - 1;
   const int lim_lo = r0 + 31 >= rows ? -1 : a.causal ? min(r0 / a.G + off, len - 1) : len - 1;
+  const int lim_hi = r0 >= rows ? -1 : a.causal ? min(min(r0 + 31, rows - 1) / a.G + off, len - 1) : len - 1;
   const int wg_hi = a.causal ? min(min((tile + 1) * RW * 32 - 1, rows - 1) / a.G + off, len - 1) : len - 1;
-  const int all = (wg_hi + KT) / KT, per = (max(all, 0) + a.splits - 1) / a.splits;
-  const int t0 = split * per, t1 = min(all, t0 + per);
+  const int all = (wg_hi + KT * BT) / (KT * BT), per = (max(all, 0) + a.splits - 1) / a.splits;
+  const int t0 = split * per, t1 = min(all, t0 + per);                         // tiles
 
   const T* q = (const T*)a.q + b * a.q_sb + n * a.q_sn + head * a.q_sh + map0 * a.q_sm + 8 * h;
   F qf[MPW][NK];
@@ -301,115 +321,178 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_fwd(DiffArgs 
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const F vf = TL::col(vt, 16 * i, 32 * c, lane);
+        const F vf = TL::col(vt, at, i, c);
 #pragma unroll
         for (int m = 0; m < MPW; ++m) o[m][c] = mma(vf, p[m][i], o[m][c]);
       }
   };
 
-  if (t0 < t1) {
-    fetch_k(t0);
-    for (int i = tid; i < kTile / 16; i += NW * 64) *(float4*)(vtile(t0 - 1) + i * 16) = make_float4(0.f, 0.f, 0.f, 0.f);   // (its probabilities are 0)
-    unsigned seen = ~0u;
-    __syncthreads();
-    if (t0 + 1 < t1) fetch_k(t0 + 1);
-    scores<T, D, MPW>(s, ktile(t0), qf, map0, lane);
-#pragma unroll
-    for (int m = 0; m < MPW; ++m) top[m] = top_of(s[m]);
-    for (int t = t0; t < t1; ++t) {
-      const int k0 = t * KT;
-      const unsigned before = seen;
-      seen = ~0u;
-      if (mask || k0 + KT > len) seen = (unsigned)keys_seen<KT>(mask, k0, len, lane);
-      __syncthreads();                                                         // k of t + 1 and v of t - 1 have come; nobody reads k of t or v of t - 2 any more
-      if (t + 2 < t1) fetch_k(t + 2);
-      if (before != ~0u) {                                                     // what stands in masked values may be anything, and 0 * NaN is NaN
-        TL::template clear<KT, NW * 64>(vtile(t - 1), before, tid);
-        __syncthreads();
-      }
-      fetch_v(t);
-      if (seen != ~0u || k0 + 31 > lim_lo) {
-        const unsigned ok = keys_of_lane(seen, lim - k0, h);
-#pragma unroll
-        for (int m = 0; m < MPW; ++m) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[m][i] = (ok >> row_of(i, 0)) & 1 ? s[m][i] : -INFINITY;
-          top[m] = top_of(s[m]);
-        }
-      }
-      // The running maximum follows only where a row outgrew it by 2^8, and by a whole power of two: sums and values stay in range, and what was rounded before
-      // scales without another rounding
+  auto hide = [&](unsigned seen, int k0) {                                      // masked keys of a block
+    if (seen != ~0u || k0 + 31 > lim_lo) {
+      const unsigned ok = keys_of_lane(seen, lim - k0, h);
 #pragma unroll
       for (int m = 0; m < MPW; ++m) {
-        const float up = with_other_half(top[m]) * a.c;
-        if (__any(up > mx[m] + 8.f)) {
-          const float grow = fmaxf(ceilf(up - mx[m]), 0.f), f = mx[m] == -INFINITY ? 1.f : ldexpf(1.f, -(int)fminf(grow, 1000.f));
-          mx[m] = mx[m] == -INFINITY ? up : mx[m] + grow;
-          l[m] *= f;
 #pragma unroll
-          for (int c = 0; c < NC; ++c) o[m][c] *= f;
+        for (int i = 0; i < 16; ++i) s[m][i] = (ok >> row_of(i, 0)) & 1 ? s[m][i] : -INFINITY;
+        top[m] = top_of(s[m]);
+      }
+    }
+  };
+  // The running maximum follows only where a row outgrew it by 2^8, and by a whole power of two: sums and values stay in range, and what was rounded before
+  // scales without another rounding
+  auto grow = [&]() {
+#pragma unroll
+    for (int m = 0; m < MPW; ++m) {
+      const float up = with_other_half(top[m]) * a.c;
+      if (__any(up > mx[m] + 8.f)) {
+        const float more = fmaxf(ceilf(up - mx[m]), 0.f), f = mx[m] == -INFINITY ? 1.f : ldexpf(1.f, -(int)fminf(more, 1000.f));
+        mx[m] = mx[m] == -INFINITY ? up : mx[m] + more;
+        l[m] *= f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) o[m][c] *= f;
+        if constexpr (Sh::kWeave)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) p[m][i][j] = (T)((float)p[m][i][j] * f);
+      }
+    }
+  };
+  if constexpr (Sh::kWeave) {
+    if (t0 < t1) {
+      fetch_k(t0);
+      for (int i = tid; i < kTile / 16; i += NW * 64) *(float4*)(vtile(t0 - 1) + i * 16) = make_float4(0.f, 0.f, 0.f, 0.f);   // (its probabilities are 0)
+      unsigned seen = ~0u;
+      __syncthreads();
+      if (t0 + 1 < t1) fetch_k(t0 + 1);
+      scores<T, D, MPW>(s, ktile(t0), qf, map0, at);
+  #pragma unroll
+      for (int m = 0; m < MPW; ++m) top[m] = top_of(s[m]);
+      for (int t = t0; t < t1; ++t) {
+        const int k0 = t * KT;
+        const unsigned before = seen;
+        seen = ~0u;
+        if (mask || k0 + KT > len) seen = (unsigned)keys_seen<KT>(mask, k0, len, lane);
+        __syncthreads();                                                         // k of t + 1 and v of t - 1 have come; nobody reads k of t or v of t - 2 any more
+        if (t + 2 < t1) fetch_k(t + 2);
+        if (before != ~0u) {                                                     // what stands in masked values may be anything, and 0 * NaN is NaN
+          TL::template clear<KT, NW * 64>(vtile(t - 1), before, tid);
+          __syncthreads();
+        }
+        fetch_v(t);
+        hide(seen, k0);
+        grow();
+        f32x16 next[MPW];
+        const char *kn = ktile(t + 1), *vb = vtile(t - 1);                       // (behind the last block: scores of whatever stands there, unused)
+        float base[MPW], sum[MPW];
+        F pn[MPW][2];
+  #pragma unroll
+        for (int m = 0; m < MPW; ++m) {
+          next[m] = zero16();
+          base[m] = mx[m] == -INFINITY ? 0.f : mx[m];
+          sum[m] = 0.f;
+        }
+        constexpr int NS = NK * MPW, NA = 2 * NC, NP = NS + NA;                   // fragments of k, of v; every one of v serves MPW products
+        weave<F, NP, 3>(
+            [&](int i) {
+              return i < NS ? TL::row(kn, at, (map0 + i % MPW) * NK + i / MPW) : TL::col(vb, at, (i - NS) / NC, (i - NS) % NC);
+            },
+            [&](int i, const F& f) {
+              if (i < NS) {
+                next[i % MPW] = mma(f, qf[i % MPW][i / MPW], next[i % MPW]);
+              } else {
+                const int c = (i - NS) % NC;
+  #pragma unroll
+                for (int m = 0; m < MPW; ++m) o[m][c] = mma(f, p[m][(i - NS) / NC], o[m][c]);
+              }
+            },
+            [&](int i) {
+  #pragma unroll
+              for (int x = 16 * MPW * i / NP; x < 16 * MPW * (i + 1) / NP; ++x) {
+                const int m = x / 16, e = x % 16;
+                const float w = __builtin_amdgcn_exp2f(fmaf(s[m][e], a.c, -base[m]));
+                sum[m] += w;
+                pn[m][e / 8][e % 8] = (T)w;
+              }
+            });
+  #pragma unroll
+        for (int m = 0; m < MPW; ++m) {
+          l[m] += sum[m];
+          p[m][0] = pn[m][0];
+          p[m][1] = pn[m][1];
+          s[m] = next[m];
+          top[m] = top_of(s[m]);
         }
       }
-      f32x16 next[MPW];
-      const char *kn = ktile(t + 1), *vb = vtile(t - 1);                       // (behind the last block: scores of whatever stands there, unused)
-      float base[MPW], sum[MPW];
-      F pn[MPW][2];
-#pragma unroll
-      for (int m = 0; m < MPW; ++m) {
-        next[m] = zero16();
-        base[m] = mx[m] == -INFINITY ? 0.f : mx[m];
-        sum[m] = 0.f;
-      }
-      constexpr int NS = NK * MPW, NA = 2 * NC, NP = NS + NA;                   // fragments of k, of v; every one of v serves MPW products
-      weave<F, NP, 3>(
-          [&](int i) {
-            return i < NS ? TL::row(kn, lane & 31, (map0 + i % MPW) * D + 16 * (i / MPW) + 8 * h) : TL::col(vb, 16 * ((i - NS) / NC), 32 * ((i - NS) % NC), lane);
-          },
-          [&](int i, const F& f) {
-            if (i < NS) {
-              next[i % MPW] = mma(f, qf[i % MPW][i / MPW], next[i % MPW]);
-            } else {
-              const int c = (i - NS) % NC;
-#pragma unroll
-              for (int m = 0; m < MPW; ++m) o[m][c] = mma(f, p[m][(i - NS) / NC], o[m][c]);
-            }
-          },
-          [&](int i) {
-#pragma unroll
-            for (int x = 16 * MPW * i / NP; x < 16 * MPW * (i + 1) / NP; ++x) {
-              const int m = x / 16, e = x % 16;
-              const float w = __builtin_amdgcn_exp2f(fmaf(s[m][e], a.c, -base[m]));
-              sum[m] += w;
-              pn[m][e / 8][e % 8] = (T)w;
-            }
-          });
-#pragma unroll
-      for (int m = 0; m < MPW; ++m) {
-        l[m] += sum[m];
-        p[m][0] = pn[m][0];
-        p[m][1] = pn[m][1];
-        s[m] = next[m];
-        top[m] = top_of(s[m]);
-      }
-    }
-    __syncthreads();
-    if (seen != ~0u) {
-      TL::template clear<KT, NW * 64>(vtile(t1 - 1), seen, tid);
       __syncthreads();
+      if (seen != ~0u) {
+        TL::template clear<KT, NW * 64>(vtile(t1 - 1), seen, tid);
+        __syncthreads();
+      }
+      add_block(vtile(t1 - 1));
     }
-    add_block(vtile(t1 - 1));
+  } else if (t0 < t1) {
+    // two or more waves on a SIMD: one's exponentials run beside another's products, block by block
+    constexpr int kB = BT * KT;
+    const typename TL::template Loader<kB, NW> bk(a.k_sn, a.k_sm, tid), bv(a.v_sn, D, tid);
+    auto tile_at = [&](int t) { return tiles_lds + (t & 1) * 2 * BT * kTile; };  // k, then v
+    auto fetch = [&](int t) {
+      bk(tile_at(t), k + (long long)t * kB * a.k_sn, len - t * kB, tid, wave);
+      bv(tile_at(t) + BT * kTile, v + (long long)t * kB * a.v_sn, len - t * kB, tid, wave);
+    };
+    fetch(t0);
+    for (int t = t0; t < t1; ++t) {
+      const char *kt = tile_at(t), *vt = kt + BT * kTile;
+      unsigned long long seen = kB == 64 ? ~0ull : 0xffffffffull;
+      if (mask || t * kB + kB > len) seen = keys_seen<kB>(mask, t * kB, len, lane);
+      __syncthreads();                                                         // tile t has come; nobody reads the other any more
+      if (t + 1 < t1) fetch(t + 1);
+      if (seen == 0) continue;
+      if (seen != (kB == 64 ? ~0ull : 0xffffffffull)) {
+        TL::template clear<kB, NW * 64>((char*)vt, seen, tid);
+        __syncthreads();
+      }
+#pragma unroll
+      for (int u = 0; u < BT; ++u) {
+        const int k0 = (t * BT + u) * KT;
+        if (k0 > lim_hi) break;
+        const char *kb = kt + u * kTile, *vb = vt + u * kTile;
+#pragma unroll
+        for (int m = 0; m < MPW; ++m) s[m] = zero16();
+        weave<F, NK * MPW, 2>([&](int i) { return TL::row(kb, at, (map0 + i % MPW) * NK + i / MPW); },
+                              [&](int i, const F& f) { s[i % MPW] = mma(f, qf[i % MPW][i / MPW], s[i % MPW]); }, [](int) {});
+#pragma unroll
+        for (int m = 0; m < MPW; ++m) top[m] = top_of(s[m]);
+        hide((unsigned)(seen >> (KT * u)), k0);
+        grow();
+#pragma unroll
+        for (int m = 0; m < MPW; ++m) {
+          const float base = mx[m] == -INFINITY ? 0.f : mx[m];
+          float sum = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float w = __builtin_amdgcn_exp2f(fmaf(s[m][e], a.c, -base));
+            sum += w;
+            p[m][e / 8][e % 8] = (T)w;
+          }
+          l[m] += sum;
+        }
+        weave<F, 2 * NC, 2>([&](int i) { return TL::col(vb, at, i / NC, i % NC); },
+                            [&](int i, const F& f) {
+#pragma unroll
+                              for (int m = 0; m < MPW; ++m) o[m][i % NC] = mma(f, p[m][i / NC], o[m][i % NC]);
+                            },
+                            [](int) {});
+      }
+    }
   }
 #pragma unroll
   for (int m = 0; m < MPW; ++m) l[m] += __shfl_xor(l[m], 32, 64);
   const bool live = r < rows;
   if (a.splits > 1) {
     if (!live) return;
-    const long long at = ((long long)split * a.B * a.Hk + bh) * rows + r;
-    float* po = a.part_o + at * 4 * D + map0 * 2 * D + 4 * h;
+    const long long pat = ((long long)split * a.B * a.Hk + bh) * rows + r;
+    float* po = a.part_o + pat * 4 * D + map0 * 2 * D + 4 * h;
 #pragma unroll
     for (int m = 0; m < MPW; ++m) {
 #pragma unroll
@@ -417,19 +500,19 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_fwd(DiffArgs 
 #pragma unroll
         for (int g = 0; g < 4; ++g)
           store4<float>(po + m * 2 * D + 32 * c + 8 * g, o[m][c][4 * g], o[m][c][4 * g + 1], o[m][c][4 * g + 2], o[m][c][4 * g + 3]);
-      if (h == 0) *(float2*)(a.part_ml + at * 4 + 2 * (map0 + m)) = make_float2(mx[m], l[m]);
+      if (h == 0) *(float2*)(a.part_ml + pat * 4 + 2 * (map0 + m)) = make_float2(mx[m], l[m]);
     }
     return;
   }
   const float lam = lam_of<T>(a, head);
-  const long long at = ((long long)b * a.N + n) * a.H + head;
+  const long long oat = ((long long)b * a.N + n) * a.H + head;
 #pragma unroll
   for (int m = 0; m < MPW; ++m) {
     const float inv = l[m] > 0.f ? 1.f / l[m] : l[m];                          // (a NaN stays one)
 #pragma unroll
     for (int c = 0; c < NC; ++c) o[m][c] *= inv;
     if (a.o12 && live) {
-      float* oo = a.o12 + at * 4 * D + (map0 + m) * 2 * D + 4 * h;
+      float* oo = a.o12 + oat * 4 * D + (map0 + m) * 2 * D + 4 * h;
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -437,10 +520,10 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_fwd(DiffArgs 
       if (h == 0) a.lse[(((long long)b * a.H + head) * 2 + map0 + m) * a.N + n] = l[m] == 0.f ? INFINITY : mx[m] + log2f(l[m]);
     }
   }
-  T* out = (T*)a.out + at * 2 * D + 4 * h;
+  T* out = (T*)a.out + oat * 2 * D + 4 * h;
   if constexpr (MPW == 1) {
     // the second map's waves hand their values over through LDS, as many column blocks at a time as the tiles' room holds
-    constexpr int kFit = 4 * kTile / (RW * 64 * 64), kAt = kFit < NC ? kFit : NC;
+    constexpr int kFit = 4 * BT * kTile / (RW * 64 * 64), kAt = kFit < NC ? kFit : NC;
     static_assert(kAt >= 1 && NC % kAt == 0, "");
     float* room = (float*)tiles_lds + group * kAt * 16 * 64 + lane;
     for (int c0 = 0; c0 < NC; c0 += kAt) {
@@ -520,11 +603,12 @@ __global__ __launch_bounds__(256) void diff_attn_join(DiffArgs a) {
 // dv = (A1 - lam A2)^T dout, dlam = -sum A2 G.  A and G are formed again from q, k, v, dout and the saved log sums, twice: once by rows (dq, delta,
 // dlam) and once by keys (dk, dv), 14 instead of 10 products of N M D, so that no two workgroups add to one value and gradients do not depend on scheduling.
 //
-// Both kernels weave three blocks as the forward kernel does (scores and G of block j + 1, probabilities of block j, products of block j - 1); float does not, as
-// its products take eight times as long and hide the rest by themselves.
-template <typename T> struct BwdShape {
-  static constexpr bool kWeave = sizeof(T) == 2;
-  static constexpr int kLate = kWeave ? 1 : 0;                                 // blocks between a block's scores and its last use
+// At D = 128 in 16 bits a wave's registers leave a SIMD one wave, and both kernels weave three blocks as the forward kernel does; else two waves or more share a SIMD and
+// run beside each other.  Float does neither, as its products take eight times as long and hide the rest by themselves.
+template <typename T, int D> struct BwdShape {
+  static constexpr bool kWeave = sizeof(T) == 2 && D == 128;
+  static constexpr int kMinWaves = sizeof(T) == 2 && D < 128 ? 2 : 1;
+  static constexpr bool kLdsV = sizeof(T) == 2 && D == 64;                     // dk, dv: the wave's own values stay in LDS, to keep two waves on a SIMD
 };
 
 // Bit row_of(i, 0): whether value i of a lane, row row_of(i, h) of its block, is one of rows lo .. hi
@@ -534,14 +618,15 @@ __device__ __forceinline__ unsigned rows_of_lane(int lo, int hi, int h) {
 }
 
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dq(DiffArgs a) {
+__global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_attn_dq(DiffArgs a) {
   using TL = Tile<T, D>;
   using F = typename Frag8<T>::type;
-  constexpr bool kWeave = BwdShape<T>::kWeave;
+  constexpr bool kWeave = BwdShape<T, D>::kWeave;
   constexpr int KT = 32, NK = D / 16, NV = 2 * D / 16, NC = D / 32, KR = kWeave ? 4 : 2;   // KR: blocks of k in LDS
   constexpr int kTile = KT * TL::kRow;
   __shared__ __attribute__((aligned(16))) char tiles_lds[(KR + 2) * kTile];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const typename TL::Lane at(lane);
   const int rows = a.N * a.G, tiles = (rows + NW * 32 - 1) / (NW * 32);
   const unsigned id = by_xcd(blockIdx.x, gridDim.x);
   const int tile = tiles - 1 - (int)(id % tiles);
@@ -554,10 +639,10 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dq(DiffArgs a
   const int lim_lo = r0 + 31 >= rows ? -1 : a.causal ? min(r0 / a.G + off, len - 1) : len - 1;
   const int wg_hi = a.causal ? min(min((tile + 1) * NW * 32 - 1, rows - 1) / a.G + off, len - 1) : len - 1;
   const int t1 = max((wg_hi + KT) / KT, 0);
-  const long long at = ((long long)b * a.N + n) * a.H + head;
+  const long long oat = ((long long)b * a.N + n) * a.H + head;
 
   const T* q = (const T*)a.q + b * a.q_sb + n * a.q_sn + head * a.q_sh + 8 * h;
-  const T* go = (const T*)a.dout + at * 2 * D + 8 * h;
+  const T* go = (const T*)a.dout + oat * 2 * D + 8 * h;
   F qf[2][NK], gf[NV];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -568,7 +653,7 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dq(DiffArgs a
   float delta[2] = {0.f, 0.f}, lse[2];
   const long long st = ((long long)b * a.H + head) * 2 * a.N + n;
   {
-    const float* oo = a.o12 + at * 4 * D + 8 * h;
+    const float* oo = a.o12 + oat * 4 * D + 8 * h;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
 #pragma unroll
@@ -606,10 +691,14 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dq(DiffArgs a
   };
   auto seen_of = [&](int t) { return mask || t * KT + KT > len ? (unsigned)keys_seen<KT>(mask, t * KT, len, lane) : ~0u; };
   auto form = [&](f32x16 (&s_)[2], f32x16& g_, int t) {
-    scores<T, D, 2>(s_, ktile(t), qf, 0, lane);
-    g_ = zero16();
-#pragma unroll
-    for (int i = 0; i < NV; ++i) g_ = mma(TL::row(vtile(t), lane & 31, 16 * i + 8 * h), gf[i], g_);
+    const char *kb = ktile(t), *vb = vtile(t);
+    s_[0] = s_[1] = g_ = zero16();
+    weave<F, 2 * NK + NV, 2>([&](int i) { return i < 2 * NK ? TL::row(kb, at, (i & 1) * NK + i / 2) : TL::row(vb, at, i - 2 * NK); },
+                             [&](int i, const F& f) {
+                               if (i < 2 * NK) s_[i & 1] = mma(f, qf[i & 1][i / 2], s_[i & 1]);
+                               else g_ = mma(f, gf[i - 2 * NK], g_);
+                             },
+                             [](int) {});
   };
   auto hide = [&](unsigned seen, int t) {                                      // masked keys of block t: their probability becomes 0
     if (seen != ~0u || t * KT + 31 > lim_lo) {
@@ -634,12 +723,13 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dq(DiffArgs a
       for (int i = 0; i < 2; ++i) ds[m][i] = pack<T>(s[m], i);
   };
   auto add = [&](int t) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) dq[m][c] = mma(TL::col(ktile(t), 16 * i, m * D + 32 * c, lane), ds[m][i], dq[m][c]);
+    const char* kb = ktile(t);
+    weave<F, 4 * NC, 2>([&](int i) { return TL::col(kb, at, i / (2 * NC), i % (2 * NC)); },
+                        [&](int i, const F& f) {
+                          const int c = i % (2 * NC);
+                          dq[c / NC][c % NC] = mma(f, ds[c / NC][i / (2 * NC)], dq[c / NC][c % NC]);
+                        },
+                        [](int) {});
   };
   auto clean = [&](unsigned seen, int t) {                                     // what stands in masked keys may be anything, and 0 * NaN is NaN
     if (seen != ~0u) {
@@ -670,8 +760,8 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dq(DiffArgs a
         constexpr int NS = 2 * NK, NG = NS + NV, NP = NG + 4 * NC;
         weave<F, NP, 3>(
             [&](int i) {
-              return i < NS ? TL::row(kn, lane & 31, (i & 1) * D + 16 * (i / 2) + 8 * h) : i < NG ? TL::row(vn, lane & 31, 16 * (i - NS) + 8 * h)
-                                                                                        : TL::col(kb, 16 * ((i - NG) / (2 * NC)), 32 * ((i - NG) % (2 * NC)), lane);
+              return i < NS ? TL::row(kn, at, (i & 1) * NK + i / 2) : i < NG ? TL::row(vn, at, i - NS)
+                                                                                        : TL::col(kb, at, (i - NG) / (2 * NC), (i - NG) % (2 * NC));
             },
             [&](int i, const F& f) {
               if (i < NS) s2[i & 1] = mma(f, qf[i & 1][i / 2], s2[i & 1]);
@@ -725,7 +815,7 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dq(DiffArgs a
     a.dlam_part[(long long)bh * rows + r] = dlam;
   }
   if (r < rows && a.dq) {
-    T* out = (T*)a.dq + at * 2 * D + 4 * h;
+    T* out = (T*)a.dq + oat * 2 * D + 4 * h;
     const float f[2] = {a.scale, -lam_of<T>(a, head) * a.scale};
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -739,15 +829,17 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dq(DiffArgs a
 
 // DK, DV: which of the two this launch forms.  At D = 128 their sums and the keys' own values do not fit a wave's registers together, and the scores are formed twice.
 template <typename T, int D, int NW, bool DK, bool DV>
-__global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dkv(DiffArgs a) {
+__global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_attn_dkv(DiffArgs a) {
   using TL = Tile<T, D>;
   using F = typename Frag8<T>::type;
-  constexpr bool kWeave = BwdShape<T>::kWeave;
+  constexpr bool kWeave = BwdShape<T, D>::kWeave;
   constexpr int QT = 32, NK = D / 16, NV = DK ? 2 * D / 16 : 1, NC = DK ? D / 32 : 1, ND = DV ? 2 * D / 32 : 1, R = kWeave ? 4 : 2;   // R: blocks in LDS
   constexpr int kTile = QT * TL::kRow;
-  __shared__ __attribute__((aligned(16))) char tiles_lds[2 * R * kTile];
+  constexpr bool kLdsV = BwdShape<T, D>::kLdsV && DK;
+  __shared__ __attribute__((aligned(16))) char tiles_lds[(2 * R + (kLdsV ? NW : 0)) * kTile];
   __shared__ __attribute__((aligned(16))) float stat[R][4][QT];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const typename TL::Lane at(lane);
   const int tiles = (a.M + NW * 32 - 1) / (NW * 32);
   const unsigned id = by_xcd(blockIdx.x, gridDim.x);
   const int tile = (int)(id % tiles), bh = id / tiles, b = bh / a.Hk, hk = bh % a.Hk;
@@ -756,14 +848,19 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dkv(DiffArgs 
   const T* k = (const T*)a.k + b * a.k_sb + kc * a.k_sn + hk * a.k_sh + 8 * h;
   const T* v = (const T*)a.v + b * a.v_sb + kc * a.v_sn + hk * a.v_sh + 8 * h;
   const bool seen = key < a.M && (!a.mask || a.mask[b * a.mask_sb + kc]);
-  F kf[2][NK], vf[NV];
+  F kf[2][NK], vf[kLdsV ? 1 : NV];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int s = 0; s < NK; ++s) kf[m][s] = load8<T>(k + m * a.k_sm + 16 * s);
-  if constexpr (DK)
+  const char* own_v = tiles_lds + (2 * R + wave) * kTile;
+  if constexpr (kLdsV) {
+    const typename TL::template Loader<NW * 32, NW> lv(a.v_sn, D, tid);
+    lv(tiles_lds + 2 * R * kTile, (const T*)a.v + b * a.v_sb + (long long)tile * NW * 32 * a.v_sn + hk * a.v_sh, a.M - tile * NW * 32, tid, wave);
+  } else if constexpr (DK) {
 #pragma unroll
     for (int s = 0; s < NV; ++s) vf[s] = load8<T>(v + 16 * s);
+  }
   f32x16 dk[2][NC], dv[ND], s[2], g;
   F ds[2][2], pc[2];
 #pragma unroll
@@ -797,11 +894,24 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dkv(DiffArgs 
     }
   };
   auto form = [&](f32x16 (&s_)[2], f32x16& g_, int t) {
-    scores<T, D, 2>(s_, qtile(t), kf, 0, lane);
+    const char *qb = qtile(t), *gb = gtile(t);
+    s_[0] = s_[1] = zero16();
+    weave<F, 2 * NK, 2>([&](int i) { return TL::row(qb, at, (i & 1) * NK + i / 2); }, [&](int i, const F& f) { s_[i & 1] = mma(f, kf[i & 1][i / 2], s_[i & 1]); },
+                        [](int) {});
     if constexpr (DK) {
       g_ = zero16();
-#pragma unroll
-      for (int i = 0; i < NV; ++i) g_ = mma(TL::row(gtile(t), lane & 31, 16 * i + 8 * h), vf[i], g_);
+      F w[2];
+      if constexpr (kLdsV) w[0] = TL::row(own_v, at, 0);
+      weave<F, NV, 2>([&](int i) { return TL::row(gb, at, i); },
+                      [&](int i, const F& f) {
+                        if constexpr (kLdsV) {
+                          if (i + 1 < NV) w[(i + 1) & 1] = TL::row(own_v, at, i + 1);
+                          g_ = mma(f, w[i & 1], g_);
+                        } else {
+                          g_ = mma(f, vf[i], g_);
+                        }
+                      },
+                      [](int) {});
     }
   };
   auto hide = [&](int n0) {                                                    // queries behind the last, and those that do not see the lane's key
@@ -819,8 +929,8 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dkv(DiffArgs 
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       typedef float f4 __attribute__((ext_vector_type(4)));
-      const int at = 8 * u + 4 * h;
-      const f4 e0 = *(const f4*)&e[0][at], e1 = *(const f4*)&e[1][at], d0 = *(const f4*)&e[2][at], d1 = *(const f4*)&e[3][at];
+      const int x0 = 8 * u + 4 * h;
+      const f4 e0 = *(const f4*)&e[0][x0], e1 = *(const f4*)&e[1][x0], d0 = *(const f4*)&e[2][x0], d1 = *(const f4*)&e[3][x0];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int x = 4 * u + j;
@@ -842,17 +952,17 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dkv(DiffArgs 
     }
   };
   auto add = [&](int t) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if constexpr (DV)
-#pragma unroll
-        for (int c = 0; c < ND; ++c) dv[c] = mma(TL::col(gtile(t), 16 * i, 32 * c, lane), pc[i], dv[c]);
-      if constexpr (DK)
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int c = 0; c < NC; ++c) dk[m][c] = mma(TL::col(qtile(t), 16 * i, m * D + 32 * c, lane), ds[m][i], dk[m][c]);
-    }
+    const char *qb = qtile(t), *gb = gtile(t);
+    constexpr int NDV = DV ? 2 * ND : 0, NP = NDV + (DK ? 4 * NC : 0);
+    weave<F, NP, 2>([&](int i) { return i < NDV ? TL::col(gb, at, i / ND, i % ND) : TL::col(qb, at, (i - NDV) / (2 * NC), (i - NDV) % (2 * NC)); },
+                    [&](int i, const F& f) {
+                      if (i < NDV) dv[i % ND] = mma(f, pc[i / ND], dv[i % ND]);
+                      else {
+                        const int c = (i - NDV) % (2 * NC);
+                        dk[c / NC][c % NC] = mma(f, ds[c / NC][(i - NDV) / (2 * NC)], dk[c / NC][c % NC]);
+                      }
+                    },
+                    [](int) {});
   };
   if (total > 0) {
     fetch(0);
@@ -886,10 +996,10 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dkv(DiffArgs 
         constexpr int NS = 2 * NK, NG = NS + (DK ? NV : 0), NDV = NG + (DV ? 2 * ND : 0), NP = NDV + (DK ? 4 * NC : 0);
         weave<F, NP, 3>(
             [&](int i) {
-              return i < NS    ? TL::row(qn, lane & 31, (i & 1) * D + 16 * (i / 2) + 8 * h)
-                     : i < NG  ? TL::row(gn, lane & 31, 16 * (i - NS) + 8 * h)
-                     : i < NDV ? TL::col(gb, 16 * ((i - NG) / ND), 32 * ((i - NG) % ND), lane)
-                               : TL::col(qb, 16 * ((i - NDV) / (2 * NC)), 32 * ((i - NDV) % (2 * NC)), lane);
+              return i < NS    ? TL::row(qn, at, (i & 1) * NK + i / 2)
+                     : i < NG  ? TL::row(gn, at, i - NS)
+                     : i < NDV ? TL::col(gb, at, (i - NG) / ND, (i - NG) % ND)
+                               : TL::col(qb, at, (i - NDV) / (2 * NC), (i - NDV) % (2 * NC));
             },
             [&](int i, const F& f) {
               if (i < NS) s2[i & 1] = mma(f, kf[i & 1][i / 2], s2[i & 1]);
@@ -945,7 +1055,7 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dkv(DiffArgs 
   }
   if (key >= a.M) return;
   // (a key nobody sees has gradient 0; what its lanes hold came of values that may be anything, and stayed in their own columns)
-  const long long at = (((long long)b * a.M + key) * a.Hk + hk) * 2 * D + 4 * h;
+  const long long oat = (((long long)b * a.M + key) * a.Hk + hk) * 2 * D + 4 * h;
   auto put = [&](T* to, const f32x16& x, float f) {
 #pragma unroll
     for (int u = 0; u < 4; ++u)
@@ -953,12 +1063,12 @@ __global__ __launch_bounds__(NW * 64, (NW + 3) / 4) void diff_attn_dkv(DiffArgs 
   };
   if constexpr (DV)
 #pragma unroll
-    for (int c = 0; c < ND; ++c) put((T*)a.dv + at + 32 * c, dv[c], 1.f);
+    for (int c = 0; c < ND; ++c) put((T*)a.dv + oat + 32 * c, dv[c], 1.f);
   if constexpr (DK)
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int c = 0; c < NC; ++c) put((T*)a.dk + at + m * D + 32 * c, dk[m][c], m ? -a.scale : a.scale);
+      for (int c = 0; c < NC; ++c) put((T*)a.dk + oat + m * D + 32 * c, dk[m][c], m ? -a.scale : a.scale);
 }
 
 // dlam[h] = - the sum of what the waves (or rows) left for it, in a fixed order

@@ -20,12 +20,14 @@ using DaT = f16;
 #if !PGRF_DA_BWD
 int PGRF_DA_NAME(launch_da_fwd)(const DiffArgs& a, int waves, unsigned grid, hipStream_t s) {
   const char* who = "pgrf_diff_attention";
-  if constexpr (PGRF_DA_D < 128)
-    if (waves == 1) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 1>), dim3(grid), dim3(64), 0, s, a);
+#if PGRF_DA_D < 128
+  if (waves == 1) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 1>), dim3(grid), dim3(64), 0, s, a);
+#endif
   if (waves == 2) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 2>), dim3(grid), dim3(128), 0, s, a);
   if (waves == 4) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 4>), dim3(grid), dim3(256), 0, s, a);
-  if constexpr (PGRF_DA_D == 128 && sizeof(DaT) == 2)
-    if (waves == 8) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 8>), dim3(grid), dim3(512), 0, s, a);
+#if PGRF_DA_D == 128 && PGRF_DA_TYPE != 0
+  if (waves == 8) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 8>), dim3(grid), dim3(512), 0, s, a);
+#endif
   PGRF_TOK_LAUNCHED(who);
   if (a.splits > 1) {
     const long long rows = (long long)a.B * a.Hk * a.N * a.G, per = 256 / (2 * PGRF_DA_D);
