@@ -29,57 +29,86 @@ __device__ __forceinline__ f32x16 mma(Frag8<float>::type a, Frag8<float>::type b
   return c;
 }
 
-// A tile of rows of 2 D values in LDS, in chunks of 16 bytes; chunk c of row r lies at place c ^ turn(r).  Reading the same chunk of 8 consecutive rows, or two
-// neighbouring chunks of 4, meets every bank once.
+// A tile of rows of 2 D values in LDS (at a multiple of 256 bytes), in chunks of 16 bytes; chunk c of row r lies at place c ^ turn(r).  turn swaps bits of the row
+// number so that the lanes that LDS serves at a time (256 bytes: 64 banks) meet every bank once, both where 16 rows hand out the same chunk and where the transposed
+// reads take 64 bytes of 4 rows (16 bits), or 128 of 2 (float).  (b128 reads of 16 rows: 4.3 cycles; with 8 different places 8.4, with the plain layout 64.)
+__device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) const char*)(const char*)p; }
+
+// 16 (or 4) bytes of every lane, from base + its offset, straight into LDS, one lane behind the other from the wave's address `to`.  As assembly, because the compiler lets a
+// transposed read wait for every such load in flight, though it goes to another tile.  Nothing but fetched() waits for these.
+__device__ __forceinline__ void fetch16(const void* base, unsigned off, unsigned to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "m0", "memory");
+}
+__device__ __forceinline__ void fetch4(const void* base, unsigned off, unsigned to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(off), "s"(base) : "m0", "memory");
+}
+// Everything that the workgroup's waves fetched so far is in LDS, and their reads so far are done
+__device__ __forceinline__ void fetched() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
 template <typename T, int D>
 struct Tile {
   static constexpr int kRow = 2 * D * (int)sizeof(T), kChunks = kRow / 16, kPer = 16 / (int)sizeof(T);
   using F = typename Frag8<T>::type;
-  static __device__ __forceinline__ int turn(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
-  // Where a lane reads: what the places of its fragments have that depends on the lane, so that a read is one of these, the tile, and a constant.
+  static __host__ __device__ constexpr int turn(int r) {
+    return kChunks == 8      ? ((r >> 1) & 1) << 2 | ((r >> 2) & 3)
+           : sizeof(T) == 2  ? (r & 3) << 2 | ((r >> 2) & 3)
+                             : ((r >> 2) & 1) << 3 | ((r >> 3) & 1) << 2 | (r & 3);
+  }
+  // Where a lane reads: turn is a swap of bits, so every place a lane needs is one of these two with some constant bits flipped, and a constant behind
   struct Lane {
-    int row[4], col[4];
+    unsigned row, col;
     __device__ explicit Lane(int lane) {
       const int r = lane & 31, h = lane >> 5;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        if constexpr (sizeof(T) == 2) {
-          row[x] = r * kRow + (((2 * x + h) ^ turn(r)) << 4);
-          // ds_read_b64_tr: the 16 lanes of a group hand in 4 rows x 16 values (4 values each) and each gets a column of 4
-          const int i = lane & 15, rr = 4 * h + (i >> 2), c = 4 * (x & 1) + ((lane & 16) >> 3) + ((i & 3) >> 1);
-          col[x] = rr * kRow + ((c ^ turn(rr)) << 4) + (i & 1) * 8;
-        } else {
-          row[x] = r * kRow + (((4 * (x >> 1) + 2 * h + (x & 1)) ^ turn(r)) << 4);
-          const int rr = 4 * h + x;
-          col[x] = rr * kRow + (((r >> 2) ^ turn(rr)) << 4) + (r & 3) * 4;
-        }
+      if constexpr (sizeof(T) == 2) {
+        row = r * kRow + ((h ^ turn(r)) << 4);
+        // ds_read_b64_tr: the 16 lanes of a group hand in 4 rows x 16 values (4 values each) and each gets a column of 4
+        const int i = lane & 15, rr = 4 * h + (i >> 2), c = ((lane & 16) >> 3) + ((i & 3) >> 1);
+        col = rr * kRow + ((c ^ turn(rr)) << 4) + (i & 1) * 8;
+      } else {
+        row = r * kRow + (((2 * h) ^ turn(r)) << 4);
+        col = 4 * h * kRow + (((r >> 2) ^ turn(4 * h)) << 4) + (r & 3) * 4;
       }
     }
   };
+  static constexpr int kLow = kChunks < 16 ? kChunks : 16;                     // chunks that turn moves among themselves
+  template <typename W>
+  static __device__ __forceinline__ W read(unsigned at) { return *(__attribute__((address_space(3))) W*)(size_t)at; }
+  static __device__ __forceinline__ unsigned lds(const char* t) { return lds_address(t); }
+
   // 8 values, 16 q + 8 h .. + 7, of row `lane & 31`
   static __device__ __forceinline__ F row(const char* t, const Lane& l, int q) {
+    const unsigned b = lds(t) + l.row;
     if constexpr (sizeof(T) == 2) {
-      return *(const F*)(t + l.row[q & 3] + (q >> 2) * 128);
+      return read<F>((b ^ (2 * q % kLow << 4)) + 2 * q / kLow * kLow * 16);
     } else {
       typedef float f4 __attribute__((ext_vector_type(4)));
-      const f4 lo = *(const f4*)(t + l.row[2 * (q & 1)] + (q >> 1) * 128), hi = *(const f4*)(t + l.row[2 * (q & 1) + 1] + (q >> 1) * 128);
+      const int c = 4 * q;
+      const f4 lo = read<f4>((b ^ (c % kLow << 4)) + c / kLow * kLow * 16), hi = read<f4>((b ^ ((c + 1) % kLow << 4)) + c / kLow * kLow * 16);
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
   // the transposed fragment: value 32 c + (lane & 31) of rows 16 s + 4 h + {0..3, 8..11}
   static __device__ __forceinline__ F col(const char* t, const Lane& l, int s, int c) {
+    const unsigned b = lds(t) + l.col;
     if constexpr (sizeof(T) == 2) {
       typedef short s4 __attribute__((ext_vector_type(4)));
       typedef short s8 __attribute__((ext_vector_type(8)));
-      const char* p = t + l.col[c & 1] + s * 16 * kRow + (c >> 1) * 128;
-      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(__attribute__((address_space(3))) char*)p);
-      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(__attribute__((address_space(3))) char*)(p + 8 * kRow));
+      const int k = 4 * c, behind = s * 16 * kRow + k / kLow * kLow * 16;
+      const unsigned p = (b ^ (k % kLow << 4)) + behind, q = (b ^ ((k % kLow ^ turn(8)) << 4)) + behind + 8 * kRow;
+      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(size_t)p);
+      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(size_t)q);
       const s8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
       return __builtin_bit_cast(F, v);
     } else {
       F v;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = *(const float*)(t + l.col[j & 3] + (16 * s + 8 * (j >> 2)) * kRow + c * 128);
+      for (int j = 0; j < 8; ++j) {
+        const int r = (j & 3) + 8 * (j >> 2), k = 8 * c;
+        v[j] = read<float>((b ^ ((k % kLow ^ turn(r)) << 4)) + (16 * s + r) * kRow + k / kLow * kLow * 16);
+      }
       return v;
     }
   }
@@ -89,10 +118,10 @@ struct Tile {
   struct Loader {
     static constexpr int kSteps = R * kChunks / 64 / NW, kRowsPer = 64 * NW / kChunks;   // rows between a lane's steps
     static_assert(R * kChunks % (64 * NW) == 0 && kRowsPer * kChunks == 64 * NW, "whole waves, whole rows");
-    int row0, sn, sm;
-    __device__ Loader(long long sn_, long long sm_, int tid) : row0(tid / kChunks), sn((int)sn_), sm((int)sm_) {}
-    __device__ __forceinline__ int val(int i, int tid) const {
-      const int e = ((tid % kChunks) ^ turn(row0 + i * kRowsPer)) * kPer;
+    int row0, chunk, sn, sm;
+    __device__ Loader(long long sn_, long long sm_, int tid) : row0(tid / kChunks), chunk((tid % kChunks) ^ turn(tid / kChunks)), sn((int)sn_), sm((int)sm_) {}
+    __device__ __forceinline__ int val(int i) const {
+      const int e = (chunk ^ turn(i * kRowsPer)) * kPer;                       // (row0 < kRowsPer, a power of two: the bits of the two stay apart)
       return e >= D ? e - D + sm : e;
     }
     // base: the tile's first row; rows from `rows` on repeat the last one (they are masked)
@@ -100,8 +129,7 @@ struct Tile {
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         const int r = row0 + i * kRowsPer, g = min(r, rows - 1);
-        const char* p = (const char*)base + (unsigned)((g * sn + val(i, tid)) * (int)sizeof(T));
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)(t + (i * NW + wave) * 1024), 16, 0, 0);
+        fetch16(base, (g * sn + val(i)) * (int)sizeof(T), lds(t) + (i * NW + wave) * 1024);
       }
     }
   };
@@ -264,7 +292,7 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
   constexpr int KT = Sh::KT, MPW = Sh::MPW, NK = D / 16, NC = 2 * D / 32, RW = NW * MPW / 2;   // RW: groups of 32 rows in the workgroup
   constexpr int kTile = KT * TL::kRow;
   constexpr int BT = Sh::kTileKeys / KT;                                         // blocks between barriers
-  __shared__ __attribute__((aligned(16))) char tiles_lds[4 * BT * kTile];        // two tiles of k, two of v
+  __shared__ __attribute__((aligned(1024))) char tiles_lds[4 * BT * kTile];        // two tiles of k, two of v
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const typename TL::Lane at(lane);
   const int group = MPW == 2 ? wave : wave >> 1, map0 = MPW == 2 ? 0 : wave & 1;
@@ -363,7 +391,7 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
       fetch_k(t0);
       for (int i = tid; i < kTile / 16; i += NW * 64) *(float4*)(vtile(t0 - 1) + i * 16) = make_float4(0.f, 0.f, 0.f, 0.f);   // (its probabilities are 0)
       unsigned seen = ~0u;
-      __syncthreads();
+      fetched();
       if (t0 + 1 < t1) fetch_k(t0 + 1);
       scores<T, D, MPW>(s, ktile(t0), qf, map0, at);
   #pragma unroll
@@ -373,7 +401,7 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
         const unsigned before = seen;
         seen = ~0u;
         if (mask || k0 + KT > len) seen = (unsigned)keys_seen<KT>(mask, k0, len, lane);
-        __syncthreads();                                                         // k of t + 1 and v of t - 1 have come; nobody reads k of t or v of t - 2 any more
+        fetched();                                                         // k of t + 1 and v of t - 1 have come; nobody reads k of t or v of t - 2 any more
         if (t + 2 < t1) fetch_k(t + 2);
         if (before != ~0u) {                                                     // what stands in masked values may be anything, and 0 * NaN is NaN
           TL::template clear<KT, NW * 64>(vtile(t - 1), before, tid);
@@ -424,7 +452,7 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
           top[m] = top_of(s[m]);
         }
       }
-      __syncthreads();
+      fetched();
       if (seen != ~0u) {
         TL::template clear<KT, NW * 64>(vtile(t1 - 1), seen, tid);
         __syncthreads();
@@ -445,7 +473,7 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
       const char *kt = tile_at(t), *vt = kt + BT * kTile;
       unsigned long long seen = kB == 64 ? ~0ull : 0xffffffffull;
       if (mask || t * kB + kB > len) seen = keys_seen<kB>(mask, t * kB, len, lane);
-      __syncthreads();                                                         // tile t has come; nobody reads the other any more
+      fetched();                                                         // tile t has come; nobody reads the other any more
       if (t + 1 < t1) fetch(t + 1);
       if (seen == 0) continue;
       if (seen != (kB == 64 ? ~0ull : 0xffffffffull)) {
@@ -527,7 +555,7 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
     static_assert(kAt >= 1 && NC % kAt == 0, "");
     float* room = (float*)tiles_lds + group * kAt * 16 * 64 + lane;
     for (int c0 = 0; c0 < NC; c0 += kAt) {
-      __syncthreads();                                                         // (also: the tiles are read)
+      fetched();                                                         // (also: the tiles are read)
 #pragma unroll
       for (int c = 0; c < NC; ++c)
         if (map0 == 1 && c >= c0 && c < c0 + kAt)
@@ -624,7 +652,7 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
   constexpr bool kWeave = BwdShape<T, D>::kWeave;
   constexpr int KT = 32, NK = D / 16, NV = 2 * D / 16, NC = D / 32, KR = kWeave ? 4 : 2;   // KR: blocks of k in LDS
   constexpr int kTile = KT * TL::kRow;
-  __shared__ __attribute__((aligned(16))) char tiles_lds[(KR + 2) * kTile];
+  __shared__ __attribute__((aligned(1024))) char tiles_lds[(KR + 2) * kTile];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const typename TL::Lane at(lane);
   const int rows = a.N * a.G, tiles = (rows + NW * 32 - 1) / (NW * 32);
@@ -743,14 +771,14 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
     unsigned seen = seen_of(0);
     if constexpr (kWeave)
       for (int i = tid; i < kTile / 16; i += NW * 64) *(float4*)(ktile(-1) + i * 16) = make_float4(0.f, 0.f, 0.f, 0.f);   // (its score gradients are 0)
-    __syncthreads();
+    fetched();
     if (t1 > 1) fetch(1);
     clean(seen, 0);
     if constexpr (kWeave) {
       form(s, g, 0);
       for (int t = 0; t < t1; ++t) {
         const unsigned next = t + 1 < t1 ? seen_of(t + 1) : ~0u;
-        __syncthreads();                                                       // block t + 1 has come; nobody reads k of t - 2 or v of t any more
+        fetched();                                                       // block t + 1 has come; nobody reads k of t - 2 or v of t any more
         if (t + 2 < t1) fetch(t + 2);
         clean(next, t + 1);
         hide(seen, t);
@@ -799,7 +827,7 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
         add(t);
         if (t + 1 < t1) {
           seen = seen_of(t + 1);
-          __syncthreads();
+          fetched();
           if (t + 2 < t1) fetch(t + 2);
           clean(seen, t + 1);
         }
@@ -836,7 +864,7 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
   constexpr int QT = 32, NK = D / 16, NV = DK ? 2 * D / 16 : 1, NC = DK ? D / 32 : 1, ND = DV ? 2 * D / 32 : 1, R = kWeave ? 4 : 2;   // R: blocks in LDS
   constexpr int kTile = QT * TL::kRow;
   constexpr bool kLdsV = BwdShape<T, D>::kLdsV && DK;
-  __shared__ __attribute__((aligned(16))) char tiles_lds[(2 * R + (kLdsV ? NW : 0)) * kTile];
+  __shared__ __attribute__((aligned(1024))) char tiles_lds[(2 * R + (kLdsV ? NW : 0)) * kTile];
   __shared__ __attribute__((aligned(16))) float stat[R][4][QT];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const typename TL::Lane at(lane);
@@ -887,11 +915,10 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
     if (to_n >= a.N) { to_n = first * QT; ++to_head; }
     lq(qtile(t), (const T*)a.q + b * a.q_sb + head * a.q_sh + n0 * a.q_sn, a.N - n0, tid, wave);
     lg(gtile(t), (const T*)a.dout + (((long long)b * a.N + n0) * a.H + head) * 2 * D, a.N - n0, tid, wave);
-    const long long st = ((long long)b * a.H + head) * 2 * a.N;
-    for (int w = wave; w < 2; w += NW) {                                       // lse of both maps, then delta of both: 32 values each
-      const float* src = (w == 0 ? a.lse : a.delta) + st + (long long)h * a.N + min(n0 + (lane & 31), a.N - 1);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)(&stat[t & (R - 1)][2 * w][0]), 4, 0, 0);
-    }
+    const long long st = ((long long)b * a.H + head) * 2 * a.N + n0;
+    const unsigned off = ((unsigned)h * a.N + min(lane & 31, a.N - 1 - n0)) * 4u;
+    for (int w = wave; w < 2; w += NW)                                         // lse of both maps, then delta of both: 32 values each
+      fetch4((w == 0 ? a.lse : a.delta) + st, off, lds_address(&stat[t & (R - 1)][2 * w][0]));
   };
   auto form = [&](f32x16 (&s_)[2], f32x16& g_, int t) {
     const char *qb = qtile(t), *gb = gtile(t);
@@ -971,7 +998,7 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
         *(float4*)(qtile(-1) + i * 16) = make_float4(0.f, 0.f, 0.f, 0.f);
         *(float4*)(gtile(-1) + i * 16) = make_float4(0.f, 0.f, 0.f, 0.f);
       }
-    __syncthreads();
+    fetched();
     if (total > 1) fetch(1);
     int head = hk * a.G, n0 = first * QT;
     float lam = lam_of<T>(a, head);
@@ -982,7 +1009,7 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
     if constexpr (kWeave) {
       form(s, g, 0);
       for (int t = 0; t < total; ++t) {
-        __syncthreads();                                                       // block t + 1 has come; nobody reads block t - 2 any more
+        fetched();                                                       // block t + 1 has come; nobody reads block t - 2 any more
         if (t + 2 < total) fetch(t + 2);
         hide(n0);
         const float lam_t = lam;
@@ -1047,7 +1074,7 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
         add(t);
         step();
         if (t + 1 < total) {
-          __syncthreads();
+          fetched();
           if (t + 2 < total) fetch(t + 2);
         }
       }
