@@ -483,17 +483,24 @@ int pgrf_equirec_to_cube(const float* erp, int N, int H, int W, int C, long long
 #define PGRF_NORM_POST 2
 #define PGRF_NORM_PRE 4
 #define PGRF_BLOCK_NORM_MAX_C 8192
-int pgrf_block_norm(const void* x, const void* y, const void* gate, long long rows_per_gate, const void* post_w, const void* post_b,
-                    const void* pre_w, const void* pre_b, int dtype, long long rows, int C, int flags, float scale, float eps, void* x_out,
-                    void* z_out, float* stats, void* stream);
-/* Gradients for upstream dx_out, dz [rows, C] (NULL = zero); x, y, the gate and the weights are the forward's, stats what it wrote.  Any of dx, dy, dgate, dpost_w, dpost_b, dpre_w, dpre_b may be NULL; those
- * asked for are written, not accumulated (a bias' only with PGRF_NORM_LAYER).  `workspace`: 16-byte aligned scratch of the size the
- * function below names, read only where a weight's or a shared gate's gradient is asked for. */
+typedef struct PgrfBlockNorm {
+  const void *x, *y, *gate, *post_w, *post_b, *pre_w, *pre_b;
+  void *x_out, *z_out;
+  float* stats;                /* 16-byte aligned */
+  /* backward: gradients for upstream dx_out, dz [rows, C] (NULL = zero); x, y, the gate and the weights are the forward's, stats what it wrote.  Any of
+   * dx .. dpre_b may be NULL; those asked for are written, not accumulated (a bias' only with PGRF_NORM_LAYER).  A weight's or a shared gate's gradient
+   * needs `workspace`, 16-byte aligned scratch of the size the function below names. */
+  const void *dx_out, *dz;
+  void *dx, *dy, *dgate, *dpost_w, *dpost_b, *dpre_w, *dpre_b;
+  void* workspace;
+  size_t workspace_bytes;
+  long long rows, rows_per_gate;
+  int dtype, C, flags;
+  float scale, eps;
+} PgrfBlockNorm;
+int pgrf_block_norm(const PgrfBlockNorm* a, void* stream);
 size_t pgrf_block_norm_backward_workspace_bytes(long long rows, int C, long long rows_per_gate);
-int pgrf_block_norm_backward(const void* x, const void* y, const void* gate, long long rows_per_gate, const void* post_w, const void* post_b,
-                             const void* pre_w, const float* stats, const void* dx_out, const void* dz, int dtype, long long rows, int C, int flags,
-                             float scale, void* dx, void* dy, void* dgate, void* dpost_w, void* dpost_b, void* dpre_w, void* dpre_b, void* workspace,
-                             size_t workspace_bytes, void* stream);
+int pgrf_block_norm_backward(const PgrfBlockNorm* a, void* stream);
 
 /* Rotary positions of queries and keys in one launch: q [B,N,q_heads,D] and k [B,N,k_heads,D] (k_heads 0: none) by the strides of their first
  * three axes, the channels side by side; q_out, k_out contiguous.  Pair i of the first rotary_dim channels (interleaved: 2i, 2i+1; otherwise
@@ -508,10 +515,15 @@ int pgrf_block_norm_backward(const void* x, const void* y, const void* gate, lon
 #define PGRF_ROTARY_LINEAR 1
 #define PGRF_ROTARY_NTK 2
 #define PGRF_ROTARY_PARTS 3
-int pgrf_rotary(const void* q, long long q_sb, long long q_sn, long long q_sh, int q_heads, const void* k, long long k_sb, long long k_sn,
-                long long k_sh, int k_heads, const void* positions, int position_type, long long pos_sb, int dtype, int B, int N, int D,
-                int rotary_dim, int interleaved, double base, int scaling, double factor, double trained_length, double low, double high,
-                float magnitude, int backward, void* q_out, void* k_out, void* stream);
+typedef struct PgrfRotary {
+  const void *q, *k, *positions;
+  void *q_out, *k_out;
+  long long q_sb, q_sn, q_sh, k_sb, k_sn, k_sh, pos_sb;
+  double base, factor, trained_length, low, high;
+  int dtype, B, N, D, q_heads, k_heads, rotary_dim, interleaved, position_type, scaling, backward;
+  float magnitude;
+} PgrfRotary;
+int pgrf_rotary(const PgrfRotary* a, void* stream);
 
 /* Differential attention: out = (softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v, per head.
  * q [B,N,H,2,D], k [B,M,Hk,2,D], v [B,M,Hk,2D] by strides (channels side by side; rows 16-byte aligned: every stride a multiple of 16 bytes), D 32, 64

@@ -52,6 +52,21 @@ class PgrfRenderCfg(C.Structure):
                 ("use_vis_coarse", C.c_int), ("use_vis_fine", C.c_int), ("precision", C.c_int)]
 
 
+class PgrfBlockNorm(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "y", "gate", "post_w", "post_b", "pre_w", "pre_b", "x_out", "z_out", "stats", "dx_out", "dz", "dx", "dy",
+                                          "dgate", "dpost_w", "dpost_b", "dpre_w", "dpre_b", "workspace")] + \
+               [("workspace_bytes", C.c_size_t), ("rows", C.c_longlong), ("rows_per_gate", C.c_longlong)] + \
+               [(n, C.c_int) for n in ("dtype", "C", "flags")] + [("scale", C.c_float), ("eps", C.c_float)]
+
+
+class PgrfRotary(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "positions", "q_out", "k_out")] + \
+               [(n, C.c_longlong) for n in ("q_sb", "q_sn", "q_sh", "k_sb", "k_sn", "k_sh", "pos_sb")] + \
+               [(n, C.c_double) for n in ("base", "factor", "trained_length", "low", "high")] + \
+               [(n, C.c_int) for n in ("dtype", "B", "N", "D", "q_heads", "k_heads", "rotary_dim", "interleaved", "position_type", "scaling",
+                                       "backward")] + [("magnitude", C.c_float)]
+
+
 class PgrfDiffAttn(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "lam", "key_mask", "lengths", "out", "lse", "maps_out", "workspace")] + \
                [("workspace_bytes", C.c_size_t)] + \
@@ -160,18 +175,15 @@ SYMBOLS = {
     "pgrf_equirec_to_cube": (C.c_int, [_P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_longlong, C.c_longlong, C.c_longlong, C.c_longlong,
                                        _P, _P, C.c_int, C.c_int, _P, _P, _P, _P, C.c_longlong, C.c_longlong, C.c_longlong,
                                        C.c_longlong, _P]),
-    "pgrf_block_norm": (C.c_int, [_P, _P, _P, C.c_longlong, _P, _P, _P, _P, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_float, C.c_float,
-                                  _P, _P, _P, _P]),
+    # the token operators' structures are handed over as packed bytes (panogrf_amd/_token.py): void pointers
+    "pgrf_block_norm": (C.c_int, [_P, _P]),
     "pgrf_block_norm_backward_workspace_bytes": (C.c_size_t, [C.c_longlong, C.c_int, C.c_longlong]),
-    "pgrf_block_norm_backward": (C.c_int, [_P, _P, _P, C.c_longlong, _P, _P, _P, _P, _P, _P, C.c_int, C.c_longlong, C.c_int, C.c_int,
-                                           C.c_float, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
-    "pgrf_rotary": (C.c_int, [_P, C.c_longlong, C.c_longlong, C.c_longlong, C.c_int, _P, C.c_longlong, C.c_longlong, C.c_longlong, C.c_int,
-                              _P, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_double, C.c_int,
-                              C.c_double, C.c_double, C.c_double, C.c_double, C.c_float, C.c_int, _P, _P, _P]),
+    "pgrf_block_norm_backward": (C.c_int, [_P, _P]),
+    "pgrf_rotary": (C.c_int, [_P, _P]),
     "pgrf_diff_attention_workspace_bytes": (C.c_size_t, [C.c_int] * 7),
-    "pgrf_diff_attention": (C.c_int, [C.POINTER(PgrfDiffAttn), _P]),
+    "pgrf_diff_attention": (C.c_int, [_P, _P]),
     "pgrf_diff_attention_backward_workspace_bytes": (C.c_size_t, [C.c_int] * 7),
-    "pgrf_diff_attention_backward": (C.c_int, [C.POINTER(PgrfDiffAttn), _P, _P, _P, _P, _P, _P]),
+    "pgrf_diff_attention_backward": (C.c_int, [_P, _P, _P, _P, _P, _P, _P]),
     "pgrf_render_rays_train": (C.c_int, [C.POINTER(PgrfFrame), _P, _P, C.POINTER(PgrfRenderCfg), _P, C.c_int, _P, _P,
                                          C.POINTER(PgrfPassOut), C.POINTER(PgrfPassOut), _P, _P, _P, C.c_size_t, _P]),
 }

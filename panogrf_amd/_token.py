@@ -1,16 +1,39 @@
-"""What the token operators (block_norm, rotary, attention) share: checks of their tensors and the launch's device and stream."""
+"""What the token operators (block_norm, rotary, attention) share: checks of their tensors and the call into the library.
+
+A small call costs the host more than the GPU, so the way down is short: argument structures are packed as bytes in one go, entry points are looked up once,
+and the device is switched only where the tensors are on another one."""
+import struct
+
 import torch
 
-from ._lib import PgrfError
+from ._lib import PgrfError, lib
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # PGRF_DTYPE_* of include/panogrf_hip.h
 
+# the structures of include/panogrf_hip.h, field by field
+BLOCK_NORM = struct.Struct('@20PN2q3i2f4x')
+ROTARY = struct.Struct('@5P7q5d11if')
+DIFF_ATTN = struct.Struct('@10PN12q9if')
+
+_entries = {}
+
+
+def entry(name):
+    f = _entries.get(name)
+    if f is None:
+        f = _entries[name] = getattr(lib, name)
+    return f
+
+
+def refuse(who, what):
+    raise PgrfError(f'{who}: {what}')
+
 
 def dtype_code(t, who):
-    try:
-        return DTYPES[t.dtype]
-    except KeyError:
-        raise PgrfError(f'{who}: dtype {t.dtype} (float32, bfloat16 or float16)') from None
+    code = DTYPES.get(t.dtype)
+    if code is None:
+        refuse(who, f'dtype {t.dtype} (float32, bfloat16 or float16)')
+    return code
 
 
 def require(ok, who, what):
@@ -20,40 +43,39 @@ def require(ok, who, what):
 
 def on_gpu(t, who):
     if not t.is_cuda:
-        raise PgrfError(f'{who}: the tensors must be on a ROCm GPU (gfx950); there is no CPU fallback')
+        refuse(who, 'the tensors must be on a ROCm GPU (gfx950); there is no CPU fallback')
 
 
-def alike(who, dtype, device, **tensors):
-    """Every tensor given has this dtype and device."""
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not torch.is_tensor(t):
-            raise PgrfError(f'{who}: {name} must be a tensor')
-        if t.device != device:
-            raise PgrfError(f'{who}: {name} is on {t.device}, expected {device}')
-        if t.dtype != dtype:
-            raise PgrfError(f'{who}: {name} is {t.dtype}, expected {dtype}')
+def alike(who, name, t, dtype, device):
+    """The tensor has this dtype and device."""
+    if not isinstance(t, torch.Tensor):
+        refuse(who, f'{name} must be a tensor')
+    if t.device != device:
+        refuse(who, f'{name} is on {t.device}, expected {device}')
+    if t.dtype != dtype:
+        refuse(who, f'{name} is {t.dtype}, expected {dtype}')
 
 
-class on_device:
-    """The launch goes to the tensors' device, whatever the current one is, and to that device's current stream."""
-    __slots__ = ('index', 'before')
+def launch(device, name, *args):
+    """Calls an entry point with `args` and the current stream of the tensors' device, whatever the current device is."""
+    index = device.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            rc = entry(name)(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        rc = entry(name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        lib.check(rc)
 
-    def __init__(self, device):
-        self.index = device.index
 
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
+def first_derivatives_only(backward):
+    """torch's once_differentiable where a graph of the gradients is asked for (its wrapper costs more than a small backward pass)."""
+    guarded = torch.autograd.function.once_differentiable(backward)
 
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
-        return False
+    def call(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return call
 
 
 def ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()

@@ -4,39 +4,39 @@
 
 per head, with a learned weight lam: what both maps spread over tokens that do not matter cancels.  It stands beside the aggregation net's ray attention
 (network/ibrnet.py:160-204), which the render pass computes in its own kernel, for nets over more tokens than a ray has samples."""
-import ctypes as C
+from functools import lru_cache
 
 import torch
 
-from ._lib import PgrfDiffAttn, lib
-from ._token import alike, dtype_code, on_device, on_gpu, ptr, require
+from ._token import DIFF_ATTN, DTYPES, alike, entry, first_derivatives_only, launch, on_gpu, ptr, refuse, require
 
 
 def _aligned(t):
     """A tensor whose last axis is side by side and whose rows start at multiples of 16 bytes, with tokens and maps at most 2^22 values apart: t itself where it is one."""
-    per = 16 // t.element_size()
-    if t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(s % per == 0 or n == 1 for s, n in zip(t.stride()[:-1], t.shape[:-1])) and \
-            all(t.stride(i) <= 1 << 22 for i in (1, 3) if i < t.dim() - 1 and t.shape[i] > 1):
+    s = t.stride()
+    odd = 0
+    for x in s[:-1]:
+        odd |= x
+    if s[-1] == 1 and odd % (16 // t.element_size()) == 0 and s[1] <= 1 << 22 and (len(s) < 5 or s[3] <= 1 << 22) and t.data_ptr() % 16 == 0:
         return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    t = t.contiguous()                              # (a contiguous tensor's rows are multiples of 16 bytes; axes of one may have any stride)
+    s = t.stride()
+    if t.data_ptr() % 16 or (t.shape[1] > 1 and s[1] > 1 << 22) or any(x % (16 // t.element_size()) for x in s[:-1]):
+        t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+    return t
 
 
-def _strides(t):
-    return [0 if n == 1 else s for s, n in zip(t.stride(), t.shape)][:-1]
+@lru_cache(maxsize=256)
+def _workspace_bytes(name, *sizes):
+    return entry(name)(*sizes)
 
 
-def _args(q, k, v, lam, mask, lengths, causal, scale):
+def _pack(q, k, v, lam, mask, lengths, causal, scale, out, lse, maps, ws, ws_bytes):
     B, N, H, _, D = q.shape
-    a = PgrfDiffAttn(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), ptr(mask), ptr(lengths))
-    a.q_sb, a.q_sn, a.q_sh, a.q_sm = _strides(q)
-    a.k_sb, a.k_sn, a.k_sh, a.k_sm = _strides(k)
-    a.v_sb, a.v_sn, a.v_sh = _strides(v)
-    if mask is not None:
-        a.mask_sb = mask.stride(0) if B > 1 else 0
-    a.dtype, a.lam_f32 = dtype_code(q, 'diff_attention'), int(lam.dtype == torch.float32)
-    a.B, a.N, a.M, a.H, a.Hk, a.D, a.causal, a.scale = B, N, k.shape[1], H, k.shape[2], D, int(causal), scale
-    return a
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    return DIFF_ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), ptr(mask), ptr(lengths), ptr(out), ptr(lse), ptr(maps), ptr(ws), ws_bytes,
+                          qs[0], qs[1], qs[2], qs[3], ks[0], ks[1], ks[2], ks[3], vs[0], vs[1], vs[2], 0 if mask is None or B == 1 else mask.stride(0),
+                          DTYPES[q.dtype], lam.dtype == torch.float32, B, N, k.shape[1], H, k.shape[2], D, causal, scale)
 
 
 def _forward(q, k, v, lam, mask, lengths, causal, scale, train):
@@ -48,13 +48,9 @@ def _forward(q, k, v, lam, mask, lengths, causal, scale, train):
     out = torch.empty(B, N, H, 2 * D, dtype=q.dtype, device=dev)
     lse = torch.empty(B, H, 2, N, dtype=torch.float32, device=dev) if train else None
     maps = torch.empty(B, N, H, 2, 2 * D, dtype=torch.float32, device=dev) if train else None
-    a = _args(q, k, v, lam, mask, lengths, causal, scale)
-    a.out, a.lse, a.maps_out = out.data_ptr(), ptr(lse), ptr(maps)
-    n = lib.pgrf_diff_attention_workspace_bytes(a.dtype, B, N, M, H, a.Hk, D)
-    with on_device(dev) as stream:
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        a.workspace, a.workspace_bytes = ptr(ws), n
-        lib.check(lib.pgrf_diff_attention(C.byref(a), stream))
+    n = _workspace_bytes('pgrf_diff_attention_workspace_bytes', DTYPES[q.dtype], B, N, M, H, k.shape[2], D)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    launch(dev, 'pgrf_diff_attention', _pack(q, k, v, lam, mask, lengths, causal, scale, out, lse, maps, ws, n))
     return out, lse, maps
 
 
@@ -67,7 +63,7 @@ class _DiffAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_derivatives_only
     def backward(ctx, dout):
         q, k, v, lam, mask, lse, maps = ctx.saved_tensors
         needs = ctx.needs_input_grad
@@ -77,32 +73,41 @@ class _DiffAttention(torch.autograd.Function):
         dq, dk, dv, dlam = make(q, needs[0]), make(k, both), make(v, both), make(lam, needs[3])
         if lse is not None:
             B, N, H, _, D = q.shape
-            dout = _aligned(dout.contiguous())
-            a = _args(q, k, v, lam, mask, None, *ctx.call)
-            a.lse, a.maps_out = lse.data_ptr(), maps.data_ptr()
-            n = lib.pgrf_diff_attention_backward_workspace_bytes(a.dtype, B, N, a.M, H, a.Hk, D)
-            with on_device(q.device) as stream:
-                ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-                a.workspace, a.workspace_bytes = ws.data_ptr(), n
-                lib.check(lib.pgrf_diff_attention_backward(C.byref(a), dout.data_ptr(), ptr(dq), ptr(dk), ptr(dv), ptr(dlam), stream))
+            dout = dout.contiguous()
+            if dout.data_ptr() % 16:
+                dout = dout.clone()
+            n = _workspace_bytes('pgrf_diff_attention_backward_workspace_bytes', DTYPES[q.dtype], B, N, k.shape[1], H, k.shape[2], D)
+            ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+            launch(q.device, 'pgrf_diff_attention_backward', _pack(q, k, v, lam, mask, None, *ctx.call, None, lse, maps, ws, n), dout.data_ptr(), ptr(dq), ptr(dk),
+                   ptr(dv), ptr(dlam))
         return dq, dk if needs[1] else None, dv if needs[2] else None, dlam, None, None, None
 
 
 def _check(who, q, k, v, lam, scale):
-    for name, t, axes in (('q', q, '[B, N, H, 2, d]'), ('k', k, '[B, M, Hk, 2, d]'), ('v', v, '[B, M, Hk, 2 d]'), ('lam', lam, '[H]')):
-        require(torch.is_tensor(t) and t.dim() == axes.count(',') + 1, who, f'{name} must be a tensor {axes}')
-    dtype_code(q, who)
-    alike(who, q.dtype, q.device, k=k, v=v)
+    for name, t, axes in (('q', q, 5), ('k', k, 5), ('v', v, 4), ('lam', lam, 1)):
+        if not isinstance(t, torch.Tensor) or t.dim() != axes:
+            refuse(who, f'{name} must be a tensor of {axes} axes (q [B, N, H, 2, d], k [B, M, Hk, 2, d], v [B, M, Hk, 2 d], lam [H])')
+    dtype, device = q.dtype, q.device
+    if dtype not in DTYPES:
+        refuse(who, f'dtype {dtype} (float32, bfloat16 or float16)')
+    for name, t in (('k', k), ('v', v)):
+        if t.dtype != dtype or t.device != device:
+            alike(who, name, t, dtype, device)
     B, N, H, two, d = q.shape
-    require(two == 2 and d in (32, 64, 128), who, f'q {tuple(q.shape)} must be [B, N, H, 2, d] with d 32, 64 or 128')
-    Hk = k.shape[2]
-    require(tuple(k.shape) == (B, k.shape[1], Hk, 2, d), who, f'k {tuple(k.shape)} must be [{B}, M, Hk, 2, {d}]')
-    require(tuple(v.shape) == (B, k.shape[1], Hk, 2 * d), who, f'v {tuple(v.shape)} must be [{B}, {k.shape[1]}, {Hk}, {2 * d}]')
-    require(H >= 1 and Hk >= 1 and H % Hk == 0, who, f'{H} query heads must be a multiple of {Hk} key heads')
-    require(tuple(lam.shape) == (H,) and lam.device == q.device and lam.dtype in (q.dtype, torch.float32), who,
-            f'lam must be [{H}] on {q.device}, float32 or of the type of q')
+    kB, M, Hk, ktwo, kd = k.shape
+    if two != 2 or d not in (32, 64, 128):
+        refuse(who, f'q {tuple(q.shape)} must be [B, N, H, 2, d] with d 32, 64 or 128')
+    if kB != B or ktwo != 2 or kd != d:
+        refuse(who, f'k {tuple(k.shape)} must be [{B}, M, Hk, 2, {d}]')
+    if v.shape != (B, M, Hk, 2 * d):
+        refuse(who, f'v {tuple(v.shape)} must be [{B}, {M}, {Hk}, {2 * d}]')
+    if H < 1 or Hk < 1 or H % Hk:
+        refuse(who, f'{H} query heads must be a multiple of {Hk} key heads')
+    if lam.shape[0] != H or lam.device != device or (lam.dtype != dtype and lam.dtype != torch.float32):
+        refuse(who, f'lam must be [{H}] on {device}, float32 or of the type of q')
     scale = d ** -0.5 if scale is None else float(scale)
-    require(0.0 < scale <= 1e30, who, 'scale must be positive')
+    if not 0.0 < scale <= 1e30:
+        refuse(who, 'scale must be positive')
     return scale
 
 

@@ -6,8 +6,8 @@
 // layer only), of its weight the column sum of g h, of its bias the column sum of g.
 //
 // Both directions move each value once (4 or 6 values of traffic per element) and do ~14 / 24 operations on it, so memory bounds them: a row lives in
-// the registers of TPR threads (NIT vectors of V values each), its sums are formed by lane exchanges (and 16 bytes of LDS where a row takes the whole
-// workgroup), and the weights stay in registers over the rows a workgroup walks.  All arithmetic is float; x' is rounded once on its way out and z
+// the registers of TPR threads (NIT vectors of V values each), its sums are formed by lane exchanges (and through LDS where a row takes several
+// waves), and the weights stay in registers over the rows a workgroup walks, each loaded while the one before is worked on.  All arithmetic is float; x' is rounded once on its way out and z
 // comes from the unrounded x'.  Column sums: one partial row per workgroup in float, added in the fixed order of the workgroups by a second launch,
 // so gradients do not depend on scheduling.
 #include "pgrf_experiments.h"
@@ -32,23 +32,41 @@ struct NormArgs {
   int want;                                        // bit k: quantity k of `part` is wanted
 };
 
+// A row is held by TPR threads with eight values each (one vector of 16 bits' values, two of float's, eight single ones where rows start at any address), so that a
+// wave's registers leave room for three others beside it; rows of up to 64 threads share a wave, longer ones take several and add up through LDS.
 template <int TPR>
-struct RowSum {                                     // sums over the TPR threads of a row
-  float (*buf)[2][4];
+struct RowSum {
+  float (*buf)[2][16];
   int turn = 0;
-  __device__ explicit RowSum(float (*b)[2][4]) : buf(b) {}
-  __device__ void two(float& a, float& b) {
+  __device__ explicit RowSum(float (*b)[2][16]) : buf(b) {}
+  __device__ __forceinline__ void two(float& a, float& b) {
     a = group_sum<(TPR < 64 ? TPR : 64)>(a);
     b = group_sum<(TPR < 64 ? TPR : 64)>(b);
     if constexpr (TPR > 64) {
       // two buffers in turn: whoever writes one a second time has passed the barrier behind every read of its first contents
-      const int w = threadIdx.x >> 6;
+      constexpr int W = TPR / 64;
+      const int w = threadIdx.x >> 6, w0 = w / W * W;
       if ((threadIdx.x & 63) == 0) { buf[turn][0][w] = a; buf[turn][1][w] = b; }
       __syncthreads();
-      a = (buf[turn][0][0] + buf[turn][0][1]) + (buf[turn][0][2] + buf[turn][0][3]);
-      b = (buf[turn][1][0] + buf[turn][1][1]) + (buf[turn][1][2] + buf[turn][1][3]);
+      a = b = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) { a += buf[turn][0][w0 + i]; b += buf[turn][1][w0 + i]; }
       turn ^= 1;
     }
+  }
+  __device__ __forceinline__ float one(float a) {
+    a = group_sum<(TPR < 64 ? TPR : 64)>(a);
+    if constexpr (TPR > 64) {
+      constexpr int W = TPR / 64;
+      const int w = threadIdx.x >> 6, w0 = w / W * W;
+      if ((threadIdx.x & 63) == 0) buf[turn][0][w] = a;
+      __syncthreads();
+      a = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) a += buf[turn][0][w0 + i];
+      turn ^= 1;
+    }
+    return a;
   }
 };
 
@@ -66,11 +84,15 @@ __device__ __forceinline__ void load_row(const void* p, long long at, int t, int
   }
 }
 
+__device__ __forceinline__ long long gate_row(const NormArgs& a, long long row) {
+  return a.rows >> 32 ? row / a.rpg : (long long)((unsigned)row / (unsigned)a.rpg);
+}
+
 template <typename T, int V, int TPR, int NIT>
-__global__ __launch_bounds__(256) void block_norm_kernel(NormArgs a) {
-  __shared__ float buf[2][2][4];
+__global__ __launch_bounds__((TPR > 256 ? TPR : 256), 4) void block_norm_kernel(NormArgs a) {
+  constexpr int RPB = TPR > 256 ? 1 : 256 / TPR;
+  __shared__ float buf[2][2][16];
   RowSum<TPR> sum(buf);
-  constexpr int RPB = 256 / TPR;
   const int t = threadIdx.x % TPR, C = a.C;
   const float inv = 1.f / (float)C;
   Vec<T, V> pw[NIT], pb[NIT], qw[NIT], qb[NIT];
@@ -78,40 +100,49 @@ __global__ __launch_bounds__(256) void block_norm_kernel(NormArgs a) {
   if (a.pb) load_row<T, V, TPR, NIT>(a.pb, 0, t, C, pb);
   if (a.qw) load_row<T, V, TPR, NIT>(a.qw, 0, t, C, qw);
   if (a.qb) load_row<T, V, TPR, NIT>(a.qb, 0, t, C, qb);
-  for (long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR; row < a.rows; row += (long long)gridDim.x * RPB) {
+  struct In { Vec<T, V> x[NIT], y[NIT], g[NIT]; };
+  auto load = [&](In& r, long long row) {
+    row = row < a.rows ? row : a.rows - 1;           // (a row behind the last: read again, not written)
+    load_row<T, V, TPR, NIT>(a.x, row * C, t, C, r.x);
+    if (a.y) load_row<T, V, TPR, NIT>(a.y, row * C, t, C, r.y);
+    if (a.gate) load_row<T, V, TPR, NIT>(a.gate, gate_row(a, row) * C, t, C, r.g);
+  };
+  const long long step = (long long)gridDim.x * RPB;
+  long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+  In in;
+  load(in, row);
+  // (the workgroup's rows go together: with TPR > 64 every thread meets every barrier)
+  for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += step, row += step) {
     const long long at = row * C;
-    Vec<T, V> xv[NIT], yv[NIT], gv[NIT];
-    load_row<T, V, TPR, NIT>(a.x, at, t, C, xv);
-    if (a.y) load_row<T, V, TPR, NIT>(a.y, at, t, C, yv);
-    if (a.gate) load_row<T, V, TPR, NIT>(a.gate, (a.rows >> 32 ? row / a.rpg : (unsigned)row / (unsigned)a.rpg) * C, t, C, gv);
+    const bool live = row < a.rows;
+    In next;
+    if (row0 + step < a.rows) load(next, row + step);   // (the next row is on its way while this one is worked on)
     float h[NIT][V], st[4] = {0.f, 1.f, 0.f, 1.f};
     auto stats = [&](float& mean, float& r) {       // of h
       mean = 0.f;
-      float s0 = 0.f, s1 = 0.f;
       if (a.layer) {
+        float s = 0.f;
 #pragma unroll
         for (int i = 0; i < NIT; ++i)
 #pragma unroll
-          for (int j = 0; j < V; ++j) s0 += h[i][j];
-        sum.two(s0, s1);
-        mean = s0 * inv;
+          for (int j = 0; j < V; ++j) s += h[i][j];
+        mean = sum.one(s) * inv;
       }
-      s0 = s1 = 0.f;
+      float s = 0.f;
 #pragma unroll
       for (int i = 0; i < NIT; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float d = (i * TPR + t) * V < C ? h[i][j] - mean : 0.f;
-          s0 = fmaf(d, d, s0);
+          s = fmaf(d, d, s);
         }
-      sum.two(s0, s1);
-      r = 1.f / sqrtf(fmaf(s0, inv, a.eps));
+      r = 1.f / sqrtf(fmaf(sum.one(s), inv, a.eps));
     };
     if (a.y) {
 #pragma unroll
       for (int i = 0; i < NIT; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) h[i][j] = (float)yv[i].e[j];
+        for (int j = 0; j < V; ++j) h[i][j] = (float)in.y[i].e[j];
       if (a.post) stats(st[0], st[1]);
 #pragma unroll
       for (int i = 0; i < NIT; ++i)
@@ -124,10 +155,10 @@ __global__ __launch_bounds__(256) void block_norm_kernel(NormArgs a) {
             if (a.pb) u += (float)pb[i].e[j];
           }
           u *= a.scale;
-          if (a.gate) u *= (float)gv[i].e[j];
-          h[i][j] = (float)xv[i].e[j] + u;
+          if (a.gate) u *= (float)in.g[i].e[j];
+          h[i][j] = (float)in.x[i].e[j] + u;
         }
-      if (a.xo) {
+      if (live) {
 #pragma unroll
         for (int i = 0; i < NIT; ++i) {
           const int c = (i * TPR + t) * V;
@@ -141,7 +172,7 @@ __global__ __launch_bounds__(256) void block_norm_kernel(NormArgs a) {
 #pragma unroll
       for (int i = 0; i < NIT; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) h[i][j] = (float)xv[i].e[j];
+        for (int j = 0; j < V; ++j) h[i][j] = (float)in.x[i].e[j];
     }
     if (a.pre) {
       stats(st[2], st[3]);
@@ -156,19 +187,20 @@ __global__ __launch_bounds__(256) void block_norm_kernel(NormArgs a) {
           if (a.qb) u += (float)qb[i].e[j];
           o.e[j] = (T)u;
         }
-        if (c < C) store_vec<T, V>((T*)a.z + at + c, o);
+        if (live && c < C) store_vec<T, V>((T*)a.z + at + c, o);
       }
     }
-    if (a.stats && t == 0) *(float4*)(a.stats + row * 4) = make_float4(st[0], st[1], st[2], st[3]);
+    if (a.stats && t == 0 && live) *(float4*)(a.stats + row * 4) = make_float4(st[0], st[1], st[2], st[3]);
+    in = next;
   }
 }
 
 // One workgroup = one chunk of rows inside one gate row, so the gate is a constant of the chunk (or every row has its own: rpg == 1).
 template <typename T, int V, int TPR, int NIT, bool LAYER>
-__global__ __launch_bounds__(256) void block_norm_bwd_kernel(NormArgs a) {
-  constexpr int RPB = 256 / TPR;
-  __shared__ float buf[2][2][4];
-  __shared__ float col[RPB > 1 ? 256 * NIT * V : 1];
+__global__ __launch_bounds__((TPR > 256 ? TPR : 256), (TPR > 512 ? 4 : LAYER ? 2 : 3)) void block_norm_bwd_kernel(NormArgs a) {
+  constexpr int WG = TPR > 256 ? TPR : 256, RPB = WG / TPR;
+  __shared__ float buf[2][2][16];
+  __shared__ float col[RPB > 1 ? WG * NIT * V : 1];
   RowSum<TPR> sum(buf);
   const int t = threadIdx.x % TPR, C = a.C;
   const float inv = 1.f / (float)C;
@@ -189,64 +221,73 @@ __global__ __launch_bounds__(256) void block_norm_bwd_kernel(NormArgs a) {
   for (int i = 0; i < NIT; ++i)
 #pragma unroll
     for (int j = 0; j < V; ++j) aw[i][j] = ab[i][j] = cw[i][j] = cb[i][j] = 0.f;
-  // (the loop bounds are those of the workgroup: with TPR > 64 every thread meets every barrier)
-  for (long long row0 = first; row0 < last; row0 += RPB) {
-    const long long row = row0 + threadIdx.x / TPR;
-    const bool live = row < last;
-    if (RPB > 1 && !live) continue;
+  struct In { Vec<T, V> x[NIT], y[NIT], dx[NIT], dz[NIT], g[NIT]; float4 st; };
+  auto load = [&](In& r, long long row) {
+    row = row < last ? row : last - 1;               // (a row behind the chunk: read again, not counted)
     const long long at = row * C;
-    const float4 st = *(const float4*)(a.stats + row * 4);
-    Vec<T, V> xv[NIT], yv[NIT], dxv[NIT], dzv[NIT];
-    if (a.pre) load_row<T, V, TPR, NIT>(a.x, at, t, C, xv);
-    if (a.y) load_row<T, V, TPR, NIT>(a.y, at, t, C, yv);
-    if (a.dxo) load_row<T, V, TPR, NIT>(a.dxo, at, t, C, dxv);
-    if (a.pre && a.dz) load_row<T, V, TPR, NIT>(a.dz, at, t, C, dzv);
-    // (row, not row / rpg: rpg is 1 here)
-    if (per_row) load_row<T, V, TPR, NIT>(a.gate, at, t, C, gv);
+    r.st = *(const float4*)(a.stats + row * 4);
+    if (a.pre && a.dz) {
+      load_row<T, V, TPR, NIT>(a.x, at, t, C, r.x);
+      load_row<T, V, TPR, NIT>(a.dz, at, t, C, r.dz);
+    }
+    if (a.y) load_row<T, V, TPR, NIT>(a.y, at, t, C, r.y);
+    if (a.dxo) load_row<T, V, TPR, NIT>(a.dxo, at, t, C, r.dx);
+    if (per_row) load_row<T, V, TPR, NIT>(a.gate, at, t, C, r.g);
+  };
+  In in;
+  long long row = first + threadIdx.x / TPR;
+  if (first < last) load(in, row);
+  // (the loop bounds are those of the workgroup: with TPR > 64 every thread meets every barrier)
+  for (long long row0 = first; row0 < last; row0 += RPB, row += RPB) {
+    const bool live = row < last;
+    const long long at = row * C;
+    In next;
+    if (row0 + RPB < last) load(next, row + RPB);   // (the next row is on its way while this one is worked on)
+    const float4 st = in.st;
+    auto gate_of = [&](int i, int j) { return a.gate ? (float)(per_row ? in.g[i].e[j] : gv[i].e[j]) : 1.f; };
     float dh[NIT][V];
 #pragma unroll
     for (int i = 0; i < NIT; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) dh[i][j] = a.dxo ? (float)dxv[i].e[j] : 0.f;
+      for (int j = 0; j < V; ++j) dh[i][j] = a.dxo ? (float)in.dx[i].e[j] : 0.f;
     if (a.pre && a.dz) {
       // x' is formed again from x and y, unrounded: a rounded x' would put its rounding into the gradients of the norm behind it
-      auto hat_of = [&](int i, int j) {
-        float v = (float)xv[i].e[j];
-        if (a.y) {
-          float u = (float)yv[i].e[j];
-          if (a.post) {
-            u = (u - st.x) * st.y;
-            if (a.pw) u *= (float)pw[i].e[j];
-            if (a.pb) u += (float)pb[i].e[j];
-          }
-          u *= a.scale;
-          if (a.gate) u *= (float)gv[i].e[j];
-          v += u;
-        }
-        return (v - st.z) * st.w;
-      };
-      float s0 = 0.f, s1 = 0.f;
+      float hat[NIT][V], s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int i = 0; i < NIT; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {               // (columns behind C: dz was loaded as 0)
-          const float hat = hat_of(i, j), g = (float)dzv[i].e[j], tt = a.qw ? g * (float)qw[i].e[j] : g;
+          float v = (float)in.x[i].e[j];
+          if (a.y) {
+            float u = (float)in.y[i].e[j];
+            if (a.post) {
+              u = (u - st.x) * st.y;
+              if (a.pw) u *= (float)pw[i].e[j];
+              if (a.pb) u += (float)pb[i].e[j];
+            }
+            u *= a.scale;
+            if (a.gate) u *= gate_of(i, j);
+            v += u;
+          }
+          hat[i][j] = (v - st.z) * st.w;
+          const float g = live ? (float)in.dz[i].e[j] : 0.f, tt = a.qw ? g * (float)qw[i].e[j] : g;
           if (LAYER) { s0 += tt; cb[i][j] += g; }
-          s1 = fmaf(tt, hat, s1);
-          cw[i][j] = fmaf(g, hat, cw[i][j]);
+          s1 = fmaf(tt, hat[i][j], s1);
+          cw[i][j] = live ? fmaf(g, hat[i][j], cw[i][j]) : cw[i][j];   // (a row that counts twice may be NaN, and 0 * NaN is NaN)
         }
-      sum.two(s0, s1);
+      if (LAYER) sum.two(s0, s1);
+      else s1 = sum.one(s1);
       s0 *= inv;
       s1 *= inv;
 #pragma unroll
       for (int i = 0; i < NIT; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float hat = hat_of(i, j), g = (float)dzv[i].e[j], tt = a.qw ? g * (float)qw[i].e[j] : g;
-          dh[i][j] += st.w * ((LAYER ? tt - s0 : tt) - hat * s1);
+          const float g = (float)in.dz[i].e[j], tt = a.qw ? g * (float)qw[i].e[j] : g;
+          dh[i][j] += st.w * ((LAYER ? tt - s0 : tt) - hat[i][j] * s1);
         }
     }
-    if (a.dx) {
+    if (a.dx && live) {
 #pragma unroll
       for (int i = 0; i < NIT; ++i) {
         const int c = (i * TPR + t) * V;
@@ -263,12 +304,12 @@ __global__ __launch_bounds__(256) void block_norm_bwd_kernel(NormArgs a) {
         Vec<T, V> o;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const bool in = (i * TPR + t) * V < C;    // (behind C the gradient of the pre norm left something)
-          const float d = in ? dh[i][j] : 0.f, gate = a.gate ? (float)gv[i].e[j] : 1.f;
-          const float hat = a.post ? ((float)yv[i].e[j] - st.x) * st.y : (float)yv[i].e[j];
+          const bool in_row = (i * TPR + t) * V < C && live;    // (behind C the gradient of the pre norm left something)
+          const float d = in_row ? dh[i][j] : 0.f, gate = gate_of(i, j);
+          const float hat = a.post ? ((float)in.y[i].e[j] - st.x) * st.y : (float)in.y[i].e[j];
           const float w = a.pw ? (float)pw[i].e[j] : 1.f;
           const float ge = per_row ? gate * d : d;
-          aw[i][j] = fmaf(ge, hat, aw[i][j]);
+          aw[i][j] = live ? fmaf(ge, hat, aw[i][j]) : aw[i][j];
           if (LAYER) ab[i][j] += ge;
           if (own_gate) o.e[j] = (T)(a.scale * d * fmaf(hat, w, a.pb ? (float)pb[i].e[j] : 0.f));
           const float tt = a.scale * gate * d * w;
@@ -277,27 +318,29 @@ __global__ __launch_bounds__(256) void block_norm_bwd_kernel(NormArgs a) {
           dh[i][j] = tt;
         }
         const int c = (i * TPR + t) * V;
-        if (own_gate && c < C) store_vec<T, V>((T*)a.dgate + at + c, o);
+        if (own_gate && live && c < C) store_vec<T, V>((T*)a.dgate + at + c, o);
       }
       if (a.post) {
-        sum.two(s0, s1);
+        if (LAYER) sum.two(s0, s1);
+        else s1 = sum.one(s1);
         s0 *= inv;
         s1 *= inv;
       }
-      if (a.dy) {
+      if (a.dy && live) {
 #pragma unroll
         for (int i = 0; i < NIT; ++i) {
           const int c = (i * TPR + t) * V;
           Vec<T, V> o;
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            const float hat = ((float)yv[i].e[j] - st.x) * st.y;
+            const float hat = ((float)in.y[i].e[j] - st.x) * st.y;
             o.e[j] = (T)(a.post ? st.y * ((LAYER ? dh[i][j] - s0 : dh[i][j]) - hat * s1) : dh[i][j]);
           }
           if (c < C) store_vec<T, V>((T*)a.dy + at + c, o);
         }
       }
     }
+    in = next;
   }
   // the chunk's column sums: RPB rows side by side are added in LDS, in order
   auto across = [&](float (&v)[NIT][V]) {
@@ -306,22 +349,21 @@ __global__ __launch_bounds__(256) void block_norm_bwd_kernel(NormArgs a) {
 #pragma unroll
       for (int i = 0; i < NIT; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) col[(i * V + j) * 256 + threadIdx.x] = v[i][j];
+        for (int j = 0; j < V; ++j) col[(i * V + j) * WG + threadIdx.x] = v[i][j];
       __syncthreads();
       if (threadIdx.x < TPR)
         for (int k = 1; k < RPB; ++k)
 #pragma unroll
           for (int i = 0; i < NIT; ++i)
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[i][j] += col[(i * V + j) * 256 + k * TPR + t];
+            for (int j = 0; j < V; ++j) v[i][j] += col[(i * V + j) * WG + k * TPR + t];
     }
   };
   if (!a.want) return;
-  const bool use_b = LAYER;
   if (a.y) across(aw);
-  if (a.y && use_b) across(ab);
+  if (a.y && LAYER) across(ab);
   if (a.pre) across(cw);
-  if (a.pre && use_b) across(cb);
+  if (a.pre && LAYER) across(cb);
   if (threadIdx.x >= TPR) return;
   float* out = a.part + (long long)blockIdx.x * 5 * C;
 #pragma unroll
@@ -343,40 +385,41 @@ __global__ __launch_bounds__(256) void block_norm_bwd_kernel(NormArgs a) {
     }
 }
 
-// Adds the partial rows of a column: 64 columns x 4 shares of the chunks per workgroup; blockIdx.y = quantity (0..3) or 4 + gate row
+// Adds the partial rows of a column: W columns x 1024 / W shares of the chunks per workgroup; blockIdx.y = quantity (0..3) or 4 + gate row
 template <typename T>
-__global__ __launch_bounds__(256) void column_sum_kernel(const float* part, long long chunks, int cpg, int C, void* o0, void* o1, void* o2, void* o3,
-                                                         void* o4) {
-  __shared__ float s[4][64];
+__global__ __launch_bounds__(1024) void column_sum_kernel(const float* part, long long chunks, int cpg, int C, int W, void* o0, void* o1, void* o2, void* o3,
+                                                          void* o4) {
+  __shared__ float s[1024];
   const int k = blockIdx.y < 4 ? blockIdx.y : 4;
   void* o = k == 0 ? o0 : k == 1 ? o1 : k == 2 ? o2 : k == 3 ? o3 : o4;
   if (!o) return;
   const long long gr = (long long)blockIdx.y - 4, lo = k < 4 ? 0 : gr * cpg, n = k < 4 ? chunks : cpg;
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), share = threadIdx.x >> 6;
+  const int x = threadIdx.x % W, c = blockIdx.x * W + x, share = threadIdx.x / W, shares = 1024 / W;
   float v = 0.f;
   if (c < C) {
     const float* p = part + ((lo * 5 + k) * C + c);
-    float u[4] = {0.f, 0.f, 0.f, 0.f};
+    float u[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     long long i = share;
-    for (; i + 12 < n; i += 16)
+    for (; i + 7 * shares < n; i += 8 * shares)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) u[j] += p[(i + 4 * j) * 5 * C];
-    for (; i < n; i += 4) u[0] += p[i * 5 * C];
-    v = (u[0] + u[1]) + (u[2] + u[3]);
+      for (int j = 0; j < 8; ++j) u[j] += p[(i + j * shares) * 5 * C];
+    for (int j = 0; i < n; i += shares, ++j) u[j & 7] += p[i * 5 * C];
+    v = ((u[0] + u[1]) + (u[2] + u[3])) + ((u[4] + u[5]) + (u[6] + u[7]));
   }
-  s[share][threadIdx.x & 63] = v;
-  __syncthreads();
-  if (share == 0 && c < C) {
-    const int x = threadIdx.x & 63;
-    ((T*)o)[(k < 4 ? 0 : gr * C) + c] = (T)((s[0][x] + s[1][x]) + (s[2][x] + s[3][x]));
+  s[threadIdx.x] = v;
+  for (int d = shares / 2; d >= 1; d /= 2) {
+    __syncthreads();
+    if (share < d) s[threadIdx.x] += s[threadIdx.x + d * W];
   }
+  if (share == 0 && c < C) ((T*)o)[(k < 4 ? 0 : gr * C) + c] = (T)s[x];
 }
 
-// chunks: enough workgroups to fill the chip several times over, none across a gate row
+// chunks: as many workgroups as the chip holds at a time (three per CU, two for the layer norm's registers), none across a gate row
 static long long cut_rows(NormArgs& a, int rpb) {
   a.span = a.gate && a.rpg > 1 ? a.rpg : a.rows;
   const long long gates = a.rows / a.span;         // (check_norm: rows divide into gate rows)
-  long long cpg = (1024 + gates - 1) / gates;
+  const long long want = a.layer ? 512 : 768;
+  long long cpg = (want + gates - 1) / gates;
   const long long most = (a.span + rpb - 1) / rpb;
   if (cpg > most) cpg = most;
   a.rpc = (a.span + cpg - 1) / cpg;
@@ -387,26 +430,13 @@ static long long cut_rows(NormArgs& a, int rpb) {
 
 struct Shape { int v, tpr, nit; };
 
-// A row takes as few threads as hold it in one to four vectors each (up to 32 single values where rows start at any address): a wave then walks
-// several rows at once and the sums stay inside it.  C = 1 024 in 16 bits: a wave per row with two vectors per lane.
 static Shape shape_for(int C, int dtype, bool vec) {
   const int v = vec ? (dtype == PGRF_DTYPE_F32 ? 4 : 8) : 1;
-  const int n = (C + v - 1) / v;
-  if (vec) {
-    if (n <= 4) return {v, 4, 1};
-    if (n <= 16) return {v, 16, 1};
-    if (n <= 64) return {v, 64, 1};
-    if (n <= 128) return {v, 64, 2};
-    if (n <= 256) return {v, 256, 1};
-    if (n <= 512) return {v, 256, 2};
-    if (n <= 1024) return {v, 256, 4};
-    return {v, 256, 8};
-  }
-  if (n <= 16) return {1, 16, 1};
-  if (n <= 64) return {1, 16, 4};
-  if (n <= 256) return {1, 64, 4};
-  if (n <= 1024) return {1, 256, 4};
-  return {1, 256, 32};
+  const int n = (C + 7) / 8;                         // threads of eight values
+  if (v == 4 && C <= 16) return {4, 4, 1};
+  if (v == 1 && C <= 16) return {1, 16, 1};
+  int tpr = n <= 4 ? 4 : n <= 16 ? 16 : n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : n <= 512 ? 512 : 1024;
+  return {v, tpr, 8 / v};
 }
 
 static bool rows_vectorise(int C, int dtype, const void* const* ps, int n) {
@@ -418,13 +448,14 @@ static bool rows_vectorise(int C, int dtype, const void* const* ps, int n) {
 
 template <typename T, int V, int TPR, int NIT>
 static void run_norm(const NormArgs& a, long long chunks, bool bwd, hipStream_t s) {
+  constexpr int WG = TPR > 256 ? TPR : 256;
   if (bwd) {
-    if (a.layer) hipLaunchKernelGGL((block_norm_bwd_kernel<T, V, TPR, NIT, true>), dim3((unsigned)chunks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((block_norm_bwd_kernel<T, V, TPR, NIT, false>), dim3((unsigned)chunks), dim3(256), 0, s, a);
+    if (a.layer) hipLaunchKernelGGL((block_norm_bwd_kernel<T, V, TPR, NIT, true>), dim3((unsigned)chunks), dim3(WG), 0, s, a);
+    else hipLaunchKernelGGL((block_norm_bwd_kernel<T, V, TPR, NIT, false>), dim3((unsigned)chunks), dim3(WG), 0, s, a);
     return;
   }
-  const long long need = (a.rows + 256 / TPR - 1) / (256 / TPR);
-  hipLaunchKernelGGL((block_norm_kernel<T, V, TPR, NIT>), dim3((unsigned)(need < 4096 ? need : 4096)), dim3(256), 0, s, a);
+  const long long need = (a.rows + WG / TPR - 1) / (WG / TPR), most = 8 * 256 * 256 / WG;
+  hipLaunchKernelGGL((block_norm_kernel<T, V, TPR, NIT>), dim3((unsigned)(need < most ? need : most)), dim3(WG), 0, s, a);
 }
 
 template <typename T>
@@ -432,19 +463,14 @@ static void pick_norm(const NormArgs& a, const Shape& h, long long chunks, bool 
   constexpr int V = 16 / sizeof(T);
 #define PGRF_NORM(VV, TT, NN) \
   if (h.v == VV && h.tpr == TT && h.nit == NN) return run_norm<T, VV, TT, NN>(a, chunks, bwd, s)
-  PGRF_NORM(V, 4, 1);
-  PGRF_NORM(V, 16, 1);
-  PGRF_NORM(V, 64, 1);
-  PGRF_NORM(V, 64, 2);
-  PGRF_NORM(V, 256, 1);
-  PGRF_NORM(V, 256, 2);
-  PGRF_NORM(V, 256, 4);
-  if constexpr (V == 4) { PGRF_NORM(V, 256, 8); }
+#define PGRF_NORMS(VV) \
+  PGRF_NORM(VV, 4, 8 / VV); PGRF_NORM(VV, 16, 8 / VV); PGRF_NORM(VV, 64, 8 / VV); PGRF_NORM(VV, 128, 8 / VV); PGRF_NORM(VV, 256, 8 / VV); \
+  PGRF_NORM(VV, 512, 8 / VV); PGRF_NORM(VV, 1024, 8 / VV)
+  PGRF_NORMS(V);
+  PGRF_NORMS(1);
+  if constexpr (V == 4) { PGRF_NORM(4, 4, 1); }
   PGRF_NORM(1, 16, 1);
-  PGRF_NORM(1, 16, 4);
-  PGRF_NORM(1, 64, 4);
-  PGRF_NORM(1, 256, 4);
-  PGRF_NORM(1, 256, 32);
+#undef PGRF_NORMS
 #undef PGRF_NORM
 }
 
@@ -465,6 +491,15 @@ static int check_norm(const char* who, int dtype, long long rows, int C, int fla
   return PGRF_OK;
 }
 
+static NormArgs args_of(const PgrfBlockNorm* p) {
+  NormArgs a = {};
+  a.post = (p->flags & PGRF_NORM_POST) ? 1 : 0; a.pre = (p->flags & PGRF_NORM_PRE) ? 1 : 0; a.layer = (p->flags & PGRF_NORM_LAYER) ? 1 : 0;
+  a.x = p->x; a.y = p->y; a.gate = p->gate; a.rpg = p->gate ? p->rows_per_gate : (p->rows ? p->rows : 1);
+  a.pw = a.post ? p->post_w : nullptr; a.pb = a.post && a.layer ? p->post_b : nullptr; a.qw = a.pre ? p->pre_w : nullptr;
+  a.stats = p->stats; a.rows = p->rows; a.C = p->C; a.scale = p->scale;
+  return a;
+}
+
 }  // namespace tok
 }  // namespace pgrf
 
@@ -473,75 +508,68 @@ using namespace pgrf::tok;
 
 extern "C" {
 
-int pgrf_block_norm(const void* x, const void* y, const void* gate, long long rows_per_gate, const void* post_w, const void* post_b,
-                    const void* pre_w, const void* pre_b, int dtype, long long rows, int C, int flags, float scale, float eps, void* x_out,
-                    void* z_out, float* stats, void* stream) {
+int pgrf_block_norm(const PgrfBlockNorm* p, void* stream) {
   const char* who = "pgrf_block_norm";
-  int rc = check_norm(who, dtype, rows, C, flags, rows_per_gate, y, gate);
+  if (!p) return set_error(PGRF_ERR_ARG, "%s: null arguments", who);
+  int rc = check_norm(who, p->dtype, p->rows, p->C, p->flags, p->rows_per_gate, p->y, p->gate);
   if (rc) return rc;
-  if (rows == 0) return PGRF_OK;
-  if (!x || (y && !x_out) || ((flags & PGRF_NORM_PRE) && !z_out)) return set_error(PGRF_ERR_ARG, "%s: null x / x_out / z_out", who);
-  if (stats && !aligned16(stats)) return set_error(PGRF_ERR_ARG, "%s: stats must be 16-byte aligned", who);
-  NormArgs a = {};
-  a.x = x; a.y = y; a.gate = gate; a.rpg = gate ? rows_per_gate : rows;
-  a.post = (flags & PGRF_NORM_POST) ? 1 : 0; a.pre = (flags & PGRF_NORM_PRE) ? 1 : 0; a.layer = (flags & PGRF_NORM_LAYER) ? 1 : 0;
-  a.pw = a.post ? post_w : nullptr; a.pb = a.post && a.layer ? post_b : nullptr;
-  a.qw = a.pre ? pre_w : nullptr; a.qb = a.pre && a.layer ? pre_b : nullptr;
-  a.xo = y ? x_out : nullptr; a.z = z_out; a.stats = stats; a.rows = rows; a.C = C; a.scale = scale; a.eps = eps;
-  const void* ps[] = {x, y, gate, a.pw, a.pb, a.qw, a.qb, a.xo, a.pre ? z_out : nullptr};
-  dispatch_norm(a, dtype, shape_for(C, dtype, rows_vectorise(C, dtype, ps, 9)), 0, false, (hipStream_t)stream);
+  if (p->rows == 0) return PGRF_OK;
+  if (!p->x || (p->y && !p->x_out) || ((p->flags & PGRF_NORM_PRE) && !p->z_out)) return set_error(PGRF_ERR_ARG, "%s: null x / x_out / z_out", who);
+  if (p->stats && !aligned16(p->stats)) return set_error(PGRF_ERR_ARG, "%s: stats must be 16-byte aligned", who);
+  NormArgs a = args_of(p);
+  a.qb = a.pre && a.layer ? p->pre_b : nullptr;
+  a.xo = p->y ? p->x_out : nullptr; a.z = p->z_out; a.eps = p->eps;
+  const void* ps[] = {a.x, a.y, a.gate, a.pw, a.pb, a.qw, a.qb, a.xo, a.pre ? a.z : nullptr};
+  dispatch_norm(a, p->dtype, shape_for(p->C, p->dtype, rows_vectorise(p->C, p->dtype, ps, 9)), 0, false, (hipStream_t)stream);
   PGRF_TOK_LAUNCHED(who);
   return PGRF_OK;
 }
 
 size_t pgrf_block_norm_backward_workspace_bytes(long long rows, int C, long long rows_per_gate) {
   if (rows < 1 || C < 1 || rows_per_gate < 1) return 16;
-  // an upper bound of cut_rows' chunks for every row split: at most 1 024 chunks plus one per gate row
+  // an upper bound of cut_rows' chunks: 768, plus one for each gate row
   const long long gates = rows_per_gate > 1 ? (rows + rows_per_gate - 1) / rows_per_gate : 1;
-  return (size_t)(1024 + gates) * 5 * (size_t)C * sizeof(float);
+  return (size_t)(768 + gates) * 5 * (size_t)C * sizeof(float);
 }
 
-int pgrf_block_norm_backward(const void* x, const void* y, const void* gate, long long rows_per_gate, const void* post_w, const void* post_b,
-                             const void* pre_w, const float* stats, const void* dx_out, const void* dz, int dtype, long long rows, int C, int flags,
-                             float scale, void* dx, void* dy, void* dgate, void* dpost_w, void* dpost_b, void* dpre_w, void* dpre_b, void* workspace,
-                             size_t workspace_bytes, void* stream) {
+int pgrf_block_norm_backward(const PgrfBlockNorm* p, void* stream) {
   const char* who = "pgrf_block_norm_backward";
-  int rc = check_norm(who, dtype, rows, C, flags, rows_per_gate, y, gate);
+  if (!p) return set_error(PGRF_ERR_ARG, "%s: null arguments", who);
+  int rc = check_norm(who, p->dtype, p->rows, p->C, p->flags, p->rows_per_gate, p->y, p->gate);
   if (rc) return rc;
-  if (dgate && !gate) return set_error(PGRF_ERR_ARG, "%s: dgate without gate", who);
-  NormArgs a = {};
-  a.post = (flags & PGRF_NORM_POST) ? 1 : 0; a.pre = (flags & PGRF_NORM_PRE) ? 1 : 0; a.layer = (flags & PGRF_NORM_LAYER) ? 1 : 0;
-  if (rows && (!stats || (a.pre && !x))) return set_error(PGRF_ERR_ARG, "%s: null stats / x", who);
-  if (rows && !aligned16(stats)) return set_error(PGRF_ERR_ARG, "%s: stats must be 16-byte aligned", who);
-  a.x = x; a.y = y; a.gate = gate; a.rpg = gate ? rows_per_gate : (rows ? rows : 1);
-  a.pw = a.post ? post_w : nullptr; a.pb = a.post && a.layer ? post_b : nullptr; a.qw = a.pre ? pre_w : nullptr;
-  a.stats = const_cast<float*>(stats); a.rows = rows; a.C = C; a.scale = scale;
-  a.dxo = dx_out; a.dz = a.pre ? dz : nullptr; a.dx = dx; a.dy = y ? dy : nullptr;
-  const bool per_row = gate && rows_per_gate == 1;
-  a.dgate = per_row ? dgate : nullptr;
-  a.part = (float*)workspace;
-  a.want = (a.post && dpost_w ? 1 : 0) | (a.post && a.layer && dpost_b ? 2 : 0) | (a.pre && dpre_w ? 4 : 0) | (a.pre && a.layer && dpre_b ? 8 : 0) |
-           (dgate && !per_row ? 16 : 0);
-  const void* ps[] = {x, y, gate, a.pw, a.pb, a.qw, dx_out, dz, dx, dy, a.dgate};
-  const Shape h = shape_for(C, dtype, rows_vectorise(C, dtype, ps, 11));
+  if (p->dgate && !p->gate) return set_error(PGRF_ERR_ARG, "%s: dgate without gate", who);
+  NormArgs a = args_of(p);
+  if (p->rows && (!p->stats || !p->x)) return set_error(PGRF_ERR_ARG, "%s: null stats / x", who);
+  if (p->rows && !aligned16(p->stats)) return set_error(PGRF_ERR_ARG, "%s: stats must be 16-byte aligned", who);
+  a.dxo = p->dx_out; a.dz = a.pre ? p->dz : nullptr; a.dx = p->dx; a.dy = p->y ? p->dy : nullptr;
+  const bool per_row = p->gate && p->rows_per_gate == 1;
+  a.dgate = per_row ? p->dgate : nullptr;
+  a.part = (float*)p->workspace;
+  a.want = (a.post && p->dpost_w ? 1 : 0) | (a.post && a.layer && p->dpost_b ? 2 : 0) | (a.pre && p->dpre_w ? 4 : 0) | (a.pre && a.layer && p->dpre_b ? 8 : 0) |
+           (p->dgate && !per_row ? 16 : 0);
+  const void* ps[] = {a.x, a.y, a.gate, a.pw, a.pb, a.qw, a.dxo, a.dz, a.dx, a.dy, a.dgate};
+  const int C = p->C;
+  const Shape h = shape_for(C, p->dtype, rows_vectorise(C, p->dtype, ps, 11));
   long long chunks = 0;
   a.cpg = 1;
-  const long long gates = (a.want & 16) && rows ? rows / rows_per_gate : 0;
+  const long long gates = (a.want & 16) && p->rows ? p->rows / p->rows_per_gate : 0;
   if (gates > 60000) return set_error(PGRF_ERR_UNSUPPORTED, "%s: %lld gate rows (at most 60000, or one for each row)", who, gates);
-  if (rows) {
-    chunks = cut_rows(a, 256 / h.tpr);
-    if (a.want && (!workspace || workspace_bytes < (size_t)chunks * 5 * C * sizeof(float)))
-      return set_error(PGRF_ERR_ARG, "%s: workspace too small (%zu < %zu bytes)", who, workspace_bytes, (size_t)chunks * 5 * C * sizeof(float));
-    dispatch_norm(a, dtype, h, chunks, true, (hipStream_t)stream);
+  if (p->rows) {
+    chunks = cut_rows(a, h.tpr > 256 ? 1 : 256 / h.tpr);
+    const size_t need = (size_t)chunks * 5 * C * sizeof(float);
+    if (a.want && (!p->workspace || p->workspace_bytes < need)) return set_error(PGRF_ERR_ARG, "%s: workspace too small (%zu < %zu bytes)", who, p->workspace_bytes, need);
+    dispatch_norm(a, p->dtype, h, chunks, true, (hipStream_t)stream);
     PGRF_TOK_LAUNCHED(who);
   }
   if (a.want) {
-    const dim3 grid((C + 63) / 64, 4 + (unsigned)gates);
-    void *o0 = a.want & 1 ? dpost_w : nullptr, *o1 = a.want & 2 ? dpost_b : nullptr, *o2 = a.want & 4 ? dpre_w : nullptr,
-         *o3 = a.want & 8 ? dpre_b : nullptr, *o4 = a.want & 16 ? dgate : nullptr;
-#define PGRF_COLS(T) hipLaunchKernelGGL(column_sum_kernel<T>, grid, dim3(256), 0, (hipStream_t)stream, a.part, chunks, a.cpg, C, o0, o1, o2, o3, o4)
-    if (dtype == PGRF_DTYPE_F32) PGRF_COLS(float);
-    else if (dtype == PGRF_DTYPE_BF16) PGRF_COLS(bf16);
+    int W = 64;
+    while (W > 4 && W / 2 >= C) W /= 2;
+    const dim3 grid((C + W - 1) / W, 4 + (unsigned)gates);
+    void *o0 = a.want & 1 ? p->dpost_w : nullptr, *o1 = a.want & 2 ? p->dpost_b : nullptr, *o2 = a.want & 4 ? p->dpre_w : nullptr,
+         *o3 = a.want & 8 ? p->dpre_b : nullptr, *o4 = a.want & 16 ? p->dgate : nullptr;
+#define PGRF_COLS(T) hipLaunchKernelGGL(column_sum_kernel<T>, grid, dim3(1024), 0, (hipStream_t)stream, a.part, chunks, a.cpg, C, W, o0, o1, o2, o3, o4)
+    if (p->dtype == PGRF_DTYPE_F32) PGRF_COLS(float);
+    else if (p->dtype == PGRF_DTYPE_BF16) PGRF_COLS(bf16);
     else PGRF_COLS(f16);
 #undef PGRF_COLS
     PGRF_TOK_LAUNCHED(who);

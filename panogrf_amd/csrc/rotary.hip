@@ -14,7 +14,7 @@
 namespace pgrf {
 namespace tok {
 
-constexpr int kMaxPairs = PGRF_ROTARY_MAX_DIM / 2;
+constexpr int kMaxPairs = PGRF_ROTARY_MAX_DIM / 2, kMaxTile = 64;
 
 struct Strided { const void* in; void* out; long long sb, sn, sh; int heads; };   // in: [B,N,heads,D] by strides; out: contiguous
 
@@ -34,15 +34,30 @@ __device__ __forceinline__ int quick_div(int n, float inv) { return (int)(((floa
 
 enum { kPairs = 0, kHalves = 1, kAnyHalves = 2 };
 
+// An item is what a thread moves at a time: V neighbouring channels (interleaved pairs, or halves that vectors straddle), or two vectors - V pairs, or what
+// is copied behind them.  A thread has two items on their way at once.
 template <typename T, int V, int HOW>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   extern __shared__ float2 turn[];                   // [tile][rot/2]: cos, sin
+  __shared__ long long from[2][kMaxTile];            // where a token's query and key heads start
   const int half = a.rot >> 1;
   const long long tokens = (long long)a.B * a.N, t0 = (long long)blockIdx.x * a.tile;
   const int here = tokens - t0 < a.tile ? (int)(tokens - t0) : a.tile;
+  const long long b0 = t0 / a.N, n0 = t0 - b0 * a.N;
+  auto place = [&](int k, long long& b, long long& n) {   // batch entry and place of the tile's token k
+    b = b0;
+    n = n0 + k;
+    if (n >= a.N) {
+      const unsigned more = (unsigned)n / (unsigned)a.N;   // (n < 2^31 + a tile)
+      b += more;
+      n -= (long long)more * a.N;
+    }
+  };
   for (int i = threadIdx.x; i < here * half; i += 256) {
     const int k = i / half, pair = i - k * half;
-    const long long tok = t0 + k, b = tok / a.N, at = b * a.pos_b + (tok - b * a.N);
+    long long b, n;
+    place(k, b, n);
+    const long long at = b * a.pos_b + n;
     const double p = a.pos_kind == 0 ? (double)((const int*)a.pos)[at] : a.pos_kind == 1 ? (double)((const long long*)a.pos)[at]
                    : a.pos_kind == 2 ? (double)((const float*)a.pos)[at] : ((const double*)a.pos)[at];
     const double r = p * a.rev[pair];
@@ -51,72 +66,91 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     sincospif(f, &s, &c);
     turn[i] = make_float2(c * a.magnitude, s * a.magnitude * a.sign);
   }
+  if ((int)threadIdx.x < 2 * here) {
+    const int k = threadIdx.x >> 1, w = threadIdx.x & 1;
+    long long b, n;
+    place(k, b, n);
+    from[w][k] = b * a.x[w].sb + n * a.x[w].sn;
+  }
   __syncthreads();
-  const int total = here * a.items;
-  for (int it = threadIdx.x; it < total; it += 256) {
+  const int total = here * a.items, np = half / V;
+  struct Item { Vec<T, V> u, w; T* out; const T* in; const float2* cs; int j; bool has_w; };
+  auto bring = [&](Item& m, int it) {
     const int k = quick_div(it, a.inv_items), rem = it - k * a.items;
     int head = quick_div(rem, a.inv_per_head);
-    const int j = rem - head * a.per_head;
-    const long long tok = t0 + k, b = tok / a.N, n = tok - b * a.N;
+    m.j = rem - head * a.per_head;
     const int which = head >= a.x[0].heads ? 1 : 0;
-    const Strided& x = a.x[which];
     if (which) head -= a.x[0].heads;
-    const T* in = (const T*)x.in + b * x.sb + n * x.sn + head * x.sh;
-    T* out = (T*)x.out + (tok * x.heads + head) * a.D;
-    const float2* cs = turn + k * half;
-    if constexpr (HOW == kHalves) {                  // an item = V pairs (two vectors), or a vector behind `rot`
-      const int np = half / V;
-      if (j < np) {
-        const int c0 = j * V;
-        const Vec<T, V> u = load_vec<T, V>(in + c0), w = load_vec<T, V>(in + c0 + half);
-        Vec<T, V> ou, ow;
+    const long long sh = which ? a.x[1].sh : a.x[0].sh;
+    const int heads = which ? a.x[1].heads : a.x[0].heads;
+    m.in = (const T*)(which ? a.x[1].in : a.x[0].in) + from[which][k] + head * sh;
+    m.out = (T*)(which ? a.x[1].out : a.x[0].out) + ((t0 + k) * heads + head) * a.D;
+    m.cs = turn + k * half;
+    if constexpr (HOW == kHalves) {
+      const bool pair = m.j < np;
+      const int c0 = pair ? m.j * V : a.rot + 2 * (m.j - np) * V, c1 = pair ? c0 + half : c0 + V;
+      m.has_w = c1 < a.D;
+      m.u = load_vec<T, V>(m.in + c0);
+      if (m.has_w) m.w = load_vec<T, V>(m.in + c1);
+    } else {
+      m.u = load_vec<T, V>(m.in + m.j * V);
+    }
+  };
+  auto finish = [&](Item& m) {
+    if constexpr (HOW == kHalves) {
+      const bool pair = m.j < np;
+      const int c0 = pair ? m.j * V : a.rot + 2 * (m.j - np) * V, c1 = pair ? c0 + half : c0 + V;
+      if (pair) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float2 q = cs[c0 + e];
-          const float p = (float)u.e[e], r = (float)w.e[e];
-          ou.e[e] = (T)(p * q.x - r * q.y);
-          ow.e[e] = (T)(r * q.x + p * q.y);
+          const float2 q = m.cs[c0 + e];
+          const float p = (float)m.u.e[e], r = (float)m.w.e[e];
+          m.u.e[e] = (T)(p * q.x - r * q.y);
+          m.w.e[e] = (T)(r * q.x + p * q.y);
         }
-        store_vec<T, V>(out + c0, ou);
-        store_vec<T, V>(out + c0 + half, ow);
-      } else {
-        const int c0 = a.rot + (j - np) * V;
-        store_vec<T, V>(out + c0, load_vec<T, V>(in + c0));
       }
-    } else {                                         // an item = V neighbouring channels
-      const int c0 = j * V;
-      const Vec<T, V> u = load_vec<T, V>(in + c0);
-      Vec<T, V> o = u;
-      if constexpr (HOW == kPairs) {
+      store_vec<T, V>(m.out + c0, m.u);
+      if (m.has_w) store_vec<T, V>(m.out + c1, m.w);
+    } else {
+      const int c0 = m.j * V;
+      Vec<T, V> o = m.u;
+      if constexpr (HOW == kPairs && V == 1) {
+        if (c0 < a.rot) {
+          const float2 q = m.cs[c0 >> 1];
+          const float p = (float)m.u.e[0], r = (float)m.in[c0 ^ 1];
+          o.e[0] = (T)((c0 & 1) ? p * q.x + r * q.y : p * q.x - r * q.y);
+        }
+      } else if constexpr (HOW == kPairs) {
 #pragma unroll
         for (int e = 0; e + 1 < V; e += 2)
           if (c0 + e < a.rot) {
-            const float2 q = cs[(c0 + e) >> 1];
-            const float p = (float)u.e[e], r = (float)u.e[e + 1];
+            const float2 q = m.cs[(c0 + e) >> 1];
+            const float p = (float)m.u.e[e], r = (float)m.u.e[e + 1];
             o.e[e] = (T)(p * q.x - r * q.y);
             o.e[e + 1] = (T)(r * q.x + p * q.y);
           }
-        if constexpr (V == 1) {
-          if (c0 < a.rot) {
-            const float2 q = cs[c0 >> 1];
-            const float p = (float)u.e[0], r = (float)in[c0 ^ 1];
-            o.e[0] = (T)((c0 & 1) ? p * q.x + r * q.y : p * q.x - r * q.y);
-          }
-        }
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const int c = c0 + e;
           if (c < a.rot) {
             const bool low = c < half;
-            const float2 q = cs[low ? c : c - half];
-            const float p = (float)u.e[e], r = (float)in[low ? c + half : c - half];
+            const float2 q = m.cs[low ? c : c - half];
+            const float p = (float)m.u.e[e], r = (float)m.in[low ? c + half : c - half];
             o.e[e] = (T)(low ? p * q.x - r * q.y : p * q.x + r * q.y);
           }
         }
       }
-      store_vec<T, V>(out + c0, o);
+      store_vec<T, V>(m.out + c0, o);
     }
+  };
+  for (int it = threadIdx.x; it < total; it += 512) {
+    Item m0, m1;
+    bring(m0, it);
+    const bool two = it + 256 < total;
+    if (two) bring(m1, it + 256);
+    finish(m0);
+    if (two) finish(m1);
   }
 }
 
@@ -141,30 +175,33 @@ static void launch_rotary(const RotaryArgs& a, bool vec, dim3 grid, size_t lds, 
 using namespace pgrf;
 using namespace pgrf::tok;
 
-extern "C" int pgrf_rotary(const void* q, long long q_sb, long long q_sn, long long q_sh, int q_heads, const void* k, long long k_sb, long long k_sn,
-                           long long k_sh, int k_heads, const void* positions, int position_type, long long pos_sb, int dtype, int B, int N, int D,
-                           int rotary_dim, int interleaved, double base, int scaling, double factor, double trained_length, double low, double high,
-                           float magnitude, int backward, void* q_out, void* k_out, void* stream) {
+extern "C" int pgrf_rotary(const PgrfRotary* p, void* stream) {
   const char* who = "pgrf_rotary";
+  if (!p) return set_error(PGRF_ERR_ARG, "%s: null arguments", who);
+  const int dtype = p->dtype, B = p->B, N = p->N, D = p->D, q_heads = p->q_heads, k_heads = p->k_heads, rotary_dim = p->rotary_dim, scaling = p->scaling;
+  const double base = p->base, factor = p->factor, trained_length = p->trained_length, low = p->low, high = p->high;
+  const void *q = p->q, *k = p->k;
+  void *q_out = p->q_out, *k_out = p->k_out;
+  const long long q_sb = p->q_sb, q_sn = p->q_sn, q_sh = p->q_sh, k_sb = p->k_sb, k_sn = p->k_sn, k_sh = p->k_sh;
   if (!dtype_ok(dtype)) return set_error(PGRF_ERR_UNSUPPORTED, "%s: dtype %d (PGRF_DTYPE_F32 | BF16 | F16)", who, dtype);
   if (B < 0 || N < 0 || q_heads < 1 || k_heads < 0 || D < 2) return set_error(PGRF_ERR_ARG, "%s: bad sizes B=%d N=%d heads=%d,%d D=%d", who, B, N, q_heads, k_heads, D);
   if (rotary_dim < 2 || (rotary_dim & 1) || rotary_dim > D || rotary_dim > PGRF_ROTARY_MAX_DIM)
     return set_error(PGRF_ERR_UNSUPPORTED, "%s: rotary_dim=%d (even, at most the head's %d channels and %d)", who, rotary_dim, D, PGRF_ROTARY_MAX_DIM);
   if ((long long)(q_heads + (long long)k_heads) * D > (1 << 20)) return set_error(PGRF_ERR_UNSUPPORTED, "%s: over 2^20 channels by token", who);
-  if (position_type < 0 || position_type > 3) return set_error(PGRF_ERR_ARG, "%s: position_type %d", who, position_type);
+  if (p->position_type < 0 || p->position_type > 3) return set_error(PGRF_ERR_ARG, "%s: position_type %d", who, p->position_type);
   if (!(base > 0) || !std::isfinite(base)) return set_error(PGRF_ERR_ARG, "%s: base must be positive", who);
   if (scaling < PGRF_ROTARY_PLAIN || scaling > PGRF_ROTARY_PARTS) return set_error(PGRF_ERR_ARG, "%s: scaling %d", who, scaling);
   if (scaling != PGRF_ROTARY_PLAIN && !(factor > 0 && std::isfinite(factor))) return set_error(PGRF_ERR_ARG, "%s: factor must be positive", who);
   if (scaling == PGRF_ROTARY_NTK && rotary_dim < 4) return set_error(PGRF_ERR_UNSUPPORTED, "%s: this scaling needs rotary_dim of 4 at least", who);
   if (scaling == PGRF_ROTARY_PARTS && !(trained_length > 0 && high > low)) return set_error(PGRF_ERR_ARG, "%s: scaling by parts needs trained_length > 0 and high > low", who);
   if ((long long)B * N == 0) return PGRF_OK;
-  if (!q || !q_out || !positions || (k_heads && (!k || !k_out))) return set_error(PGRF_ERR_ARG, "%s: null pointer", who);
+  if (!q || !q_out || !p->positions || (k_heads && (!k || !k_out))) return set_error(PGRF_ERR_ARG, "%s: null pointer", who);
   RotaryArgs a = {};
   a.x[0] = {q, q_out, q_sb, q_sn, q_sh, q_heads};
   a.x[1] = {k, k_out, k_sb, k_sn, k_sh, k_heads};
-  a.pos = positions; a.pos_b = pos_sb; a.pos_kind = position_type;
-  a.B = B; a.N = N; a.D = D; a.rot = rotary_dim; a.interleaved = interleaved ? 1 : 0;
-  a.sign = backward ? -1.f : 1.f; a.magnitude = magnitude;
+  a.pos = p->positions; a.pos_b = p->pos_sb; a.pos_kind = p->position_type;
+  a.B = B; a.N = N; a.D = D; a.rot = rotary_dim; a.interleaved = p->interleaved ? 1 : 0;
+  a.sign = p->backward ? -1.f : 1.f; a.magnitude = p->magnitude;
   const double pi2 = 6.283185307179586476925286766559, bs = scaling == PGRF_ROTARY_NTK ? base * std::pow(factor, rotary_dim / (rotary_dim - 2.0)) : base;
   const double step = -2.0 * std::log2(bs) / rotary_dim;
   for (int i = 0; i < rotary_dim / 2; ++i) {
@@ -181,8 +218,8 @@ extern "C" int pgrf_rotary(const void* q, long long q_sb, long long q_sn, long l
   bool vec = D % V == 0 && aligned16(q) && aligned16(q_out) && !((q_sb | q_sn | q_sh) % V);
   if (k_heads) vec = vec && aligned16(k) && aligned16(k_out) && !((k_sb | k_sn | k_sh) % V);
   const int step_v = vec ? V : 1;
-  const bool halves = !interleaved && vec && (rotary_dim / 2) % V == 0;
-  a.per_head = halves ? rotary_dim / 2 / V + (D - rotary_dim) / V : D / step_v;
+  const bool halves = !p->interleaved && vec && (rotary_dim / 2) % V == 0;
+  a.per_head = halves ? rotary_dim / 2 / V + ((D - rotary_dim) / V + 1) / 2 : D / step_v;
   a.items = (q_heads + k_heads) * a.per_head;
   a.inv_items = 1.f / a.items;
   a.inv_per_head = 1.f / a.per_head;
@@ -191,6 +228,7 @@ extern "C" int pgrf_rotary(const void* q, long long q_sb, long long q_sn, long l
   long long tile = 2048 / a.items;
   if (tile > tokens / 1024) tile = tokens / 1024;
   if (tile > 4096 / (rotary_dim / 2)) tile = 4096 / (rotary_dim / 2);
+  if (tile > kMaxTile) tile = kMaxTile;
   a.tile = tile < 1 ? 1 : (int)tile;
   const long long grid = (tokens + a.tile - 1) / a.tile;
   if (grid > 0x7fffffffll) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tokens", who);

@@ -2,32 +2,39 @@
 difference of their positions.  Positions may be whole (tokens) or continuous (the depths of a ray's samples)."""
 import torch
 
-from ._lib import lib
-from ._token import alike, dtype_code, on_device, on_gpu, require
+from ._token import DTYPES, ROTARY, alike, first_derivatives_only, launch, on_gpu, refuse, require
 
 _SCALINGS = {None: 0, 'linear': 1, 'ntk': 2, 'parts': 3}             # PGRF_ROTARY_* of include/panogrf_hip.h
 _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
 _MAX_DIM = 256
 
 
+def _heads(t):
+    """[B, N, ..., D] as [B, N, heads, D] with the channels side by side."""
+    d = t.dim()
+    if d != 4:
+        t = t.flatten(2, -2) if d > 4 else t.unsqueeze(2)
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
 def _launch(q, k, positions, call, backward):
-    """q, k [B,N,heads,D], any strides with the channels side by side."""
-    B, N, hq, D = q.shape
+    """-> tensors of the shapes of q and k, contiguous."""
     q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    B, N = q.shape[:2]
     if B and N:
         rot, interleaved, base, scaling, factor, trained, low, high, magnitude = call
-        qs, ks = q.stride(), (0, 0, 0) if k is None else k.stride()
-        with on_device(q.device) as stream:
-            lib.check(lib.pgrf_rotary(q.data_ptr(), qs[0], qs[1], qs[2], hq, None if k is None else k.data_ptr(), ks[0], ks[1], ks[2],
-                                      0 if k is None else k.shape[2], positions.data_ptr(), _POSITIONS[positions.dtype],
-                                      N if positions.dim() == 2 and B > 1 else 0, dtype_code(q, 'rotary'), B, N, D, rot, interleaved, base, scaling,
-                                      factor, trained, low, high, magnitude, backward, q_out.data_ptr(), None if k is None else k_out.data_ptr(), stream))
+        q4 = _heads(q)
+        qs, hq, D = q4.stride(), q4.shape[2], q4.shape[3]
+        if k is None:
+            kp, kop, ks, hk = 0, 0, (0, 0, 0), 0
+        else:
+            k4 = _heads(k)
+            kp, kop, ks, hk = k4.data_ptr(), k_out.data_ptr(), k4.stride(), k4.shape[2]
+        launch(q.device, 'pgrf_rotary', ROTARY.pack(q4.data_ptr(), kp, positions.data_ptr(), q_out.data_ptr(), kop, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
+                                                    N if positions.dim() == 2 and B > 1 else 0, base, factor, trained, low, high, DTYPES[q.dtype], B, N, D, hq, hk,
+                                                    rot, interleaved, _POSITIONS[positions.dtype], scaling, backward, magnitude))
     return q_out, k_out
-
-
-def _rows(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 class _Rotary(torch.autograd.Function):
@@ -39,16 +46,17 @@ class _Rotary(torch.autograd.Function):
         return _launch(q, k, positions, call, 0)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_derivatives_only
     def backward(ctx, dq, dk):
         positions, = ctx.saved_tensors
         needs = ctx.needs_input_grad
-        gs = [g if need else None for g, need in ((dq, needs[0]), (dk, needs[1]))]
-        first, second = (gs[0], gs[1]) if gs[0] is not None else (gs[1], None)
-        if first is None:
-            return None, None, None, None
-        a, b = _launch(_rows(first), None if second is None else _rows(second), positions, ctx.call, 1)
-        return (a, b, None, None) if gs[0] is not None else (None, a, None, None)
+        if not needs[0]:
+            dq = None
+        if not needs[1]:
+            dk = None
+        if dq is None:
+            return None, None if dk is None else _launch(dk, None, positions, ctx.call, 1)[0], None, None
+        return (*_launch(dq, dk, positions, ctx.call, 1), None, None)
 
 
 def rotary(q, k, positions, *, rotary_dim=None, layout='half', base=10000.0, scaling=None, factor=1.0, trained_length=4096, low=1.0, high=32.0,
@@ -64,27 +72,33 @@ def rotary(q, k, positions, *, rotary_dim=None, layout='half', base=10000.0, sca
                 context stay, those of under `low` are stretched
     and `magnitude` multiplies every turned pair.  float32, bfloat16 or float16; gradients to q and k."""
     who = 'rotary'
-    require(torch.is_tensor(q) and q.dim() >= 3, who, 'q must be [B, N, ..., D]')
-    dtype_code(q, who)
-    alike(who, q.dtype, q.device, k=k)
-    B, N, D = q.shape[0], q.shape[1], q.shape[-1]
-    require(k is None or (k.dim() >= 3 and k.shape[:2] == q.shape[:2] and k.shape[-1] == D), who, 'k must be [B, N, ..., D] with the axes of q')
+    require(isinstance(q, torch.Tensor) and q.dim() >= 3, who, 'q must be [B, N, ..., D]')
+    dtype, device, shape = q.dtype, q.device, q.shape
+    if dtype not in DTYPES:
+        refuse(who, f'dtype {dtype} (float32, bfloat16 or float16)')
+    B, N, D = shape[0], shape[1], shape[-1]
+    if k is not None:
+        if not isinstance(k, torch.Tensor) or k.dtype != dtype or k.device != device:
+            alike(who, 'k', k, dtype, device)
+        require(k.dim() >= 3 and k.shape[:2] == shape[:2] and k.shape[-1] == D, who, 'k must be [B, N, ..., D] with the axes of q')
+        require(k.numel() > 0 or B * N == 0, who, 'k has no heads')
     rot = D if rotary_dim is None else int(rotary_dim)
-    require(2 <= rot <= min(D, _MAX_DIM) and rot % 2 == 0, who, f'rotary_dim {rot} (even, at most {min(D, _MAX_DIM)})')
-    require(layout in ('half', 'interleaved'), who, f"layout {layout!r} ('half' or 'interleaved')")
-    require(scaling in _SCALINGS, who, f"scaling {scaling!r} (None, 'linear', 'ntk' or 'parts')")
-    require(torch.is_tensor(positions) and positions.device == q.device and positions.dtype in _POSITIONS, who,
+    if not 2 <= rot <= min(D, _MAX_DIM) or rot % 2:
+        refuse(who, f'rotary_dim {rot} (even, at most {min(D, _MAX_DIM)})')
+    if layout != 'half' and layout != 'interleaved':
+        refuse(who, f"layout {layout!r} ('half' or 'interleaved')")
+    if scaling not in _SCALINGS:
+        refuse(who, f"scaling {scaling!r} (None, 'linear', 'ntk' or 'parts')")
+    require(isinstance(positions, torch.Tensor) and positions.dtype in _POSITIONS and positions.device == device, who,
             'positions must be an int32, int64, float32 or float64 tensor on the device of q')
-    require(tuple(positions.shape) in ((N,), (B, N)), who, f'positions {tuple(positions.shape)} must be [{N}] or [{B}, {N}]')
+    if positions.shape != shape[1:2] and positions.shape != shape[:2]:
+        refuse(who, f'positions {tuple(positions.shape)} must be [{N}] or [{B}, {N}]')
     require(q.numel() > 0 or B * N == 0, who, 'q has no heads')
-    require(k is None or k.numel() > 0 or B * N == 0, who, 'k has no heads')
     on_gpu(q, who)
     call = (rot, int(layout == 'interleaved'), float(base), _SCALINGS[scaling], float(factor), float(trained_length), float(low), float(high),
             float(magnitude))
-    q4, k4 = (None if t is None else _rows(t.flatten(2, -2) if t.dim() > 3 else t.unsqueeze(2)) for t in (q, k))
-    positions = positions.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        q_out, k_out = _Rotary.apply(q4, k4, positions, call)
-    else:
-        q_out, k_out = _launch(q4, k4, positions, call, 0)
-    return q_out.view(q.shape), None if k is None else k_out.view(k.shape)
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
+        return _Rotary.apply(q, k, positions, call)
+    return _launch(q, k, positions, call, 0)

@@ -10,7 +10,20 @@ PTR = 1 << 20        # an address no kernel ever sees: every call below ends in 
 
 
 def norm_c(dtype=0, rows=4, channels=8, flags=6, rpg=4, x=PTR, y=PTR, gate=None, x_out=PTR, z=PTR, stats=None):
-    return lib.pgrf_block_norm(x, y, gate, rpg, None, None, None, None, dtype, rows, channels, flags, 1.0, 1e-6, x_out, z, stats, None)
+    from panogrf_amd._lib import PgrfBlockNorm
+    a = PgrfBlockNorm(x=x, y=y, gate=gate, x_out=x_out, z_out=z, stats=stats, rows=rows, rows_per_gate=rpg, dtype=dtype, C=channels, flags=flags, scale=1.0, eps=1e-6)
+    return lib.pgrf_block_norm(C.byref(a), None)
+
+
+def test_packed_structures_are_the_header_s():
+    from panogrf_amd import _lib, _token
+    for packed, fields in ((_token.BLOCK_NORM, _lib.PgrfBlockNorm), (_token.ROTARY, _lib.PgrfRotary), (_token.DIFF_ATTN, _lib.PgrfDiffAttn)):
+        assert packed.size == C.sizeof(fields)
+        marks = []
+        for i, (n, t) in enumerate(fields._fields_):
+            marks.append(t(i + 1).value)
+        got = fields.from_buffer_copy(packed.pack(*marks))
+        assert [getattr(got, n) for n, _ in fields._fields_] == marks
 
 
 @pytest.mark.parametrize('kw,code', [(dict(dtype=3), -3), (dict(dtype=-1), -3), (dict(channels=0), -3), (dict(channels=8193), -3), (dict(rows=-1), -1),
@@ -24,10 +37,18 @@ def test_block_norm_entries_without_rows():
     assert norm_c(rows=0) == 0
     n = lib.pgrf_block_norm_backward_workspace_bytes(100, 64, 10)
     assert n >= 64 * 5 * 4
-    args = lambda ws, size: (PTR, PTR, PTR, 10, None, None, None, PTR, PTR, PTR, 0, 100, 64, 6, 1.0, PTR, PTR, PTR, PTR, None, PTR, None, ws, size, None)
-    assert lib.pgrf_block_norm_backward(*args(None, 0)) == -1 and b'workspace' in lib.pgrf_last_error()
-    assert lib.pgrf_block_norm_backward(*args(PTR, 64)) == -1
-    assert lib.pgrf_block_norm_backward(PTR, PTR, None, 1, None, None, None, PTR, PTR, PTR, 0, 100, 64, 6, 1.0, PTR, PTR, PTR, None, None, None, None, None, 0, None) == -1
+    from panogrf_amd._lib import PgrfBlockNorm
+
+    def back(**kw):
+        a = PgrfBlockNorm(**{**dict(x=PTR, y=PTR, gate=PTR, stats=PTR, dx_out=PTR, dz=PTR, dx=PTR, dy=PTR, dgate=PTR, dpost_w=PTR, dpre_w=PTR, rows=100, rows_per_gate=10,
+                                    dtype=0, C=64, flags=6, scale=1.0), **kw})
+        return lib.pgrf_block_norm_backward(C.byref(a), None)
+    assert back() == -1 and b'workspace' in lib.pgrf_last_error()
+    assert back(workspace=PTR, workspace_bytes=64) == -1 and b'workspace' in lib.pgrf_last_error()
+    assert back(gate=None) == -1 and b'dgate' in lib.pgrf_last_error()
+    assert back(stats=None) == back(x=None) == back(rows_per_gate=7) == -1
+    assert back(rows=200000, rows_per_gate=2, workspace=PTR, workspace_bytes=1 << 40) == -3
+    assert lib.pgrf_block_norm(None, None) == lib.pgrf_block_norm_backward(None, None) == lib.pgrf_rotary(None, None) == -1
 
 
 @pytest.mark.parametrize('kw', [dict(y=torch.zeros(2, 3, 7)), dict(gate=torch.ones(8)), dict(y=torch.zeros(2, 3, 8), gate=torch.ones(3, 8)),
@@ -54,8 +75,11 @@ def test_block_norm_types():
 def test_rotary_entry(kw, code):
     a = dict(q=PTR, hq=1, k=PTR, hk=0, kind=0, dtype=0, D=16, rot=16, base=1e4, scaling=0, factor=1.0, low=1.0, high=32.0)
     a.update(kw)
-    rc = lib.pgrf_rotary(a['q'], 16, 16, 16, a['hq'], a['k'], 16, 16, 16, a['hk'], PTR, a['kind'], 0, a['dtype'], 2, 3, a['D'], a['rot'], 0, a['base'],
-                         a['scaling'], a['factor'], 4096.0, a['low'], a['high'], 1.0, 0, PTR, PTR, None)
+    from panogrf_amd._lib import PgrfRotary
+    r = PgrfRotary(q=a['q'], k=a['k'], positions=PTR, q_out=PTR, k_out=PTR, q_sb=16, q_sn=16, q_sh=16, k_sb=16, k_sn=16, k_sh=16, base=a['base'], factor=a['factor'],
+                   trained_length=4096.0, low=a['low'], high=a['high'], dtype=a['dtype'], B=2, N=3, D=a['D'], q_heads=a['hq'], k_heads=a['hk'], rotary_dim=a['rot'],
+                   position_type=a['kind'], scaling=a['scaling'], magnitude=1.0)
+    rc = lib.pgrf_rotary(C.byref(r), None)
     assert rc == code and b'pgrf_rotary' in lib.pgrf_last_error()
 
 
