@@ -246,7 +246,7 @@ __device__ __forceinline__ unsigned keys_of_lane(unsigned seen32, int last, int 
 // MPW: maps of a wave.  Up to D = 64 a wave keeps the sums of both maps of its 32 rows (128 registers), and every fragment of v serves two products.  At
 // D = 128 two waves share 32 rows, one map each, and meet at the end.
 #ifndef PGRF_DA_WEAVE
-#define PGRF_DA_WEAVE(T, D, NW) (sizeof(T) == 4)
+#define PGRF_DA_WEAVE(T, D, NW) (sizeof(T) == 4 && D > 32)
 #define PGRF_DA_MINW 2
 #endif
 template <typename T, int D, int NW> struct FwdShape {
@@ -255,7 +255,7 @@ template <typename T, int D, int NW> struct FwdShape {
   static constexpr int KT = 32;                                                // keys of a block
   static constexpr bool kWeave = PGRF_DA_WEAVE(T, D, NW);
   static constexpr int kTileKeys = kWeave || sizeof(T) == 4 || NW * MPW < 4 * 2 ? 32 : D == 32 ? 64 : 64;      // keys between barriers
-  static constexpr int kMinWaves = kWeave ? (NW + 3) / 4 : sizeof(T) == 2 && NW > 1 ? PGRF_DA_MINW : (NW + 3) / 4;
+  static constexpr int kMinWaves = kWeave ? (NW + 3) / 4 : NW > 1 ? PGRF_DA_MINW : 1;
 };
 
 // Scores of a block: S^T of MPW maps
@@ -297,11 +297,23 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
   const typename TL::Lane at(lane);
   const int group = MPW == 2 ? wave : wave >> 1, map0 = MPW == 2 ? 0 : wave & 1;
   const int rows = a.N * a.G, tiles = (rows + RW * 32 - 1) / (RW * 32);
+  // Neighbouring workgroups: the tiles of rows of one key head, so that they find its keys in their L2 (causal: the longest rows first); where there is one tile, the key
+  // heads of the same keys, which stand side by side in memory
   unsigned id = by_xcd(blockIdx.x, gridDim.x);
-  const int split = id % a.splits;
-  id /= a.splits;
-  const int tile = tiles - 1 - (int)(id % tiles);                              // (causal: the longest rows first)
-  const int bh = id / tiles, b = bh / a.Hk, hk = bh % a.Hk;
+  int split, tile, bh;
+  if (tiles == 1) {
+    const int heads = id % a.Hk;
+    id /= a.Hk;
+    split = id % a.splits;
+    bh = id / a.splits * a.Hk + heads;
+    tile = 0;
+  } else {
+    split = id % a.splits;
+    id /= a.splits;
+    tile = tiles - 1 - (int)(id % tiles);
+    bh = id / tiles;
+  }
+  const int b = bh / a.Hk, hk = bh % a.Hk;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.M) : a.M;
   const int r0 = (tile * RW + group) * 32, r = r0 + (lane & 31), rc = min(r, rows - 1);
   const int n = rc / a.G, head = hk * a.G + rc % a.G;
@@ -311,7 +323,8 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
   const int lim_lo = r0 + 31 >= rows ? -1 : a.causal ? min(r0 / a.G + off, len - 1) : len - 1;
   const int lim_hi = r0 >= rows ? -1 : a.causal ? min(min(r0 + 31, rows - 1) / a.G + off, len - 1) : len - 1;
   const int wg_hi = a.causal ? min(min((tile + 1) * RW * 32 - 1, rows - 1) / a.G + off, len - 1) : len - 1;
-  const int all = (wg_hi + KT * BT) / (KT * BT), per = (max(all, 0) + a.splits - 1) / a.splits;
+  // a share is the same number of tiles for every entry, so that long entries have more of them and not longer ones
+  const int all = (wg_hi + KT * BT) / (KT * BT), per = ((a.M + KT * BT - 1) / (KT * BT) + a.splits - 1) / a.splits;
   const int t0 = split * per, t1 = min(all, t0 + per);                         // tiles
 
   const T* q = (const T*)a.q + b * a.q_sb + n * a.q_sn + head * a.q_sh + map0 * a.q_sm + 8 * h;
@@ -519,6 +532,12 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
   const bool live = r < rows;
   if (a.splits > 1) {
     if (!live) return;
+    if (t0 >= t1) {                                                            // (an empty share: only its sums are read)
+      if (h == 0)
+#pragma unroll
+        for (int m = 0; m < MPW; ++m) *(float2*)(a.part_ml + (((long long)split * a.B * a.Hk + bh) * rows + r) * 4 + 2 * (map0 + m)) = make_float2(-INFINITY, 0.f);
+      return;
+    }
     const long long pat = ((long long)split * a.B * a.Hk + bh) * rows + r;
     float* po = a.part_o + pat * 4 * D + map0 * 2 * D + 4 * h;
 #pragma unroll
@@ -604,6 +623,7 @@ __global__ __launch_bounds__(256) void diff_attn_join(DiffArgs a) {
   for (int s = 0; s < a.splits; ++s) {
     const float4 e = *(const float4*)(a.part_ml + (s * all + row) * 4);
     const float* p = a.part_o + (s * all + row) * 4 * D + ch;
+    if (e.x == -INFINITY && e.z == -INFINITY && e.y == 0.f && e.w == 0.f) continue;
     const float w0 = e.x == -INFINITY ? 0.f : exp2f(e.x - m0), w1 = e.z == -INFINITY ? 0.f : exp2f(e.z - m1);
     l0 = fmaf(w0, e.y, l0);
     l1 = fmaf(w1, e.w, l1);
