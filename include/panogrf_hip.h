@@ -536,8 +536,9 @@ typedef struct PgrfDiffAttn {
   const unsigned char* key_mask; /* [B,M] by mask_sb, NULL: every key */
   const int* lengths;          /* [B] device, NULL: M (forward only) */
   void* out;                   /* [B,N,H,2D] contiguous */
-  float* lse;                  /* [B,H,2,N] and */
-  float* maps_out;             /* [B,N,H,2,2D]: what the backward pass needs, both NULL = not wanted */
+  float* lse;                  /* [B,H,2,N]: the maps' log sums, for the backward pass; NULL = not wanted */
+  float* maps_out;             /* [B,N,H,2,2D]: the maps' outputs; NULL = not wanted.  The backward pass does without them by one more sweep over
+                                * the keys, which is the quicker way up to 512 keys (float: 64): pgrf_diff_attention_keeps_maps() */
   void* workspace;             /* >= pgrf_diff_attention_workspace_bytes(), 16-byte aligned */
   size_t workspace_bytes;
   long long q_sb, q_sn, q_sh, q_sm, k_sb, k_sn, k_sh, k_sm, v_sb, v_sn, v_sh, mask_sb;   /* strides; *_sm: between the two maps */
@@ -547,9 +548,10 @@ typedef struct PgrfDiffAttn {
 size_t pgrf_diff_attention_workspace_bytes(int dtype, int B, int N, int M, int H, int Hk, int D);
 int pgrf_diff_attention(const PgrfDiffAttn* a, void* stream);
 /* Gradients for upstream dout [B,N,H,2D] (contiguous): dq [B,N,H,2,D], dk [B,M,Hk,2,D], dv [B,M,Hk,2D] contiguous and dlam [H] of lam's type; any may be
- * NULL (dk and dv only together).  `a` as in the forward call, with what it wrote to lse and maps_out (`out` is not read); workspace >=
+ * NULL (dk and dv only together).  `a` as in the forward call, with what it wrote to lse and, if at all, maps_out (`out` is not read); workspace >=
  * pgrf_diff_attention_backward_workspace_bytes().  No atomics: gradients do not depend on scheduling. */
-size_t pgrf_diff_attention_backward_workspace_bytes(int dtype, int B, int N, int M, int H, int Hk, int D);
+int pgrf_diff_attention_keeps_maps(int dtype, int M);
+size_t pgrf_diff_attention_backward_workspace_bytes(int dtype, int B, int N, int M, int H, int Hk, int D, int causal);
 int pgrf_diff_attention_backward(const PgrfDiffAttn* a, const void* dout, void* dq, void* dk, void* dv, void* dlam, void* stream);
 
 #ifdef __cplusplus

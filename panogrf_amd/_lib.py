@@ -182,7 +182,8 @@ SYMBOLS = {
     "pgrf_rotary": (C.c_int, [_P, _P]),
     "pgrf_diff_attention_workspace_bytes": (C.c_size_t, [C.c_int] * 7),
     "pgrf_diff_attention": (C.c_int, [_P, _P]),
-    "pgrf_diff_attention_backward_workspace_bytes": (C.c_size_t, [C.c_int] * 7),
+    "pgrf_diff_attention_keeps_maps": (C.c_int, [C.c_int] * 2),
+    "pgrf_diff_attention_backward_workspace_bytes": (C.c_size_t, [C.c_int] * 8),
     "pgrf_diff_attention_backward": (C.c_int, [_P, _P, _P, _P, _P, _P, _P]),
     "pgrf_render_rays_train": (C.c_int, [C.POINTER(PgrfFrame), _P, _P, C.POINTER(PgrfRenderCfg), _P, C.c_int, _P, _P,
                                          C.POINTER(PgrfPassOut), C.POINTER(PgrfPassOut), _P, _P, _P, C.c_size_t, _P]),

@@ -27,7 +27,7 @@ def _aligned(t):
 
 
 @lru_cache(maxsize=256)
-def _workspace_bytes(name, *sizes):
+def _of_sizes(name, *sizes):
     return entry(name)(*sizes)
 
 
@@ -47,8 +47,8 @@ def _forward(q, k, v, lam, mask, lengths, causal, scale, train):
         return torch.zeros(B, N, H, 2 * D, dtype=q.dtype, device=dev), None, None
     out = torch.empty(B, N, H, 2 * D, dtype=q.dtype, device=dev)
     lse = torch.empty(B, H, 2, N, dtype=torch.float32, device=dev) if train else None
-    maps = torch.empty(B, N, H, 2, 2 * D, dtype=torch.float32, device=dev) if train else None
-    n = _workspace_bytes('pgrf_diff_attention_workspace_bytes', DTYPES[q.dtype], B, N, M, H, k.shape[2], D)
+    maps = torch.empty(B, N, H, 2, 2 * D, dtype=torch.float32, device=dev) if train and _of_sizes('pgrf_diff_attention_keeps_maps', DTYPES[q.dtype], M) else None
+    n = _of_sizes('pgrf_diff_attention_workspace_bytes', DTYPES[q.dtype], B, N, M, H, k.shape[2], D)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     launch(dev, 'pgrf_diff_attention', _pack(q, k, v, lam, mask, lengths, causal, scale, out, lse, maps, ws, n))
     return out, lse, maps
@@ -76,7 +76,7 @@ class _DiffAttention(torch.autograd.Function):
             dout = dout.contiguous()
             if dout.data_ptr() % 16:
                 dout = dout.clone()
-            n = _workspace_bytes('pgrf_diff_attention_backward_workspace_bytes', DTYPES[q.dtype], B, N, k.shape[1], H, k.shape[2], D)
+            n = _of_sizes('pgrf_diff_attention_backward_workspace_bytes', DTYPES[q.dtype], B, N, k.shape[1], H, k.shape[2], D, ctx.call[0])
             ws = torch.empty(n, dtype=torch.uint8, device=q.device)
             launch(q.device, 'pgrf_diff_attention_backward', _pack(q, k, v, lam, mask, None, *ctx.call, None, lse, maps, ws, n), dout.data_ptr(), ptr(dq), ptr(dk),
                    ptr(dv), ptr(dlam))

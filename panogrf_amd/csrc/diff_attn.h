@@ -34,12 +34,21 @@ __device__ __forceinline__ f32x16 mma(Frag8<float>::type a, Frag8<float>::type b
 // reads take 64 bytes of 4 rows (16 bits), or 128 of 2 (float).  (b128 reads of 16 rows: 4.3 cycles; with 8 different places 8.4, with the plain layout 64.)
 __device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) const char*)(const char*)p; }
 
+__device__ __forceinline__ const void* same_in_all_lanes(const void* p) {
+  const unsigned long long v = (unsigned long long)p;
+  return (const void*)((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)v));
+}
+
 // 16 (or 4) bytes of every lane, from base + its offset, straight into LDS, one lane behind the other from the wave's address `to`.  As assembly, because the compiler lets a
 // transposed read wait for every such load in flight, though it goes to another tile.  Nothing but fetched() waits for these.
 __device__ __forceinline__ void fetch16(const void* base, unsigned off, unsigned to) {
+  base = same_in_all_lanes(base);
+  to = __builtin_amdgcn_readfirstlane(to);
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "m0", "memory");
 }
 __device__ __forceinline__ void fetch4(const void* base, unsigned off, unsigned to) {
+  base = same_in_all_lanes(base);
+  to = __builtin_amdgcn_readfirstlane(to);
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(off), "s"(base) : "m0", "memory");
 }
 // Everything that the workgroup's waves fetched so far is in LDS, and their reads so far are done
@@ -158,8 +167,11 @@ struct DiffArgs {
   // backward
   const void* dout;               // [B,N,H,2D] contiguous
   float* delta;                   // [B,H,2,N]: dout . o_i
-  float* dlam_part;               // [B*Hk][units][G]: shares of -dlam, by wave of the dq kernel (G a power of two up to 32) or by token
+  float* dlam_part;               // [B*Hk][units][G]: parts of -dlam, by wave of the dq kernel (G a power of two up to 32) or by token, of every share
   void *dq, *dk, *dv, *dlam;
+  // a workgroup's blocks cut into shares: partial gradients [shares][...] in float
+  int q_shares, kv_shares;
+  float *dq_part, *dk_part, *dv_part;
 };
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -564,8 +576,8 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int g = 0; g < 4; ++g) store4<float>(oo + 32 * c + 8 * g, o[m][c][4 * g], o[m][c][4 * g + 1], o[m][c][4 * g + 2], o[m][c][4 * g + 3]);
-      if (h == 0) a.lse[(((long long)b * a.H + head) * 2 + map0 + m) * a.N + n] = l[m] == 0.f ? INFINITY : mx[m] + log2f(l[m]);
     }
+    if (a.lse && live && h == 0) a.lse[(((long long)b * a.H + head) * 2 + map0 + m) * a.N + n] = l[m] == 0.f ? INFINITY : mx[m] + log2f(l[m]);
   }
   T* out = (T*)a.out + oat * 2 * D + 4 * h;
   if constexpr (MPW == 1) {
@@ -676,7 +688,9 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const typename TL::Lane at(lane);
   const int rows = a.N * a.G, tiles = (rows + NW * 32 - 1) / (NW * 32);
-  const unsigned id = by_xcd(blockIdx.x, gridDim.x);
+  unsigned id = by_xcd(blockIdx.x, gridDim.x);
+  const int share = id % a.q_shares;
+  id /= a.q_shares;
   const int tile = tiles - 1 - (int)(id % tiles);
   const int bh = id / tiles, b = bh / a.Hk, hk = bh % a.Hk;
   const int len = a.M;
@@ -686,7 +700,7 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
   const int lim = r >= rows ? -1 : a.causal ? min(n + off, len - 1) : len - 1;
   const int lim_lo = r0 + 31 >= rows ? -1 : a.causal ? min(r0 / a.G + off, len - 1) : len - 1;
   const int wg_hi = a.causal ? min(min((tile + 1) * NW * 32 - 1, rows - 1) / a.G + off, len - 1) : len - 1;
-  const int t1 = max((wg_hi + KT) / KT, 0);
+  const int all = max((wg_hi + KT) / KT, 0), per = (all + a.q_shares - 1) / a.q_shares, t0 = share * per, t1 = min(all, t0 + per);
   const long long oat = ((long long)b * a.N + n) * a.H + head;
 
   const T* q = (const T*)a.q + b * a.q_sb + n * a.q_sn + head * a.q_sh + 8 * h;
@@ -700,20 +714,18 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
   for (int s = 0; s < NV; ++s) gf[s] = load8<T>(go + 16 * s);
   float delta[2] = {0.f, 0.f}, lse[2];
   const long long st = ((long long)b * a.H + head) * 2 * a.N + n;
-  {
+#pragma unroll
+  for (int m = 0; m < 2; ++m) lse[m] = a.lse[st + m * a.N];
+  if (a.o12) {
     const float* oo = a.o12 + oat * 4 * D + 8 * h;
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int s = 0; s < NV; ++s) {
         const Frag8<float>::type e = load8<float>(oo + m * 2 * D + 16 * s);
 #pragma unroll
         for (int j = 0; j < 8; ++j) delta[m] = fmaf((float)gf[s][j], e[j], delta[m]);
       }
-      delta[m] += __shfl_xor(delta[m], 32, 64);
-      lse[m] = a.lse[st + m * a.N];
-      if (h == 0 && r < rows) a.delta[st + m * a.N] = delta[m];
-    }
   }
   const T* k = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
   const T* v = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
@@ -786,92 +798,119 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
       __syncthreads();
     }
   };
-  if (t1 > 0) {
-    fetch(0);
-    unsigned seen = seen_of(0);
-    if constexpr (kWeave)
-      for (int i = tid; i < kTile / 16; i += NW * 64) *(float4*)(ktile(-1) + i * 16) = make_float4(0.f, 0.f, 0.f, 0.f);   // (its score gradients are 0)
+  // Blocks first .. last - 1, one after the other
+  auto sweep = [&](int first, int last, auto work) {
+    if (first >= last) return;
+    fetch(first);
+    unsigned seen = seen_of(first);
     fetched();
-    if (t1 > 1) fetch(1);
-    clean(seen, 0);
-    if constexpr (kWeave) {
-      form(s, g, 0);
-      for (int t = 0; t < t1; ++t) {
-        const unsigned next = t + 1 < t1 ? seen_of(t + 1) : ~0u;
-        fetched();                                                       // block t + 1 has come; nobody reads k of t - 2 or v of t any more
-        if (t + 2 < t1) fetch(t + 2);
-        clean(next, t + 1);
-        hide(seen, t);
-        f32x16 s2[2] = {zero16(), zero16()}, g2 = zero16();
-        const char *kn = ktile(t + 1), *vn = vtile(t + 1), *kb = ktile(t - 1);   // (behind the last block: whatever stands there, unused)
-        F dn[2][2];
-        constexpr int NS = 2 * NK, NG = NS + NV, NP = NG + 4 * NC;
-        weave<F, NP, 3>(
-            [&](int i) {
-              return i < NS ? TL::row(kn, at, (i & 1) * NK + i / 2) : i < NG ? TL::row(vn, at, i - NS)
-                                                                                        : TL::col(kb, at, (i - NG) / (2 * NC), (i - NG) % (2 * NC));
-            },
-            [&](int i, const F& f) {
-              if (i < NS) s2[i & 1] = mma(f, qf[i & 1][i / 2], s2[i & 1]);
-              else if (i < NG) g2 = mma(f, gf[i - NS], g2);
-              else {
-                const int c = (i - NG) % (2 * NC);
-                dq[c / NC][c % NC] = mma(f, ds[c / NC][(i - NG) / (2 * NC)], dq[c / NC][c % NC]);
-              }
-            },
-            [&](int i) {
-#pragma unroll
-              for (int x = 16 * i / NP; x < 16 * (i + 1) / NP; ++x) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[0][x], a.c, -lse[0])), p1 = __builtin_amdgcn_exp2f(fmaf(s[1][x], a.c, -lse[1]));
-                dlam = fmaf(p1, g[x], dlam);
-                dn[0][x / 8][x % 8] = (T)(p0 * (g[x] - delta[0]));
-                dn[1][x / 8][x % 8] = (T)(p1 * (g[x] - delta[1]));
-              }
-            });
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          ds[m][0] = dn[m][0];
-          ds[m][1] = dn[m][1];
-          s[m] = s2[m];
-        }
-        asm volatile("" : "+v"(g2));                                           // (or its products are moved behind the others, to where they are used)
-        g = g2;
-        seen = next;
-      }
-      add(t1 - 1);
-    } else {
-      for (int t = 0; t < t1; ++t) {
-        form(s, g, t);
-        hide(seen, t);
-        turn();
-        add(t);
-        if (t + 1 < t1) {
-          seen = seen_of(t + 1);
-          fetched();
-          if (t + 2 < t1) fetch(t + 2);
-          clean(seen, t + 1);
-        }
+    if (first + 1 < last) fetch(first + 1);
+    clean(seen, first);
+    for (int t = first; t < last; ++t) {
+      form(s, g, t);
+      hide(seen, t);
+      work(t);
+      if (t + 1 < last) {
+        seen = seen_of(t + 1);
+        fetched();
+        if (t + 2 < last) fetch(t + 2);
+        clean(seen, t + 1);
       }
     }
+    __syncthreads();                                                           // (the tiles are read)
+  };
+  // delta = dout . o_i = sum of A_i G: without the maps' outputs, from one more sweep over the keys
+  if (!a.o12)
+    sweep(0, all, [&](int) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) delta[m] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[m][i], a.c, -lse[m])), g[i], delta[m]);
+    });
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    delta[m] += __shfl_xor(delta[m], 32, 64);
+    if (h == 0 && r < rows && share == 0) a.delta[st + m * a.N] = delta[m];
+  }
+  if constexpr (!kWeave) {
+    sweep(t0, t1, [&](int t) {
+      turn();
+      add(t);
+    });
+  } else if (t0 < t1) {
+    fetch(t0);
+    unsigned seen = seen_of(t0);
+    for (int i = tid; i < kTile / 16; i += NW * 64) *(float4*)(ktile(t0 - 1) + i * 16) = make_float4(0.f, 0.f, 0.f, 0.f);   // (its score gradients are 0)
+    fetched();
+    if (t0 + 1 < t1) fetch(t0 + 1);
+    clean(seen, t0);
+    form(s, g, t0);
+    for (int t = t0; t < t1; ++t) {
+      const unsigned next = t + 1 < t1 ? seen_of(t + 1) : ~0u;
+      fetched();                                                       // block t + 1 has come; nobody reads k of t - 2 or v of t any more
+      if (t + 2 < t1) fetch(t + 2);
+      clean(next, t + 1);
+      hide(seen, t);
+      f32x16 s2[2] = {zero16(), zero16()}, g2 = zero16();
+      const char *kn = ktile(t + 1), *vn = vtile(t + 1), *kb = ktile(t - 1);   // (behind the last block: whatever stands there, unused)
+      F dn[2][2];
+      constexpr int NS = 2 * NK, NG = NS + NV, NP = NG + 4 * NC;
+      weave<F, NP, 3>(
+          [&](int i) {
+            return i < NS ? TL::row(kn, at, (i & 1) * NK + i / 2) : i < NG ? TL::row(vn, at, i - NS)
+                                                                                      : TL::col(kb, at, (i - NG) / (2 * NC), (i - NG) % (2 * NC));
+          },
+          [&](int i, const F& f) {
+            if (i < NS) s2[i & 1] = mma(f, qf[i & 1][i / 2], s2[i & 1]);
+            else if (i < NG) g2 = mma(f, gf[i - NS], g2);
+            else {
+              const int c = (i - NG) % (2 * NC);
+              dq[c / NC][c % NC] = mma(f, ds[c / NC][(i - NG) / (2 * NC)], dq[c / NC][c % NC]);
+            }
+          },
+          [&](int i) {
+#pragma unroll
+            for (int x = 16 * i / NP; x < 16 * (i + 1) / NP; ++x) {
+              const float p0 = __builtin_amdgcn_exp2f(fmaf(s[0][x], a.c, -lse[0])), p1 = __builtin_amdgcn_exp2f(fmaf(s[1][x], a.c, -lse[1]));
+              dlam = fmaf(p1, g[x], dlam);
+              dn[0][x / 8][x % 8] = (T)(p0 * (g[x] - delta[0]));
+              dn[1][x / 8][x % 8] = (T)(p1 * (g[x] - delta[1]));
+            }
+          });
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        ds[m][0] = dn[m][0];
+        ds[m][1] = dn[m][1];
+        s[m] = s2[m];
+      }
+      asm volatile("" : "+v"(g2));                                           // (or its products are moved behind the others, to where they are used)
+      g = g2;
+      seen = next;
+    }
+    add(t1 - 1);
   }
   dlam += __shfl_xor(dlam, 32, 64);
   if (r >= rows) dlam = 0.f;
   if ((a.G & (a.G - 1)) == 0 && a.G <= 32) {                                   // one value for each head of the wave
     for (int o = 16; o >= a.G; o >>= 1) dlam += __shfl_xor(dlam, o, 64);
-    if (lane < a.G) a.dlam_part[((long long)bh * tiles * NW + tile * NW + wave) * a.G + lane] = dlam;
+    if (lane < a.G) a.dlam_part[(((long long)bh * tiles + tile) * a.q_shares + share) * NW * a.G + wave * a.G + lane] = dlam;
   } else if (r < rows && h == 0) {
-    a.dlam_part[(long long)bh * rows + r] = dlam;
+    a.dlam_part[((long long)bh * a.q_shares + share) * rows + r] = dlam;
   }
   if (r < rows && a.dq) {
     T* out = (T*)a.dq + oat * 2 * D + 4 * h;
+    float* part = a.dq_part + ((long long)share * a.B * a.N * a.H + oat) * 2 * D + 4 * h;
     const float f[2] = {a.scale, -lam_of<T>(a, head) * a.scale};
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          store4<T>(out + m * D + 32 * c + 8 * u, dq[m][c][4 * u] * f[m], dq[m][c][4 * u + 1] * f[m], dq[m][c][4 * u + 2] * f[m], dq[m][c][4 * u + 3] * f[m]);
+        for (int u = 0; u < 4; ++u) {
+          const float w[4] = {dq[m][c][4 * u] * f[m], dq[m][c][4 * u + 1] * f[m], dq[m][c][4 * u + 2] * f[m], dq[m][c][4 * u + 3] * f[m]};
+          if (a.q_shares > 1) store4<float>(part + m * D + 32 * c + 8 * u, w[0], w[1], w[2], w[3]);
+          else store4<T>(out + m * D + 32 * c + 8 * u, w[0], w[1], w[2], w[3]);
+        }
   }
 }
 
@@ -889,7 +928,9 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const typename TL::Lane at(lane);
   const int tiles = (a.M + NW * 32 - 1) / (NW * 32);
-  const unsigned id = by_xcd(blockIdx.x, gridDim.x);
+  unsigned id = by_xcd(blockIdx.x, gridDim.x);
+  const int share = id % a.kv_shares;
+  id /= a.kv_shares;
   const int tile = (int)(id % tiles), bh = id / tiles, b = bh / a.Hk, hk = bh % a.Hk;
   const int off = a.M - a.N;
   const int k0 = (tile * NW + wave) * 32, key = k0 + (lane & 31), kc = min(key, a.M - 1);
@@ -924,11 +965,14 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
   for (int c = 0; c < ND; ++c) dv[c] = zero16();
 
   // the blocks: queries that see the workgroup's first key, of each head that shares it
-  const int first = a.causal ? max(0, tile * NW * 32 - off) / QT : 0, nq = max((a.N + QT - 1) / QT - first, 0), total = nq * a.G;
+  const int first = a.causal ? max(0, tile * NW * 32 - off) / QT : 0, nq = max((a.N + QT - 1) / QT - first, 0);
+  const int all = nq * a.G, per = (all + a.kv_shares - 1) / a.kv_shares, from = min(share * per, all), total = min(all, from + per) - from;
   auto qtile = [&](int t) { return tiles_lds + (t & (R - 1)) * kTile; };
   auto gtile = [&](int t) { return tiles_lds + (R + (t & (R - 1))) * kTile; };
   const typename TL::template Loader<QT, NW> lq(a.q_sn, a.q_sm, tid), lg((long long)a.H * 2 * D, D, tid);
-  int to_head = hk * a.G, to_n = first * QT;                                   // what the next fetch brings
+  // (divisions run in vector registers; what the fetches' bases come from has to be known to be the same in every lane)
+  const int from_g = __builtin_amdgcn_readfirstlane(nq ? from / nq : 0), from_n = from - from_g * nq;
+  int to_head = hk * a.G + from_g, to_n = (first + from_n) * QT;               // what the next fetch brings
   auto fetch = [&](int t) {
     const int head = to_head, n0 = to_n;
     to_n += QT;
@@ -1020,7 +1064,7 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
       }
     fetched();
     if (total > 1) fetch(1);
-    int head = hk * a.G, n0 = first * QT;
+    int head = hk * a.G + from_g, n0 = (first + from_n) * QT;
     float lam = lam_of<T>(a, head);
     auto step = [&]() {
       n0 += QT;
@@ -1103,19 +1147,36 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
   if (key >= a.M) return;
   // (a key nobody sees has gradient 0; what its lanes hold came of values that may be anything, and stayed in their own columns)
   const long long oat = (((long long)b * a.M + key) * a.Hk + hk) * 2 * D + 4 * h;
-  auto put = [&](T* to, const f32x16& x, float f) {
+  const long long poat = oat + (long long)share * a.B * a.M * a.Hk * 2 * D;
+  auto put = [&](void* out, float* part, int at_, const f32x16& x, float f) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      store4<T>(to + 8 * u, seen ? x[4 * u] * f : 0.f, seen ? x[4 * u + 1] * f : 0.f, seen ? x[4 * u + 2] * f : 0.f, seen ? x[4 * u + 3] * f : 0.f);
+    for (int u = 0; u < 4; ++u) {
+      const float w[4] = {seen ? x[4 * u] * f : 0.f, seen ? x[4 * u + 1] * f : 0.f, seen ? x[4 * u + 2] * f : 0.f, seen ? x[4 * u + 3] * f : 0.f};
+      if (a.kv_shares > 1) store4<float>(part + poat + at_ + 8 * u, w[0], w[1], w[2], w[3]);
+      else store4<T>((T*)out + oat + at_ + 8 * u, w[0], w[1], w[2], w[3]);
+    }
   };
   if constexpr (DV)
 #pragma unroll
-    for (int c = 0; c < ND; ++c) put((T*)a.dv + oat + 32 * c, dv[c], 1.f);
+    for (int c = 0; c < ND; ++c) put(a.dv, a.dv_part, 32 * c, dv[c], 1.f);
   if constexpr (DK)
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int c = 0; c < NC; ++c) put((T*)a.dk + oat + m * D + 32 * c, dk[m][c], m ? -a.scale : a.scale);
+      for (int c = 0; c < NC; ++c) put(a.dk, a.dk_part, m * D + 32 * c, dk[m][c], m ? -a.scale : a.scale);
+}
+
+// Adds the shares of a gradient, in order; n a multiple of 4
+template <typename T>
+__global__ __launch_bounds__(256) void diff_attn_add(const float* part, T* out, long long n, int shares) {
+  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * 1024) {
+    float4 v = *(const float4*)(part + i);
+    for (int s = 1; s < shares; ++s) {
+      const float4 w = *(const float4*)(part + s * n + i);
+      v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+    }
+    store4<T>(out + i, v.x, v.y, v.z, v.w);
+  }
 }
 
 // dlam[h] = - the sum of what the waves (or rows) left for it, in a fixed order

@@ -35,6 +35,33 @@ static FwdCut cut_fwd(int dtype, int B, int Hk, long long rows, int M, int D) {
   return f;
 }
 
+// The backward kernels' waves, workgroups and shares.  The chip holds 512 workgroups of four waves at a time (256 where their registers or tiles leave room for one per
+// CU).  Where there are fewer, or where the causal mask makes some twice as long as the mean and they cannot be dealt out, a workgroup's blocks are cut into shares of at
+// least 8 whose gradients are added in float behind.
+struct BwdCut { int row_waves, key_waves, q_shares, kv_shares, units; long long row_groups, key_groups; };
+static int shares_for(long long groups, long long blocks, bool causal, int places) {
+  const long long want = causal ? 2 * places : places;
+  if (groups * 4 > want * 3) return 1;
+  long long s = (want + groups - 1) / groups;
+  if (s > blocks / 8) s = blocks / 8;
+  return (int)(s > 16 ? 16 : s < 1 ? 1 : s);
+}
+static BwdCut cut_bwd(int dtype, int B, int N, int M, int H, int Hk, int D, bool causal) {
+  BwdCut c;
+  const int G = H / Hk, places = dtype == PGRF_DTYPE_F32 || D == 128 ? 256 : 512;
+  const long long rows = (long long)N * G;
+  c.row_waves = waves_for(rows);
+  c.key_waves = waves_for(M);
+  c.row_groups = (long long)B * Hk * ((rows + c.row_waves * 32 - 1) / (c.row_waves * 32));
+  c.key_groups = (long long)B * Hk * (((long long)M + c.key_waves * 32 - 1) / (c.key_waves * 32));
+  // (short key axes form delta in a sweep of their own, which every share would repeat)
+  c.q_shares = M < 1024 ? 1 : shares_for(c.row_groups, (M + 31) / 32, causal, places);
+  c.kv_shares = shares_for(c.key_groups, (long long)G * ((N + 31) / 32), causal, places);
+  // (a wave's parts of dlam: G for 32 rows, rounded up to whole workgroups of at most four waves; fewer than N + 4 of each head)
+  c.units = ((G & (G - 1)) == 0 && G <= 32 ? (int)((rows + c.row_waves * 32 - 1) / (c.row_waves * 32) * c.row_waves) : N) * c.q_shares;
+  return c;
+}
+
 static int check(const PgrfDiffAttn* p, const char* who, bool backward) {
   if (!p) return set_error(PGRF_ERR_ARG, "%s: null arguments", who);
   if (!dtype_ok(p->dtype)) return set_error(PGRF_ERR_UNSUPPORTED, "%s: dtype %d (PGRF_DTYPE_F32 | BF16 | F16)", who, p->dtype);
@@ -56,10 +83,10 @@ static int check(const PgrfDiffAttn* p, const char* who, bool backward) {
   if (p->q_sn > (1 << 22) || p->q_sm > (1 << 22) || p->k_sn > (1 << 22) || p->k_sm > (1 << 22) || p->v_sn > (1 << 22) || p->q_sn < 0 || p->q_sm < 0 || p->k_sn < 0 || p->k_sm < 0 ||
       p->v_sn < 0 || (long long)p->H * 2 * p->D > (1 << 22))
     return set_error(PGRF_ERR_UNSUPPORTED, "%s: a stride between tokens or maps is negative or over 2^22 values", who);
-  if (backward && (!p->lse || !p->maps_out)) return set_error(PGRF_ERR_ARG, "%s: null lse / maps_out", who);
+  if (backward && !p->lse) return set_error(PGRF_ERR_ARG, "%s: null lse", who);
   if (backward && p->lengths) return set_error(PGRF_ERR_UNSUPPORTED, "%s: lengths have no backward pass (use key_mask)", who);
   if (!backward && !p->out) return set_error(PGRF_ERR_ARG, "%s: null out", who);
-  if (!p->lse != !p->maps_out) return set_error(PGRF_ERR_ARG, "%s: lse and maps_out go together", who);
+  if (!p->lse && p->maps_out) return set_error(PGRF_ERR_ARG, "%s: maps_out without lse", who);
   if ((p->maps_out && !aligned16(p->maps_out)) || (p->out && !aligned16(p->out))) return set_error(PGRF_ERR_ARG, "%s: out / maps_out must be 16-byte aligned", who);
   return PGRF_OK;
 }
@@ -116,9 +143,16 @@ int pgrf_diff_attention(const PgrfDiffAttn* p, void* stream) {
   return set_error(PGRF_ERR_UNSUPPORTED, "%s: no kernel", who);
 }
 
-size_t pgrf_diff_attention_backward_workspace_bytes(int, int B, int N, int M, int H, int Hk, int D) {
-  if (B < 1 || N < 1 || M < 1 || H < 1 || Hk < 1 || D < 1) return 0;
-  return (size_t)B * H * ((size_t)N * 3 + 4) * sizeof(float);
+int pgrf_diff_attention_keeps_maps(int dtype, int M) { return M > (dtype == PGRF_DTYPE_F32 ? 64 : 512); }
+
+size_t pgrf_diff_attention_backward_workspace_bytes(int dtype, int B, int N, int M, int H, int Hk, int D, int causal) {
+  if (B < 1 || N < 1 || M < 1 || H < 1 || Hk < 1 || H % Hk || D < 1) return 0;
+  const BwdCut c = cut_bwd(dtype, B, N, M, H, Hk, D, causal != 0);
+  size_t n = (size_t)B * H * 2 * N + ((size_t)B * Hk * c.units * (H / Hk) + 3) / 4 * 4;
+  n = (n + 3) / 4 * 4;
+  if (c.q_shares > 1) n += (size_t)c.q_shares * B * N * H * 2 * D;
+  if (c.kv_shares > 1) n += (size_t)c.kv_shares * B * M * Hk * 4 * D;
+  return n * sizeof(float);
 }
 
 int pgrf_diff_attention_backward(const PgrfDiffAttn* p, const void* dout, void* dq, void* dk, void* dv, void* dlam, void* stream) {
@@ -128,21 +162,23 @@ int pgrf_diff_attention_backward(const PgrfDiffAttn* p, const void* dout, void* 
   if (!dk != !dv) return set_error(PGRF_ERR_ARG, "%s: dk and dv go together", who);
   if ((long long)p->B * p->N == 0) return set_error(PGRF_ERR_ARG, "%s: no rows: the gradients are 0", who);
   if (!dout || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return set_error(PGRF_ERR_ARG, "%s: dout null, or a tensor not 16-byte aligned", who);
-  const size_t need = pgrf_diff_attention_backward_workspace_bytes(p->dtype, p->B, p->N, p->M, p->H, p->Hk, p->D);
+  const size_t need = pgrf_diff_attention_backward_workspace_bytes(p->dtype, p->B, p->N, p->M, p->H, p->Hk, p->D, p->causal);
   if (!p->workspace || !aligned16(p->workspace) || p->workspace_bytes < need)
     return set_error(PGRF_ERR_ARG, "%s: workspace too small or not 16-byte aligned (%zu < %zu bytes)", who, p->workspace_bytes, need);
   DiffArgs a = args_of(p);
   a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv; a.dlam = dlam;
   a.delta = (float*)p->workspace;
-  a.dlam_part = a.delta + (size_t)a.B * a.H * 2 * a.N;
-  const long long rows = (long long)a.N * a.G;
-  const int rw = waves_for(rows), kw = waves_for(a.M);
-  // (a wave's shares of dlam: G for 32 rows, rounded up to whole workgroups of at most four waves; fewer than N + 4 of each head)
-  const int units = (a.G & (a.G - 1)) == 0 && a.G <= 32 ? (int)((rows + rw * 32 - 1) / (rw * 32) * rw) : a.N;
-  const long long rg = (long long)a.B * a.Hk * ((rows + rw * 32 - 1) / (rw * 32)), kg = (long long)a.B * a.Hk * (((long long)a.M + kw * 32 - 1) / (kw * 32));
+  const BwdCut c = cut_bwd(p->dtype, a.B, a.N, a.M, a.H, a.Hk, p->D, a.causal != 0);
+  a.q_shares = c.q_shares; a.kv_shares = c.kv_shares;
+  const size_t sums = (size_t)a.B * a.H * 2 * a.N;
+  a.dlam_part = a.delta + sums;
+  float* behind = a.delta + (sums + ((size_t)a.B * a.Hk * c.units * a.G + 3) / 4 * 4 + 3) / 4 * 4;
+  if (c.q_shares > 1) { a.dq_part = behind; behind += (size_t)c.q_shares * a.B * a.N * a.H * 2 * p->D; }
+  if (c.kv_shares > 1) { a.dk_part = behind; a.dv_part = behind + (size_t)c.kv_shares * a.B * a.M * a.Hk * 2 * p->D; }
+  const long long rg = c.row_groups * c.q_shares, kg = c.key_groups * c.kv_shares;
   if (rg > 0x7fffffffll || kg > 0x7fffffffll) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tiles", who);
 #define PGRF_DA_BWD(T, D_) \
-  if (p->dtype == T && p->D == D_) return launch_da_bwd_##T##_##D_(a, rw, (unsigned)rg, units, kw, (unsigned)kg, (hipStream_t)stream);
+  if (p->dtype == T && p->D == D_) return launch_da_bwd_##T##_##D_(a, c.row_waves, (unsigned)rg, c.units, c.key_waves, (unsigned)kg, (hipStream_t)stream);
   PGRF_DA_ALL(PGRF_DA_BWD)
   return set_error(PGRF_ERR_UNSUPPORTED, "%s: no kernel", who);
 }

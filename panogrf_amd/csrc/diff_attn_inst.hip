@@ -54,6 +54,13 @@ int PGRF_DA_NAME(launch_da_bwd)(const DiffArgs& a, int row_waves, unsigned row_g
   else if (row_waves == 2) hipLaunchKernelGGL((diff_attn_dq<DaT, PGRF_DA_D, 2>), dim3(row_grid), dim3(128), 0, s, a);
   else hipLaunchKernelGGL((diff_attn_dq<DaT, PGRF_DA_D, 4>), dim3(row_grid), dim3(256), 0, s, a);
   PGRF_TOK_LAUNCHED(who);
+  auto add = [&](const float* part, void* out, long long n, int shares) {
+    hipLaunchKernelGGL((diff_attn_add<DaT>), dim3((unsigned)(n / 1024 < 2048 ? n / 1024 + 1 : 2048)), dim3(256), 0, s, part, (DaT*)out, n, shares);
+  };
+  if (a.dq && a.q_shares > 1) {
+    add(a.dq_part, a.dq, (long long)a.B * a.N * a.H * 2 * PGRF_DA_D, a.q_shares);
+    PGRF_TOK_LAUNCHED(who);
+  }
   if (a.dlam) {
     hipLaunchKernelGGL((diff_attn_dlam<DaT>), dim3(a.H), dim3(1024), 0, s, a, units);
     PGRF_TOK_LAUNCHED(who);
@@ -63,6 +70,11 @@ int PGRF_DA_NAME(launch_da_bwd)(const DiffArgs& a, int row_waves, unsigned row_g
     else if (key_waves == 2) launch_dkv<2>(a, key_grid, s);
     else launch_dkv<4>(a, key_grid, s);
     PGRF_TOK_LAUNCHED(who);
+    if (a.kv_shares > 1) {
+      add(a.dk_part, a.dk, (long long)a.B * a.M * a.Hk * 2 * PGRF_DA_D, a.kv_shares);
+      add(a.dv_part, a.dv, (long long)a.B * a.M * a.Hk * 2 * PGRF_DA_D, a.kv_shares);
+      PGRF_TOK_LAUNCHED(who);
+    }
   }
   return PGRF_OK;
 }

@@ -106,7 +106,7 @@ def attn(**kw):
 
 BAD = [(dict(dtype=3), -3), (dict(D=48), -3), (dict(D=256), -3), (dict(M=0), -1), (dict(H=3), -1), (dict(Hk=0), -1), (dict(N=-1), -1), (dict(scale=0.0), -1),
        (dict(scale=-1.0), -1), (dict(scale=float('nan')), -1), (dict(q=None), -1), (dict(v=None), -1), (dict(lam=None), -1), (dict(q=PTR + 8), -1),
-       (dict(k_sn=63), -1), (dict(q_sm=4), -1), (dict(lse=PTR), -1), (dict(N=1 << 30), -3)]
+       (dict(k_sn=63), -1), (dict(q_sm=4), -1), (dict(maps_out=PTR), -1), (dict(N=1 << 30), -3)]
 
 
 @pytest.mark.parametrize('kw,code', BAD + [(dict(out=None), -1), (dict(N=1, M=100000, B=1), -1)])       # (the last: a cut key axis without a workspace)
@@ -114,7 +114,7 @@ def test_diff_attention_entry(kw, code):
     assert lib.pgrf_diff_attention(C.byref(attn(**kw)), None) == code and b'pgrf_diff_attention' in lib.pgrf_last_error()
 
 
-@pytest.mark.parametrize('kw,code', [b for b in BAD if 'lse' not in b[0]] + [(dict(lse=None, maps_out=None), -1), (dict(lengths=PTR), -3), (dict(B=0), -1)])
+@pytest.mark.parametrize('kw,code', [b for b in BAD if 'maps_out' not in b[0]] + [(dict(lse=None, maps_out=None), -1), (dict(lse=None), -1), (dict(lengths=PTR), -3), (dict(B=0), -1)])
 def test_diff_attention_backward_entry(kw, code):
     a = attn(**{**dict(lse=PTR, maps_out=PTR), **kw})
     assert lib.pgrf_diff_attention_backward(C.byref(a), PTR, PTR, PTR, PTR, PTR, None) == code
