@@ -29,9 +29,6 @@ __device__ __forceinline__ f32x16 mma(Frag8<float>::type a, Frag8<float>::type b
   return c;
 }
 
-// A tile of rows of 2 D values in LDS (at a multiple of 256 bytes), in chunks of 16 bytes; chunk c of row r lies at place c ^ turn(r).  turn swaps bits of the row
-// number so that the lanes that LDS serves at a time (256 bytes: 64 banks) meet every bank once, both where 16 rows hand out the same chunk and where the transposed
-// reads take 64 bytes of 4 rows (16 bits), or 128 of 2 (float).  (b128 reads of 16 rows: 4.3 cycles; with 8 different places 8.4, with the plain layout 64.)
 __device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) const char*)(const char*)p; }
 
 __device__ __forceinline__ const void* same_in_all_lanes(const void* p) {
@@ -57,6 +54,9 @@ __device__ __forceinline__ void fetched() {
   __syncthreads();
 }
 
+// A tile of rows of 2 D values in LDS (at a multiple of 256 bytes), in chunks of 16 bytes; chunk c of row r lies at place c ^ turn(r).  turn swaps bits of the row
+// number so that the lanes that LDS serves at a time (256 bytes: 64 banks) meet every bank once, both where 16 rows hand out the same chunk and where the transposed
+// reads take 64 bytes of 4 rows (16 bits), or 128 of 2 (float).  (b128 reads of 16 rows: 4.3 cycles; with 8 different places 8.4, with the plain layout 64.)
 template <typename T, int D>
 struct Tile {
   static constexpr int kRow = 2 * D * (int)sizeof(T), kChunks = kRow / 16, kPer = 16 / (int)sizeof(T);
@@ -257,17 +257,14 @@ __device__ __forceinline__ unsigned keys_of_lane(unsigned seen32, int last, int 
 // ---------------------------------------------------------------------------------------------------------------- forward
 // MPW: maps of a wave.  Up to D = 64 a wave keeps the sums of both maps of its 32 rows (128 registers), and every fragment of v serves two products.  At
 // D = 128 two waves share 32 rows, one map each, and meet at the end.
-#ifndef PGRF_DA_WEAVE
-#define PGRF_DA_WEAVE(T, D, NW) (sizeof(T) == 4 && D > 32)
-#define PGRF_DA_MINW 2
-#endif
 template <typename T, int D, int NW> struct FwdShape {
   static_assert(D < 128 || NW > 1, "a pair of waves at D = 128");
-  static constexpr int MPW = D == 128 ? 1 : 2;
+  static constexpr int MPW = D == 128 ? 1 : 2, RW = NW * MPW / 2;              // RW: groups of 32 rows in the workgroup
   static constexpr int KT = 32;                                                // keys of a block
-  static constexpr bool kWeave = PGRF_DA_WEAVE(T, D, NW);
-  static constexpr int kTileKeys = kWeave || sizeof(T) == 4 || NW * MPW < 4 * 2 ? 32 : D == 32 ? 64 : 64;      // keys between barriers
-  static constexpr int kMinWaves = kWeave ? (NW + 3) / 4 : NW > 1 ? PGRF_DA_MINW : 1;
+  // Float from D = 64 on: one wave on a SIMD (its operands take twice the registers) with three blocks in work.  All others: two waves on a SIMD.
+  static constexpr bool kWeave = sizeof(T) == 4 && D > 32;
+  static constexpr int kMinWaves = kWeave || NW == 1 ? 1 : 2;
+  static constexpr int kTileKeys = sizeof(T) == 2 && RW == 4 ? 64 : 32;        // keys between barriers: fewer barriers where LDS holds two such tiles
 };
 
 // Scores of a block: S^T of MPW maps
@@ -292,16 +289,17 @@ __device__ __forceinline__ float with_other_half(float t) {                    /
   return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
 }
 
-// One pass over the keys in blocks of 32, three blocks in work at a time: while block j goes through its exponentials, the matrix pipe forms the scores of
-// block j + 1 and adds block j - 1 times its values.  None of the three waits for another, and they stand in one stretch of code without a branch, so that a
-// wave by itself keeps both pipes busy (measured on this card: 24 products of 32x32x16, 96 FMAs and 32 exponentials take 471 ns side by side, 386 + 312 one
-// after the other); masks and a new maximum are dealt with in front of it.
+// One pass over the keys in blocks of 32 with the running maximum and sum of each row's softmax.  What bounds it: per block and wave at D = 64 the matrix pipe has 24
+// products of 32x32x16 (386 ns at its peak) and the vector pipe 96 FMAs and 32 exponentials with their sums and roundings (over 312 ns); side by side the two take 471 ns
+// at best, and here they are busy for 44% and 56% of the time.  With kWeave a wave has three blocks in work: while block j goes through its exponentials, the matrix pipe
+// forms the scores of block j + 1 and adds block j - 1 times its values, in one stretch of code without a branch; masks and a new maximum are dealt with in front of it.
+// P1 and P2 are each rounded to the tensors' type for their product with v: the difference of the two could be rounded once only where both rows' sums are known first.
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff_attn_fwd(DiffArgs a) {
   using TL = Tile<T, D>;
   using F = typename Frag8<T>::type;
   using Sh = FwdShape<T, D, NW>;
-  constexpr int KT = Sh::KT, MPW = Sh::MPW, NK = D / 16, NC = 2 * D / 32, RW = NW * MPW / 2;   // RW: groups of 32 rows in the workgroup
+  constexpr int KT = Sh::KT, MPW = Sh::MPW, NK = D / 16, NC = 2 * D / 32, RW = Sh::RW;
   constexpr int kTile = KT * TL::kRow;
   constexpr int BT = Sh::kTileKeys / KT;                                         // blocks between barriers
   __shared__ __attribute__((aligned(1024))) char tiles_lds[4 * BT * kTile];        // two tiles of k, two of v
@@ -309,9 +307,9 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
   const typename TL::Lane at(lane);
   const int group = MPW == 2 ? wave : wave >> 1, map0 = MPW == 2 ? 0 : wave & 1;
   const int rows = a.N * a.G, tiles = (rows + RW * 32 - 1) / (RW * 32);
-  // Neighbouring workgroups: the tiles of rows of one key head, so that they find its keys in their L2 (causal: the longest rows first); where there is one tile, the key
-  // heads of the same keys, which stand side by side in memory
-  unsigned id = by_xcd(blockIdx.x, gridDim.x);
+  // Workgroups side by side: the tiles of rows of one key head, on one XCD, so that they find its keys in its L2 (causal: the longest rows first).  Where there is one tile,
+  // the key heads of the same keys, which stand side by side in memory, and no XCD gets more of the longer entries than another
+  unsigned id = tiles == 1 ? blockIdx.x : by_xcd(blockIdx.x, gridDim.x);
   int split, tile, bh;
   if (tiles == 1) {
     const int heads = id % a.Hk;
@@ -419,7 +417,7 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
       fetched();
       if (t0 + 1 < t1) fetch_k(t0 + 1);
       scores<T, D, MPW>(s, ktile(t0), qf, map0, at);
-  #pragma unroll
+#pragma unroll
       for (int m = 0; m < MPW; ++m) top[m] = top_of(s[m]);
       for (int t = t0; t < t1; ++t) {
         const int k0 = t * KT;
@@ -439,7 +437,7 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
         const char *kn = ktile(t + 1), *vb = vtile(t - 1);                       // (behind the last block: scores of whatever stands there, unused)
         float base[MPW], sum[MPW];
         F pn[MPW][2];
-  #pragma unroll
+#pragma unroll
         for (int m = 0; m < MPW; ++m) {
           next[m] = zero16();
           base[m] = mx[m] == -INFINITY ? 0.f : mx[m];
@@ -455,12 +453,12 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
                 next[i % MPW] = mma(f, qf[i % MPW][i / MPW], next[i % MPW]);
               } else {
                 const int c = (i - NS) % NC;
-  #pragma unroll
+#pragma unroll
                 for (int m = 0; m < MPW; ++m) o[m][c] = mma(f, p[m][(i - NS) / NC], o[m][c]);
               }
             },
             [&](int i) {
-  #pragma unroll
+#pragma unroll
               for (int x = 16 * MPW * i / NP; x < 16 * MPW * (i + 1) / NP; ++x) {
                 const int m = x / 16, e = x % 16;
                 const float w = __builtin_amdgcn_exp2f(fmaf(s[m][e], a.c, -base[m]));
@@ -468,7 +466,7 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
                 pn[m][e / 8][e % 8] = (T)w;
               }
             });
-  #pragma unroll
+#pragma unroll
         for (int m = 0; m < MPW; ++m) {
           l[m] += sum[m];
           p[m][0] = pn[m][0];
@@ -663,11 +661,11 @@ __global__ __launch_bounds__(256) void diff_attn_join(DiffArgs a) {
 // dv = (A1 - lam A2)^T dout, dlam = -sum A2 G.  A and G are formed again from q, k, v, dout and the saved log sums, twice: once by rows (dq, delta,
 // dlam) and once by keys (dk, dv), 14 instead of 10 products of N M D, so that no two workgroups add to one value and gradients do not depend on scheduling.
 //
-// At D = 128 in 16 bits a wave's registers leave a SIMD one wave, and both kernels weave three blocks as the forward kernel does; else two waves or more share a SIMD and
-// run beside each other.  Float does neither, as its products take eight times as long and hide the rest by themselves.
-template <typename T, int D> struct BwdShape {
-  static constexpr bool kWeave = sizeof(T) == 2 && D == 128;
-  static constexpr int kMinWaves = sizeof(T) == 2 && D < 128 ? 2 : 1;
+// Two waves or more share a SIMD and run beside each other, but for dq and dk at D = 128 in 16 bits, whose registers leave a SIMD one wave: those weave three blocks as the
+// forward kernel does.  Float does neither, as its products take eight times as long and hide the rest by themselves.
+template <typename T, int D, bool MORE = true> struct BwdShape {               // MORE: dq or dk is formed
+  static constexpr bool kWeave = sizeof(T) == 2 && D == 128 && MORE;
+  static constexpr int kMinWaves = sizeof(T) == 2 && !kWeave ? 2 : 1;
   static constexpr bool kLdsV = sizeof(T) == 2 && D == 64;                     // dk, dv: the wave's own values stay in LDS, to keep two waves on a SIMD
 };
 
@@ -916,10 +914,10 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
 
 // DK, DV: which of the two this launch forms.  At D = 128 their sums and the keys' own values do not fit a wave's registers together, and the scores are formed twice.
 template <typename T, int D, int NW, bool DK, bool DV>
-__global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_attn_dkv(DiffArgs a) {
+__global__ __launch_bounds__(NW * 64, (BwdShape<T, D, DK>::kMinWaves)) void diff_attn_dkv(DiffArgs a) {
   using TL = Tile<T, D>;
   using F = typename Frag8<T>::type;
-  constexpr bool kWeave = BwdShape<T, D>::kWeave;
+  constexpr bool kWeave = BwdShape<T, D, DK>::kWeave;
   constexpr int QT = 32, NK = D / 16, NV = DK ? 2 * D / 16 : 1, NC = DK ? D / 32 : 1, ND = DV ? 2 * D / 32 : 1, R = kWeave ? 4 : 2;   // R: blocks in LDS
   constexpr int kTile = QT * TL::kRow;
   constexpr bool kLdsV = BwdShape<T, D>::kLdsV && DK;

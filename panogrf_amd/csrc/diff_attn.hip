@@ -11,9 +11,6 @@ namespace tok {
 #define PGRF_DA_ALL(X) X(0, 32) X(0, 64) X(0, 128) X(1, 32) X(1, 64) X(1, 128) X(2, 32) X(2, 64) X(2, 128)
 PGRF_DA_ALL(PGRF_DA_DECL)
 
-#ifndef PGRF_DA_SHARES
-#define PGRF_DA_SHARES 5120
-#endif
 static int waves_for(long long rows) { return rows > 64 ? 4 : rows > 32 ? 2 : 1; }
 
 // The forward kernel's waves and their rows: at D = 128 two waves share 32 rows (and float's values leave no room for eight)
@@ -24,11 +21,13 @@ static FwdCut cut_fwd(int dtype, int B, int Hk, long long rows, int M, int D) {
   if (D == 128) f.waves = f.waves == 4 && dtype == PGRF_DTYPE_F32 ? 4 : 2 * f.waves;
   f.rows = D == 128 ? f.waves * 16 : f.waves * 32;
   const long long groups = (long long)B * Hk * ((rows + f.rows - 1) / f.rows);
-  // The key axis is cut where the rows alone leave the chip idle.  The CU holds five workgroups of a single wave (two buffers of 32 KB) and two of more.  A cache's entries
-  // have lengths that only the device knows, so there its shares are small enough to be dealt out evenly, four to a place.  None is under 128 keys.
-  const long long want = rows <= 32 ? PGRF_DA_SHARES : 512, most = M / 128;
-  long long s = (want + groups - 1) / groups;
-  if (groups * 2 > (rows <= 32 ? 1280 : want) && !(rows <= 32 && groups < want)) s = 1;
+  // The key axis is cut where the rows alone leave the chip idle.  Up to 32 rows (single tokens): 1280 workgroups of one wave fit the chip (two buffers of 32 KB each), and
+  // as many shares are dealt out; more of them cost more in partial sums than they even out (32 caches of 4096 to 16384 keys, 8 key heads, bf16, D = 64: 245 us; with
+  // 2560 shares 257, with 5120 285, with 1024 263).  More rows: 512 workgroups fit, and from half of that on the join costs more than the idle half (2048 x 8192, 16
+  // heads: 245 us whole, 271 cut).  None is under 128 keys.
+  const bool few = rows <= 32;
+  const long long want = few ? 1280 : 512, most = M / 128;
+  long long s = !few && groups > want / 2 ? 1 : (want + groups - 1) / groups;
   if (s > most) s = most;
   if (s > 128) s = 128;
   f.splits = s < 1 ? 1 : (int)s;
