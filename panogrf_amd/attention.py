@@ -116,7 +116,8 @@ def diff_attention(q, k, v, lam, *, causal=False, key_mask=None, scale=None):
 
     float32, bfloat16 or float16 (lam of that type or float32); d 32, 64 or 128; H a multiple of Hk: the query heads h Hk/H share a key head.  Any strides (rows
     that do not start at multiples of 16 bytes are copied first).  key_mask [B, M] bool, False: no query sees the key, and what it holds does not matter.
-    causal: query i sees keys up to i + M - N, so the last query stands at the last key.  A query that sees no key gives 0.  scale: 1/sqrt(d) unless given.
+    causal: query i sees keys up to i + M - N, so the last query stands at the last key.  A query that sees no key gives 0 and
+    has no part in any gradient, whatever it and its gradient hold.  scale: 1/sqrt(d) unless given.
     Softmax and sums are float; probabilities and score gradients are rounded to the tensors' type for the products behind them.  Gradients (first derivatives) to
     q, k, v and lam; they do not depend on scheduling."""
     who = 'diff_attention'

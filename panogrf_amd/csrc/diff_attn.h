@@ -133,11 +133,11 @@ struct Tile {
       const int e = (chunk ^ turn(i * kRowsPer)) * kPer;                       // (row0 < kRowsPer, a power of two: the bits of the two stay apart)
       return e >= D ? e - D + sm : e;
     }
-    // base: the tile's first row; rows from `rows` on repeat the last one (they are masked)
-    __device__ __forceinline__ void operator()(char* t, const T* base, int rows, int tid, int wave) const {
+    // base: the tile's first row; rows from `rows` on repeat the last one, rows below `from` that one (they are masked)
+    __device__ __forceinline__ void operator()(char* t, const T* base, int rows, int tid, int wave, int from = -0x7fffffff - 1) const {
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        const int r = row0 + i * kRowsPer, g = min(r, rows - 1);
+        const int r = row0 + i * kRowsPer, g = max(min(r, rows - 1), from);
         fetch16(base, (g * sn + val(i)) * (int)sizeof(T), lds(t) + (i * NW + wave) * 1024);
       }
     }
@@ -714,6 +714,11 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
   const long long st = ((long long)b * a.H + head) * 2 * a.N + n;
 #pragma unroll
   for (int m = 0; m < 2; ++m) lse[m] = a.lse[st + m * a.N];
+  if (lse[0] == INFINITY)                                                      // a row that sees nothing is 0 whatever its gradient holds (in f16, often an overflow)
+#pragma unroll
+    for (int s = 0; s < NV; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) gf[s][j] = (T)0.f;
   if (a.o12) {
     const float* oo = a.o12 + oat * 4 * D + 8 * h;
 #pragma unroll
@@ -962,8 +967,26 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D, DK>::kMinWaves)) void diff
 #pragma unroll
   for (int c = 0; c < ND; ++c) dv[c] = zero16();
 
+  // Queries that see nothing stand in front of all others (they have no key at or before their place, or none at all), and have no part in any gradient, whatever they and
+  // their own gradient hold (in f16, often an overflow): blocks of them are left out, and in the block where they end the first other row takes their places
+  int blind = a.causal ? max(0, -off) : 0;
+  if (a.mask) {
+    const unsigned char* mask = a.mask + b * a.mask_sb;
+    int key0 = 0;
+    unsigned long long any = 0;
+    for (; key0 < a.M; key0 += 256) {
+      unsigned long long at4[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) at4[i] = keys_seen<64>(mask, key0 + 64 * i, a.M, lane);
+#pragma unroll
+      for (int i = 3; i >= 0; --i)
+        if (at4[i]) { any = at4[i]; blind = key0 + 64 * i + __builtin_ctzll(at4[i]); }   // (the first key anyone sees)
+      if (any) break;
+    }
+    blind = !any ? a.N : a.causal ? max(0, blind - off) : 0;
+  }
   // the blocks: queries that see the workgroup's first key, of each head that shares it
-  const int first = a.causal ? max(0, tile * NW * 32 - off) / QT : 0, nq = max((a.N + QT - 1) / QT - first, 0);
+  const int first = max(blind, a.causal ? tile * NW * 32 - off : 0) / QT, nq = max((a.N + QT - 1) / QT - first, 0);
   const int all = nq * a.G, per = (all + a.kv_shares - 1) / a.kv_shares, from = min(share * per, all), total = min(all, from + per) - from;
   auto qtile = [&](int t) { return tiles_lds + (t & (R - 1)) * kTile; };
   auto gtile = [&](int t) { return tiles_lds + (R + (t & (R - 1))) * kTile; };
@@ -975,8 +998,8 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D, DK>::kMinWaves)) void diff
     const int head = to_head, n0 = to_n;
     to_n += QT;
     if (to_n >= a.N) { to_n = first * QT; ++to_head; }
-    lq(qtile(t), (const T*)a.q + b * a.q_sb + head * a.q_sh + n0 * a.q_sn, a.N - n0, tid, wave);
-    lg(gtile(t), (const T*)a.dout + (((long long)b * a.N + n0) * a.H + head) * 2 * D, a.N - n0, tid, wave);
+    lq(qtile(t), (const T*)a.q + b * a.q_sb + head * a.q_sh + n0 * a.q_sn, a.N - n0, tid, wave, blind - n0);
+    lg(gtile(t), (const T*)a.dout + (((long long)b * a.N + n0) * a.H + head) * 2 * D, a.N - n0, tid, wave, blind - n0);
     const long long st = ((long long)b * a.H + head) * 2 * a.N + n0;
     const unsigned off = ((unsigned)h * a.N + min(lane & 31, a.N - 1 - n0)) * 4u;
     for (int w = wave; w < 2; w += NW)                                         // lse of both maps, then delta of both: 32 values each

@@ -89,6 +89,23 @@ def test_what_masked_places_hold_does_not_matter(dtype):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('D', [32, 64, 128])
+@pytest.mark.parametrize('M', [70, 600])
+def test_what_queries_that_see_nothing_hold_does_not_matter(M, D, dtype):
+    """They give 0 and move nothing, also where a 16-bit gradient overflowed on its way to them."""
+    for causal, N in ((False, 40), (True, M + 37)):
+        q, k, v, lam, do = make(2, N, M, 4, 2, D, dtype)
+        mask = mask_of('none' if causal else 'holes', 2, M)
+        blind = (torch.arange(N, device='cuda') < N - M) if causal else slice(None)
+        want = grads(q, k, v, lam, do, causal=causal, key_mask=mask)
+        q, do = q.clone(), do.clone()
+        for b in (0, 1) if causal else (0,):                                       # (the holes leave entry 0 nothing)
+            q[b, blind], do[b, blind] = float('nan'), float('inf')
+        got = grads(q, k, v, lam, do, causal=causal, key_mask=mask)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_large_scores():
     q, k, v, lam, do = make(1, 50, 200, 2, 2, 64, 'f32')
     check(q * 20, k * 4, v, lam, do, False, None)                   # maps that are nearly one key
