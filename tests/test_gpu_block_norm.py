@@ -81,6 +81,13 @@ def test_parts_left_out(post, pre, use, dtype):
     check(make((3, 21, 136), dtype, 'rms', 'full', 5, weights=False), 'rms', 'full', 0.5, dtype, post, pre, use)
 
 
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('kind', ['rms', 'layer'])
+@pytest.mark.parametrize('C', [1, 3, 17, 24, 100, 136, 520, 1001, 4104])
+def test_without_weights_and_gate(C, kind, dtype):
+    check(make((2, 5, C), dtype, kind, 'none', 14, weights=False), kind, 'none', 0.7, dtype)
+
+
 @pytest.mark.parametrize('kind', ['rms', 'layer'])
 def test_norm_alone(kind):
     t = make((4, 6, 5, 64), 'bf16', kind, 'none', 6)
