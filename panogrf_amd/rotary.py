@@ -70,7 +70,7 @@ def rotary(q, k, positions, *, rotary_dim=None, layout='half', base=10000.0, sca
       'ntk'     with base * factor^(rotary_dim/(rotary_dim-2))
       'parts'   f_i (t + (1-t)/factor), t = clamp((trained_length f_i/2pi - low)/(high - low), 0, 1): pairs of over `high` turns in the trained
                 context stay, those of under `low` are stretched
-    and `magnitude` multiplies every turned pair.  float32, bfloat16 or float16; gradients to q and k."""
+    and `magnitude` multiplies every turned pair.  float32, bfloat16 or float16; gradients to q and k (positions have none)."""
     who = 'rotary'
     require(isinstance(q, torch.Tensor) and q.dim() >= 3, who, 'q must be [B, N, ..., D]')
     dtype, device, shape = q.dtype, q.device, q.shape
@@ -94,6 +94,8 @@ def rotary(q, k, positions, *, rotary_dim=None, layout='half', base=10000.0, sca
     if positions.shape != shape[1:2] and positions.shape != shape[:2]:
         refuse(who, f'positions {tuple(positions.shape)} must be [{N}] or [{B}, {N}]')
     require(q.numel() > 0 or B * N == 0, who, 'q has no heads')
+    if positions.requires_grad and torch.is_grad_enabled():
+        refuse(who, 'positions have no gradient: detach them')
     on_gpu(q, who)
     call = (rot, int(layout == 'interleaved'), float(base), _SCALINGS[scaling], float(factor), float(trained_length), float(low), float(high),
             float(magnitude))

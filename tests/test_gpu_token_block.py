@@ -216,6 +216,17 @@ def test_a_block_served_token_by_token(dtype):
             close((name, b), torch.stack([got[i][j][b, 0] for i in range(steps)]), exact[b][j][0, n:], [m[b][j][0, n:] for m in moved])
 
 
+def test_second_derivatives_are_refused():
+    from panogrf_amd import attention, block_norm, rotary
+    x = torch.randn(1, 4, 2, 2, 32, device='cuda', requires_grad=True)
+    v, lam = torch.randn(1, 4, 2, 64, device='cuda'), torch.rand(2, device='cuda')
+    for out in (attention.diff_attention(x, x, v, lam), block_norm.block_norm(x)[1], rotary.rotary(x, None, torch.arange(4, device='cuda'))[0]):
+        g, = torch.autograd.grad(out.square().sum(), x, create_graph=True)         # (the gradient itself is given)
+        assert torch.isfinite(g).all()
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.square().sum(), x)
+
+
 class TokenMono(nn.Module):
     """A small mono-depth net over the panorama's patches, behind the renderer's call d_net(erp, cube, dnet=True) -> {'pred_depth', 'mono_feat'}."""
 

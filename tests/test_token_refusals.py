@@ -94,6 +94,12 @@ def test_rotary(kw):
         rotary(torch.zeros(2, 3, 4, 16), kw.pop('k'), kw.pop('positions'), **kw)
 
 
+def test_rotary_positions_have_no_gradient():
+    from panogrf_amd.rotary import rotary
+    with pytest.raises(PgrfError, match='detach'):
+        rotary(torch.zeros(2, 3, 4, 16), None, torch.zeros(3, requires_grad=True))
+
+
 def attn(**kw):
     from panogrf_amd._lib import PgrfDiffAttn
     a = PgrfDiffAttn(q=PTR, k=PTR, v=PTR, lam=PTR, out=PTR, dtype=1, B=2, N=3, M=4, H=4, Hk=2, D=64, scale=0.1)
