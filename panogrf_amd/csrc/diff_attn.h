@@ -986,7 +986,7 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D, DK>::kMinWaves)) void diff
     blind = !any ? a.N : a.causal ? max(0, blind - off) : 0;
   }
   // the blocks: queries that see the workgroup's first key, of each head that shares it
-  const int first = max(blind, a.causal ? tile * NW * 32 - off : 0) / QT, nq = max((a.N + QT - 1) / QT - first, 0);
+  const int first = max(blind, a.causal ? tile * NW * 32 - off : 0) / QT, nq = blind < a.N ? max((a.N + QT - 1) / QT - first, 0) : 0;
   const int all = nq * a.G, per = (all + a.kv_shares - 1) / a.kv_shares, from = min(share * per, all), total = min(all, from + per) - from;
   auto qtile = [&](int t) { return tiles_lds + (t & (R - 1)) * kTile; };
   auto gtile = [&](int t) { return tiles_lds + (R + (t & (R - 1))) * kTile; };

@@ -106,6 +106,19 @@ def test_what_queries_that_see_nothing_hold_does_not_matter(M, D, dtype):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize('M', [40, 600])
+def test_an_entry_without_keys_reads_nothing_behind_its_rows(M):
+    """The last entry's mask leaves nothing: what stands behind its last query (here the next piece of one tensor, not finite) is not read."""
+    q, k, v, lam, do = make(2, 41, M, 2, 2, 64, 'bf16')
+    room = torch.full((3, 41, 2, 2, 64), float('nan'), device='cuda', dtype=torch.bfloat16)
+    room[:2] = q
+    mask = torch.ones(2, M, dtype=torch.bool, device='cuda')
+    mask[1] = False
+    want, got = grads(q, k, v, lam, do, key_mask=mask), grads(room[:2], k, v, lam, do, key_mask=mask)
+    assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(got, want))
+    assert all(float(t[1].abs().sum()) == 0 for t in got[:4])
+
+
 def test_large_scores():
     q, k, v, lam, do = make(1, 50, 200, 2, 2, 64, 'f32')
     check(q * 20, k * 4, v, lam, do, False, None)                   # maps that are nearly one key
