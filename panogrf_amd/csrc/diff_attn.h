@@ -1187,6 +1187,226 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D, DK>::kMinWaves)) void diff
       for (int c = 0; c < NC; ++c) put(a.dk, a.dk_part, m * D + 32 * c, dk[m][c], m ? -a.scale : a.scale);
 }
 
+// Sums over the 32 lanes of a half: lane l gets that of value l & 15 of a (l & 16: of b).  In every step a lane keeps one half of the values it has and gives the other
+// to its partner, 77 operations where 32 sums of their own are 192.
+__device__ __forceinline__ float sums_of_half(const f32x16& a, const f32x16& b, int lane) {
+  float w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(a[i]), __float_as_uint(b[i]), false, false);
+    w[i] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  }
+  auto step = [&](int n, auto ctrl) {                                          // partners differ in the bit of lane that is n (and perhaps in lower ones)
+    const bool upper = lane & n;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float keep = upper ? w[i + n] : w[i], give = upper ? w[i] : w[i + n];
+      w[i] = keep + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(give), decltype(ctrl)::value, 0xf, 0xf, true));
+    }
+  };
+  step(8, std::integral_constant<int, 0x128>{});                               // lane ^ 8
+  step(4, std::integral_constant<int, 0x141>{});                               // lane ^ 7
+  step(2, std::integral_constant<int, 0x4E>{});                                // lane ^ 2
+  step(1, std::integral_constant<int, 0xB1>{});                                // lane ^ 1
+  return w[0];
+}
+
+// All gradients of a key head with up to 64 keys in one go: a workgroup holds the keys, a wave 32 of them, and the queries of the head pass by once, so that scores, maps and
+// the products with v are formed once (10 products of N M D where the two kernels above have 14, or 20 with delta's sweep) and every input is read once.  delta is the sum of
+// a row's A G over the lanes and waves that hold its keys; score gradients go through LDS, turned round, to the sum over keys that is dq.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW * 64, 1) void diff_attn_short(DiffArgs a) {
+  using TL = Tile<T, D>;
+  using F = typename Frag8<T>::type;
+  constexpr int QT = 32, NK = D / 16, NV = 2 * D / 16, NC = D / 32, ND = 2 * D / 32, R = 2;
+  constexpr int kTile = QT * TL::kRow, kPitch = NW * 32 + 8;                   // (the pitch keeps the writes of neighbouring rows in other banks)
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  __shared__ __attribute__((aligned(1024))) char tiles_lds[(2 * R + NW) * kTile];
+  __shared__ __attribute__((aligned(16))) T turned[2][QT][kPitch];             // score gradients: [map][query][key]
+  __shared__ __attribute__((aligned(16))) float stat[R][2][QT], sums[NW][2][QT];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const typename TL::Lane at(lane);
+  const int bh = (int)by_xcd(blockIdx.x, gridDim.x), b = bh / a.Hk, hk = bh % a.Hk, off = a.M - a.N;
+  const int k0 = wave * 32, key = k0 + (lane & 31), kc = min(key, a.M - 1);
+  const unsigned char* mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+  const unsigned long long seen64 = keys_seen<NW * 32>(mask, 0, a.M, lane);
+  const bool seen = (seen64 >> key) & 1;
+  const unsigned seen32 = (unsigned)(seen64 >> k0);
+  char* ktile = tiles_lds + 2 * R * kTile;
+  const T* kbase = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
+  const typename TL::template Loader<NW * 32, NW> lk(a.k_sn, a.k_sm, tid);
+  lk(ktile, kbase, a.M, tid, wave);
+  F vf[NV];
+  {
+    const T* v = (const T*)a.v + b * a.v_sb + kc * a.v_sn + hk * a.v_sh + 8 * h;
+#pragma unroll
+    for (int s = 0; s < NV; ++s) vf[s] = load8<T>(v + 16 * s);
+    if (!seen) {                                                               // what stands in masked keys may be anything, and 0 * NaN is NaN
+#pragma unroll
+      for (int s = 0; s < NV; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) vf[s][j] = (T)0.f;
+    }
+  }
+  // queries that see nothing stand in front (see above)
+  const int key0 = seen64 ? __builtin_ctzll(seen64) : 0, blind = !seen64 ? a.N : a.causal ? max(0, key0 - off) : 0;
+  const int first = blind / QT, total = blind < a.N ? ((a.N + QT - 1) / QT - first) * a.G : 0;
+  if (a.dq) {                                                                  // blocks of them are left out
+    const int none = total ? first * QT : a.N, per = 2 * D / 4;
+    for (int i = tid; i < none * a.G * per; i += NW * 64) {
+      const int n = i / (a.G * per), e = i - n * a.G * per;
+      store4<T>((T*)a.dq + (((long long)b * a.N + n) * a.H + hk * a.G) * 2 * D + 4 * e, 0.f, 0.f, 0.f, 0.f);
+    }
+  }
+  f32x16 dk[2][NC], dv[ND], s[2], g;
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) dk[m][c] = zero16();
+#pragma unroll
+  for (int c = 0; c < ND; ++c) dv[c] = zero16();
+  float dlam = 0.f;
+
+  auto qtile = [&](int t) { return tiles_lds + (t % R) * kTile; };
+  auto gtile = [&](int t) { return tiles_lds + (R + t % R) * kTile; };
+  const typename TL::template Loader<QT, NW> lq(a.q_sn, a.q_sm, tid), lg((long long)a.H * 2 * D, D, tid);
+  int to_head = hk * a.G, to_n = first * QT;                                   // what the next fetch brings
+  auto fetch = [&](int t) {
+    const int head = to_head, n0 = to_n;
+    to_n += QT;
+    if (to_n >= a.N) { to_n = first * QT; ++to_head; }
+    lq(qtile(t), (const T*)a.q + b * a.q_sb + head * a.q_sh + n0 * a.q_sn, a.N - n0, tid, wave, blind - n0);
+    lg(gtile(t), (const T*)a.dout + (((long long)b * a.N + n0) * a.H + head) * 2 * D, a.N - n0, tid, wave, blind - n0);
+    if (wave == 0)
+      fetch4(a.lse + ((long long)b * a.H + head) * 2 * a.N + n0, ((unsigned)h * a.N + min(lane & 31, a.N - 1 - n0)) * 4u, lds_address(&stat[t % R][0][0]));
+  };
+  if (total > 0) {
+    fetch(0);
+    int head = hk * a.G, n0 = first * QT;
+    float lam = lam_of<T>(a, head);
+    for (int t = 0; t < total; ++t) {
+      fetched();                                                               // block t has come
+      if (t == 0 && seen64 != (NW == 2 ? ~0ull : 0xffffffffull)) {
+        TL::template clear<NW * 32, NW * 64>(ktile, seen64, tid);
+        __syncthreads();
+      }
+      if (t + 1 < total) fetch(t + 1);
+      const char *qb = qtile(t), *gb = gtile(t);
+      s[0] = s[1] = g = zero16();
+      struct Two { F q, k; };
+      weave<Two, 2 * NK, 1>([&](int i) { return Two{TL::row(qb, at, (i & 1) * NK + i / 2), TL::row(ktile + wave * kTile, at, (i & 1) * NK + i / 2)}; },
+                            [&](int i, const Two& f) { s[i & 1] = mma(f.q, f.k, s[i & 1]); }, [](int) {});
+      weave<F, NV, 2>([&](int i) { return TL::row(gb, at, i); }, [&](int i, const F& f) { g = mma(f, vf[i], g); }, [](int) {});
+      if (n0 + QT > a.N || seen32 != ~0u || (a.causal && k0 + 31 > n0 + off)) {
+        const unsigned ok = seen ? rows_of_lane(a.causal ? key - off - n0 : 0, a.N - 1 - n0, h) : 0u;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int m = 0; m < 2; ++m) s[m][i] = (ok >> row_of(i, 0)) & 1 ? s[m][i] : -INFINITY;
+      }
+      F pc[2];
+      {
+        f32x16 p;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          typedef float f4 __attribute__((ext_vector_type(4)));
+          const f4 e0 = *(const f4*)&stat[t % R][0][8 * u + 4 * h], e1 = *(const f4*)&stat[t % R][1][8 * u + 4 * h];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int x = 4 * u + j;
+            s[0][x] = __builtin_amdgcn_exp2f(fmaf(s[0][x], a.c, -e0[j]));
+            s[1][x] = __builtin_amdgcn_exp2f(fmaf(s[1][x], a.c, -e1[j]));
+            p[x] = fmaf(-lam, s[1][x], s[0][x]);
+          }
+        }
+        sums[wave][(lane >> 4) & 1][row_of(lane & 15, h)] = sums_of_half(s[0] * g, s[1] * g, lane);
+        pc[0] = pack<T>(p, 0);
+        pc[1] = pack<T>(p, 1);
+      }
+      weave<F, 2 * ND, 2>([&](int i) { return TL::col(gb, at, i / ND, i % ND); }, [&](int i, const F& f) { dv[i % ND] = mma(f, pc[i / ND], dv[i % ND]); }, [](int) {});
+      __syncthreads();
+      F ds[2][2];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        typedef float f4 __attribute__((ext_vector_type(4)));
+        f4 d0 = *(const f4*)&sums[0][0][8 * u + 4 * h], d1 = *(const f4*)&sums[0][1][8 * u + 4 * h];
+        if constexpr (NW > 1) {
+          d0 += *(const f4*)&sums[1][0][8 * u + 4 * h];
+          d1 += *(const f4*)&sums[1][1][8 * u + 4 * h];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int x = 4 * u + j;
+          if (n0 + 8 * u + 4 * h + j < a.N) dlam += d1[j];
+          s[0][x] *= g[x] - d0[j];
+          s[1][x] *= lam * (g[x] - d1[j]);                                     // (without the sign)
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          ds[m][i] = pack<T>(s[m], i);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) turned[m][row_of(8 * i + j, h)][key] = ds[m][i][j];
+        }
+      weave<F, 4 * NC, 2>([&](int i) { return TL::col(qb, at, i / (2 * NC), i % (2 * NC)); },
+                          [&](int i, const F& f) {
+                            const int c = i % (2 * NC);
+                            dk[c / NC][c % NC] = mma(f, ds[c / NC][i / (2 * NC)], dk[c / NC][c % NC]);
+                          },
+                          [](int) {});
+      __syncthreads();
+      if (a.dq)
+        for (int m = wave; m < 2; m += NW) {
+          f32x16 dq[NC];
+#pragma unroll
+          for (int c = 0; c < NC; ++c) dq[c] = zero16();
+#pragma unroll
+          for (int i = 0; i < NW * 2; ++i) {
+            const T* e = &turned[m][lane & 31][16 * i + 4 * h];
+            const F w = __builtin_shufflevector(*(const t4*)e, *(const t4*)(e + 8), 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) dq[c] = mma(TL::col(ktile, at, i, m * NC + c), w, dq[c]);
+          }
+          const int n = n0 + (lane & 31);
+          const float f = m ? -a.scale : a.scale;
+          if (n < a.N) {
+            T* out = (T*)a.dq + (((long long)b * a.N + n) * a.H + head) * 2 * D + m * D + 4 * h;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+              for (int u = 0; u < 4; ++u) store4<T>(out + 32 * c + 8 * u, dq[c][4 * u] * f, dq[c][4 * u + 1] * f, dq[c][4 * u + 2] * f, dq[c][4 * u + 3] * f);
+          }
+        }
+      n0 += QT;
+      if (n0 >= a.N) {                                                         // the head's last block
+        dlam += __shfl_xor(dlam, 32, 64);
+        if (tid == 0) a.dlam_part[(long long)bh * a.G + head - hk * a.G] = dlam;
+        dlam = 0.f;
+        n0 = first * QT;
+        if (t + 1 < total) lam = lam_of<T>(a, ++head);
+      }
+    }
+  } else {
+    for (int i = tid; i < a.G; i += NW * 64) a.dlam_part[(long long)bh * a.G + i] = 0.f;
+  }
+  fetched();                                                                   // (nothing is on its way to LDS when the workgroup ends)
+  if (key >= a.M || !a.dk) return;
+  const long long oat = (((long long)b * a.M + key) * a.Hk + hk) * 2 * D + 4 * h;
+  auto put = [&](T* out, const f32x16& x, float f) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      store4<T>(out + 8 * u, seen ? x[4 * u] * f : 0.f, seen ? x[4 * u + 1] * f : 0.f, seen ? x[4 * u + 2] * f : 0.f, seen ? x[4 * u + 3] * f : 0.f);
+  };
+#pragma unroll
+  for (int c = 0; c < ND; ++c) put((T*)a.dv + oat + 32 * c, dv[c], 1.f);
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) put((T*)a.dk + oat + m * D + 32 * c, dk[m][c], m ? -a.scale : a.scale);
+}
+
 // Adds the shares of a gradient, in order; n a multiple of 4
 template <typename T>
 __global__ __launch_bounds__(256) void diff_attn_add(const float* part, T* out, long long n, int shares) {

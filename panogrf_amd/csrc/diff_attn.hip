@@ -49,6 +49,9 @@ static BwdCut cut_bwd(int dtype, int B, int N, int M, int H, int Hk, int D, bool
   BwdCut c;
   const int G = H / Hk, places = dtype == PGRF_DTYPE_F32 || D == 128 ? 256 : 512;
   const long long rows = (long long)N * G;
+  // Key heads with up to 64 keys, as long as there is one for every CU: a workgroup each forms all gradients (row_waves 0).  (float, D = 32, 64 keys: 2048 rays of 4 heads x
+  // 64 samples 351 us, with the two kernels 523; 256 key heads x 2048 queries 400, 512; 128 of them 404, 270.  At D = 64 float's values fill the registers: 535 both ways.)
+  if (M <= 64 && D * (int)dtype_bytes(dtype) <= 128 && (long long)B * Hk >= 256) return {0, M > 32 ? 2 : 1, 1, 1, 1, 0, (long long)B * Hk};
   c.row_waves = waves_for(rows);
   c.key_waves = waves_for(M);
   c.row_groups = (long long)B * Hk * ((rows + c.row_waves * 32 - 1) / (c.row_waves * 32));

@@ -50,6 +50,19 @@ static void launch_dkv(const DiffArgs& a, unsigned grid, hipStream_t s) {
 
 int PGRF_DA_NAME(launch_da_bwd)(const DiffArgs& a, int row_waves, unsigned row_grid, int units, int key_waves, unsigned key_grid, hipStream_t s) {
   const char* who = "pgrf_diff_attention_backward";
+  auto lams = [&]() { hipLaunchKernelGGL((diff_attn_dlam<DaT>), dim3(a.H), dim3(1024), 0, s, a, units); };
+#if PGRF_DA_D == 32 || (PGRF_DA_D == 64 && PGRF_DA_TYPE != 0)
+  if (row_waves == 0) {
+    if (key_waves == 1) hipLaunchKernelGGL((diff_attn_short<DaT, PGRF_DA_D, 1>), dim3(key_grid), dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((diff_attn_short<DaT, PGRF_DA_D, 2>), dim3(key_grid), dim3(128), 0, s, a);
+    PGRF_TOK_LAUNCHED(who);
+    if (a.dlam) {
+      lams();
+      PGRF_TOK_LAUNCHED(who);
+    }
+    return PGRF_OK;
+  }
+#endif
   if (row_waves == 1) hipLaunchKernelGGL((diff_attn_dq<DaT, PGRF_DA_D, 1>), dim3(row_grid), dim3(64), 0, s, a);
   else if (row_waves == 2) hipLaunchKernelGGL((diff_attn_dq<DaT, PGRF_DA_D, 2>), dim3(row_grid), dim3(128), 0, s, a);
   else hipLaunchKernelGGL((diff_attn_dq<DaT, PGRF_DA_D, 4>), dim3(row_grid), dim3(256), 0, s, a);
@@ -62,7 +75,7 @@ int PGRF_DA_NAME(launch_da_bwd)(const DiffArgs& a, int row_waves, unsigned row_g
     PGRF_TOK_LAUNCHED(who);
   }
   if (a.dlam) {
-    hipLaunchKernelGGL((diff_attn_dlam<DaT>), dim3(a.H), dim3(1024), 0, s, a, units);
+    lams();
     PGRF_TOK_LAUNCHED(who);
   }
   if (a.dk) {

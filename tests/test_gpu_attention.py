@@ -89,6 +89,31 @@ def test_what_masked_places_hold_does_not_matter(dtype):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize('dtype,D', [('f32', 32), ('bf16', 32), ('f16', 32), ('bf16', 64), ('f16', 64)])
+@pytest.mark.parametrize('B,N,M,H,Hk', [(64, 64, 64, 4, 4), (256, 33, 40, 1, 1), (65, 70, 17, 12, 4), (128, 31, 32, 4, 2), (300, 1, 64, 1, 1), (90, 5, 1, 6, 3), (256, 100, 33, 2, 1)])
+@pytest.mark.parametrize('causal,mask', [(False, 'none'), (True, 'none'), (False, 'holes'), (True, 'tail')])
+def test_many_heads_of_few_keys(B, N, M, H, Hk, dtype, D, causal, mask):
+    q, k, v, lam, do = make(B, N, M, H, Hk, D, dtype)
+    m = mask_of(mask, B, M)
+    check(q, k, v, lam, do, causal, m)
+    # what masked keys and queries that see nothing hold does not matter
+    see = R.may_see(B, N, M, causal, m)
+    blind, hidden = ~see.any(2), torch.zeros(B, M, dtype=torch.bool, device='cuda') if m is None else ~m
+    want = grads(q, k, v, lam, do, causal=causal, key_mask=m)
+    q, k, v, do = q.clone(), k.clone(), v.clone(), do.clone()
+    q[blind], do[blind], k[hidden], v[hidden] = float('nan'), float('inf'), float('nan'), float('nan')
+    assert all(torch.equal(a, b) for a, b in zip(grads(q, k, v, lam, do, causal=causal, key_mask=m), want))
+
+
+def test_few_keys_one_gradient_at_a_time():
+    q, k, v, lam, do = make(64, 40, 50, 8, 4, 32, 'f32')
+    want = grads(q, k, v, lam, do)
+    from panogrf_amd.attention import diff_attention
+    for i in range(4):
+        ts = [t.clone().requires_grad_(j == i) for j, t in enumerate((q, k, v, lam))]
+        assert torch.equal(torch.autograd.grad(diff_attention(*ts), ts[i], do)[0], want[1 + i])
+
+
 @pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
 @pytest.mark.parametrize('D', [32, 64, 128])
 @pytest.mark.parametrize('M', [70, 600])
