@@ -138,7 +138,8 @@ def diff_attention(q, k, v, lam, *, causal=False, key_mask=None, scale=None):
 def diff_attention_cached(q, k_cache, v_cache, lam, lengths, *, scale=None):
     """The same over a cache: k_cache [B, M, Hk, 2, d], v_cache [B, M, Hk, 2 d] of which the first lengths[b] keys count (lengths [B] int32 on the device,
     clamped to [0, M]; the rest may hold anything).  q [B, N, H, 2, d]: the last N tokens of each entry, causal among themselves: query i sees keys up to
-    lengths[b] - N + i.  N = 1 is the step of a served model.  The lengths are read on the device, so a captured step follows them.  No gradients."""
+    lengths[b] - N + i.  N = 1 is the step of a served model.  The lengths are read on the device, so a captured step follows them.  Where 32 query heads and
+    tokens at most share a key head, probabilities are not rounded to the tensors' type.  No gradients."""
     who = 'diff_attention_cached'
     scale = _check(who, q, k_cache, v_cache, lam, scale)
     require(torch.is_tensor(lengths) and lengths.dtype == torch.int32 and lengths.device == q.device and tuple(lengths.shape) == (q.shape[0],), who,

@@ -261,10 +261,14 @@ template <typename T, int D, int NW> struct FwdShape {
   static_assert(D < 128 || NW > 1, "a pair of waves at D = 128");
   static constexpr int MPW = D == 128 ? 1 : 2, RW = NW * MPW / 2;              // RW: groups of 32 rows in the workgroup
   static constexpr int KT = 32;                                                // keys of a block
-  // Float from D = 64 on: one wave on a SIMD (its operands take twice the registers) with three blocks in work.  All others: two waves on a SIMD.
+  // Float from D = 64 on: one wave on a SIMD (its operands take twice the registers) with three blocks in work.  All others: two waves on a SIMD, but for a workgroup of one
+  // wave, which memory bounds (over caches 245 us with all registers it wants, 267 with half of them).
   static constexpr bool kWeave = sizeof(T) == 4 && D > 32;
   static constexpr int kMinWaves = kWeave || NW == 1 ? 1 : 2;
   static constexpr int kTileKeys = sizeof(T) == 2 && RW == 4 ? 64 : 32;        // keys between barriers: fewer barriers where LDS holds two such tiles
+  // Up to 32 rows (single tokens) memory bounds the kernel, and probabilities go into the product with v in two pieces, what the type holds and what that leaves (the result is
+  // off by 0.0017 of its norm, all from its own rounding to bf16; 0.0026 with one piece.  Caches as in cut_fwd: 246 us both ways).  Elsewhere that would cost half the speed.
+  static constexpr bool kTwoPieces = sizeof(T) == 2 && RW == 1;
 };
 
 // Scores of a block: S^T of MPW maps
@@ -293,7 +297,8 @@ __device__ __forceinline__ float with_other_half(float t) {                    /
 // products of 32x32x16 (386 ns at its peak) and the vector pipe 96 FMAs and 32 exponentials with their sums and roundings (over 312 ns); side by side the two take 471 ns
 // at best, and here they are busy for 44% and 56% of the time.  With kWeave a wave has three blocks in work: while block j goes through its exponentials, the matrix pipe
 // forms the scores of block j + 1 and adds block j - 1 times its values, in one stretch of code without a branch; masks and a new maximum are dealt with in front of it.
-// P1 and P2 are each rounded to the tensors' type for their product with v: the difference of the two could be rounded once only where both rows' sums are known first.
+// P1 and P2 are each rounded to the tensors' type for their product with v (their difference could be rounded once only if both rows' sums were known first); what the two
+// maps have in common cancels in out and their roundings do not, which is where 0.0026 of its norm in bf16 comes from (0.0017 is its own rounding).
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff_attn_fwd(DiffArgs a) {
   using TL = Tile<T, D>;
@@ -354,7 +359,7 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
   auto fetch_v = [&](int t) { lv(vtile(t), v + (long long)t * KT * a.v_sn, len - t * KT, tid, wave); };
 
   f32x16 o[MPW][NC], s[MPW];
-  F p[MPW][2];
+  F p[MPW][2], rest[Sh::kTwoPieces ? MPW : 1][2];
   float mx[MPW], l[MPW], top[MPW];
 #pragma unroll
   for (int m = 0; m < MPW; ++m) {
@@ -525,13 +530,17 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
             const float w = __builtin_amdgcn_exp2f(fmaf(s[m][e], a.c, -base));
             sum += w;
             p[m][e / 8][e % 8] = (T)w;
+            if constexpr (Sh::kTwoPieces) rest[m][e / 8][e % 8] = (T)(w - (float)(T)w);
           }
           l[m] += sum;
         }
         weave<F, 2 * NC, 2>([&](int i) { return TL::col(vb, at, i / NC, i % NC); },
                             [&](int i, const F& f) {
 #pragma unroll
-                              for (int m = 0; m < MPW; ++m) o[m][i % NC] = mma(f, p[m][i / NC], o[m][i % NC]);
+                              for (int m = 0; m < MPW; ++m) {
+                                o[m][i % NC] = mma(f, p[m][i / NC], o[m][i % NC]);
+                                if constexpr (Sh::kTwoPieces) o[m][i % NC] = mma(f, rest[m][i / NC], o[m][i % NC]);
+                              }
                             },
                             [](int) {});
       }

@@ -21,10 +21,10 @@ static FwdCut cut_fwd(int dtype, int B, int Hk, long long rows, int M, int D) {
   if (D == 128) f.waves = f.waves == 4 && dtype == PGRF_DTYPE_F32 ? 4 : 2 * f.waves;
   f.rows = D == 128 ? f.waves * 16 : f.waves * 32;
   const long long groups = (long long)B * Hk * ((rows + f.rows - 1) / f.rows);
-  // The key axis is cut where the rows alone leave the chip idle.  Up to 32 rows (single tokens): 1280 workgroups of one wave fit the chip (two buffers of 32 KB each), and
-  // as many shares are dealt out; more of them cost more in partial sums than they even out (32 caches of 4096 to 16384 keys, 8 key heads, bf16, D = 64: 245 us; with
-  // 2560 shares 257, with 5120 285, with 1024 263).  More rows: 512 workgroups fit, and from half of that on the join costs more than the idle half (2048 x 8192, 16
-  // heads: 245 us whole, 271 cut).  None is under 128 keys.
+  // The key axis is cut where the rows alone leave the chip idle.  Up to 32 rows (single tokens) it is dealt out to five workgroups of one wave for every CU; more of them
+  // cost more in partial sums than they even out (32 caches of 4096 to 16384 keys, 8 key heads, bf16, D = 64: 245 us; with 1024 263, with 2560 257, with 5120 285).
+  // More rows: 512 workgroups fit, and from half of that on the join costs more than the idle half (2048 x 8192, 16 heads: 245 us whole, 271 cut).  No share is under
+  // 128 keys.
   const bool few = rows <= 32;
   const long long want = few ? 1280 : 512, most = M / 128;
   long long s = !few && groups > want / 2 ? 1 : (want + groups - 1) / groups;
