@@ -625,43 +625,88 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
   }
 }
 
-// Joins the shares of a cut key axis, in order: one thread per value of a row
-template <typename T, int D>
-__global__ __launch_bounds__(256) void diff_attn_join(DiffArgs a) {
-  const int rows = a.N * a.G, per = 256 / (2 * D);
-  const long long all = (long long)a.B * a.Hk * rows, row = (long long)blockIdx.x * per + threadIdx.x / (2 * D);
+// Joins the shares of a cut key axis: S groups of threads take every S-th share of a row, four at a time so that their loads are on their way together (one after the other
+// 128 shares took 70 us), and the groups are joined in order; one thread per value and group.
+template <typename T, int D, int S>
+__global__ __launch_bounds__(S > 1 ? 2 * D * S : 256) void diff_attn_join(DiffArgs a) {
+  constexpr int kRows = S > 1 ? 1 : 256 / (2 * D);                             // rows of a workgroup
+  __shared__ __attribute__((aligned(16))) float sums[S > 1 ? S : 1][4];
+  __shared__ float values[S > 1 ? S : 1][2][2 * D];
+  const int rows = a.N * a.G, ch = threadIdx.x % (2 * D), group = S > 1 ? threadIdx.x / (2 * D) : 0;
+  const long long all = (long long)a.B * a.Hk * rows, row = (long long)blockIdx.x * kRows + (S > 1 ? 0 : threadIdx.x / (2 * D));
   if (row >= all) return;
-  const int ch = threadIdx.x % (2 * D);
-  float m0 = -INFINITY, m1 = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) {
-    const float4 e = *(const float4*)(a.part_ml + (s * all + row) * 4);
-    m0 = fmaxf(m0, e.x);
-    m1 = fmaxf(m1, e.z);
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[2] = {0.f, 0.f};
+  // adds up to four parts of (m1, l1, m2, l2) and two values; one that saw no key (its values were never written) counts for nothing
+  auto add = [&](const float4 (&e)[4], const float (&v)[4][2]) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float top = m[k];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = fmaxf(top, k ? e[j].z : e[j].x);
+      const float f = m[k] == -INFINITY ? 0.f : exp2f(m[k] - top);
+      l[k] *= f;
+      o[k] *= f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float mj = k ? e[j].z : e[j].x, lj = k ? e[j].w : e[j].y, w = mj == -INFINITY ? 0.f : exp2f(mj - top);
+        const bool none = e[j].x == -INFINITY && e[j].z == -INFINITY && e[j].y == 0.f && e[j].w == 0.f;
+        l[k] = fmaf(w, lj, l[k]);
+        o[k] = none ? o[k] : fmaf(w, v[j][k], o[k]);
+      }
+      m[k] = top;
+    }
+  };
+  const float4 nothing = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+  for (int s = group; s < a.splits; s += 4 * S) {
+    float4 e[4];
+    float v[4][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const long long at = min(s + j * S, a.splits - 1) * all + row;           // (behind the last: read again, not counted)
+      const float* p = a.part_o + at * 4 * D + ch;
+      e[j] = *(const float4*)(a.part_ml + at * 4);
+      v[j][0] = p[0];
+      v[j][1] = p[2 * D];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (s + j * S >= a.splits) e[j] = nothing;
+    add(e, v);
   }
-  float l0 = 0.f, l1 = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float4 e = *(const float4*)(a.part_ml + (s * all + row) * 4);
-    const float* p = a.part_o + (s * all + row) * 4 * D + ch;
-    if (e.x == -INFINITY && e.z == -INFINITY && e.y == 0.f && e.w == 0.f) continue;
-    const float w0 = e.x == -INFINITY ? 0.f : exp2f(e.x - m0), w1 = e.z == -INFINITY ? 0.f : exp2f(e.z - m1);
-    l0 = fmaf(w0, e.y, l0);
-    l1 = fmaf(w1, e.w, l1);
-    o0 = fmaf(w0, p[0], o0);
-    o1 = fmaf(w1, p[2 * D], o1);
+  if constexpr (S > 1) {
+    if (ch == 0) *(float4*)sums[group] = make_float4(m[0], l[0], m[1], l[1]);
+    values[group][0][ch] = o[0];
+    values[group][1][ch] = o[1];
+    __syncthreads();
+    if (group) return;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = o[0] = o[1] = 0.f;
+#pragma unroll
+    for (int g = 0; g < S; g += 4) {
+      float4 e[4];
+      float v[4][2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        e[j] = *(const float4*)sums[g + j];
+        v[j][0] = values[g + j][0][ch];
+        v[j][1] = values[g + j][1][ch];
+      }
+      add(e, v);
+    }
   }
   const int bh = (int)(row / rows), r = (int)(row % rows), b = bh / a.Hk, head = bh % a.Hk * a.G + r % a.G, n = r / a.G;
-  o0 *= l0 > 0.f ? 1.f / l0 : l0;
-  o1 *= l1 > 0.f ? 1.f / l1 : l1;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) o[k] *= l[k] > 0.f ? 1.f / l[k] : l[k];
   const long long at = ((long long)b * a.N + n) * a.H + head;
-  ((T*)a.out)[at * 2 * D + ch] = (T)(o0 - lam_of<T>(a, head) * o1);
+  ((T*)a.out)[at * 2 * D + ch] = (T)(o[0] - lam_of<T>(a, head) * o[1]);
   if (a.o12) {
-    a.o12[at * 4 * D + ch] = o0;
-    a.o12[at * 4 * D + 2 * D + ch] = o1;
+    a.o12[at * 4 * D + ch] = o[0];
+    a.o12[at * 4 * D + 2 * D + ch] = o[1];
   }
   if (a.lse && ch == 0) {
     float* e = a.lse + ((long long)b * a.H + head) * 2 * a.N + n;
-    e[0] = l0 == 0.f ? INFINITY : m0 + log2f(l0);
-    e[a.N] = l1 == 0.f ? INFINITY : m1 + log2f(l1);
+    e[0] = l[0] == 0.f ? INFINITY : m[0] + log2f(l[0]);
+    e[a.N] = l[1] == 0.f ? INFINITY : m[1] + log2f(l[1]);
   }
 }
 

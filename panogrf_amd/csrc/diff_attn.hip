@@ -22,11 +22,11 @@ static FwdCut cut_fwd(int dtype, int B, int Hk, long long rows, int M, int D) {
   f.rows = D == 128 ? f.waves * 16 : f.waves * 32;
   const long long groups = (long long)B * Hk * ((rows + f.rows - 1) / f.rows);
   // The key axis is cut where the rows alone leave the chip idle.  Up to 32 rows (single tokens) it is dealt out to five workgroups of one wave for every CU; more of them
-  // cost more in partial sums than they even out (32 caches of 4096 to 16384 keys, 8 key heads, bf16, D = 64: 245 us; with 1024 263, with 2560 257, with 5120 285).
-  // More rows: 512 workgroups fit, and from half of that on the join costs more than the idle half (2048 x 8192, 16 heads: 245 us whole, 271 cut).  No share is under
-  // 128 keys.
+  // cost more in partial sums than they even out (32 caches of 4096 to 16384 keys, 8 key heads, bf16, D = 64: 245 us; with 1024 263, with 2560 257, with 5120 285).  There a
+  // share may be a single block of 32 keys, as a wave's blocks come one after the other (one cache of 500 keys, 2 key heads: 10.5 us; with 64 keys at least 11.0, with
+  // 128 15.7).  More rows: 512 workgroups fit, and from half of that on the join costs more than the idle half (2048 x 8192, 16 heads: 245 us whole, 271 cut).
   const bool few = rows <= 32;
-  const long long want = few ? 1280 : 512, most = M / 128;
+  const long long want = few ? 1280 : 512, most = few ? (M + 31) / 32 : M / 128;
   long long s = !few && groups > want / 2 ? 1 : (want + groups - 1) / groups;
   if (s > most) s = most;
   if (s > 128) s = 128;

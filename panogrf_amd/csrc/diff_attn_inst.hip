@@ -31,7 +31,9 @@ int PGRF_DA_NAME(launch_da_fwd)(const DiffArgs& a, int waves, unsigned grid, hip
   PGRF_TOK_LAUNCHED(who);
   if (a.splits > 1) {
     const long long rows = (long long)a.B * a.Hk * a.N * a.G, per = 256 / (2 * PGRF_DA_D);
-    hipLaunchKernelGGL((diff_attn_join<DaT, PGRF_DA_D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, a);
+    constexpr int S = 1024 / (2 * PGRF_DA_D);
+    if (a.splits > 8) hipLaunchKernelGGL((diff_attn_join<DaT, PGRF_DA_D, S>), dim3((unsigned)rows), dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((diff_attn_join<DaT, PGRF_DA_D, 1>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, a);
     PGRF_TOK_LAUNCHED(who);
   }
   return PGRF_OK;
