@@ -295,7 +295,7 @@ __device__ __forceinline__ float with_other_half(float t) {                    /
 
 // One pass over the keys in blocks of 32 with the running maximum and sum of each row's softmax.  What bounds it: per block and wave at D = 64 the matrix pipe has 24
 // products of 32x32x16 (386 ns at its peak) and the vector pipe 96 FMAs and 32 exponentials with their sums and roundings (over 312 ns); side by side the two take 471 ns
-// at best, and here they are busy for 44% and 56% of the time.  With kWeave a wave has three blocks in work: while block j goes through its exponentials, the matrix pipe
+// at best, and here they are busy for 45% and 57% of the time (2 x 8192 rows and keys, 8 heads, bf16: 895 us, 924 TFLOP/s; at D = 128 no exponential is left over, 1000).  With kWeave a wave has three blocks in work: while block j goes through its exponentials, the matrix pipe
 // forms the scores of block j + 1 and adds block j - 1 times its values, in one stretch of code without a branch; masks and a new maximum are dealt with in front of it.
 // P1 and P2 are each rounded to the tensors' type for their product with v (their difference could be rounded once only if both rows' sums were known first); what the two
 // maps have in common cancels in out and their roundings do not, which is where 0.0026 of its norm in bf16 comes from (0.0017 is its own rounding).
@@ -716,7 +716,8 @@ __global__ __launch_bounds__(S > 1 ? 2 * D * S : 256) void diff_attn_join(DiffAr
 // dlam) and once by keys (dk, dv), 14 instead of 10 products of N M D, so that no two workgroups add to one value and gradients do not depend on scheduling.
 //
 // Two waves or more share a SIMD and run beside each other, but for dq and dk at D = 128 in 16 bits, whose registers leave a SIMD one wave: those weave three blocks as the
-// forward kernel does.  Float does neither, as its products take eight times as long and hide the rest by themselves.
+// forward kernel does.  Float does neither, as its products take eight times as long and hide the rest by themselves.  Both pipes are bound as in the forward kernel (2 x 8192,
+// 8 heads, bf16, D = 64: dq 920 us, 896 TFLOP/s; dk and dv 1244 us, 884 TFLOP/s).
 template <typename T, int D, bool MORE = true> struct BwdShape {               // MORE: dq or dk is formed
   static constexpr bool kWeave = sizeof(T) == 2 && D == 128 && MORE;
   static constexpr int kMinWaves = sizeof(T) == 2 && !kWeave ? 2 : 1;
@@ -1267,7 +1268,9 @@ __device__ __forceinline__ float sums_of_half(const f32x16& a, const f32x16& b, 
 
 // All gradients of a key head with up to 64 keys in one go: a workgroup holds the keys, a wave 32 of them, and the queries of the head pass by once, so that scores, maps and
 // the products with v are formed once (10 products of N M D where the two kernels above have 14, or 20 with delta's sweep) and every input is read once.  delta is the sum of
-// a row's A G over the lanes and waves that hold its keys; score gradients go through LDS, turned round, to the sum over keys that is dq.
+// a row's A G over the lanes and waves that hold its keys; score gradients go through LDS, turned round, to the sum over keys that is dq.  Bound by its chain of loads, products
+// and stores with a wave on a SIMD (2048 rays x 4 heads x 64 samples, float, D = 32: 351 us, the matrix pipe busy for 41%; three workgroups to a CU, or starts apart from each
+// other, were no quicker).
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, 1) void diff_attn_short(DiffArgs a) {
   using TL = Tile<T, D>;
