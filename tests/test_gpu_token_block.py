@@ -227,6 +227,60 @@ def test_second_derivatives_are_refused():
             torch.autograd.grad(g.square().sum(), x)
 
 
+@pytest.fixture
+def room():
+    """Tensors of over 2^31 values, here and nowhere else."""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip('needs 60 GB')
+    yield
+    torch.cuda.empty_cache()
+
+
+def test_norms_and_rotations_of_over_2_to_the_31_values(room):
+    """What stands behind 2^31 values is what the same rows give by themselves."""
+    from panogrf_amd.block_norm import block_norm
+    from panogrf_amd.rotary import rotary
+    rows, C = 265000, 8192
+    x = torch.randn(rows, C, device='cuda', dtype=torch.bfloat16)
+    y, ends = x.flip(1), (slice(0, 300), slice(rows - 300, rows))
+    assert x.numel() > 2 ** 31
+    w = torch.rand(C, device='cuda').to(x.dtype)
+    for e in ends:
+        xs, ys = x[e].clone(), y[e].clone()
+        got = block_norm(x, y, post_weight=w, kind='layer')
+        assert all(torch.equal(a[e], b) for a, b in zip(got, block_norm(xs, ys, post_weight=w, kind='layer')))
+        del got
+    xl, yl = x.requires_grad_(True), y.requires_grad_(True)
+    out = block_norm(xl, yl, post_weight=w, kind='rms')
+    dx, dy = torch.autograd.grad(out, [xl, yl], [x.detach(), y.detach()])
+    del out
+    for e in ends:
+        xs, ys = x.detach()[e].clone().requires_grad_(True), y.detach()[e].clone().requires_grad_(True)
+        want = torch.autograd.grad(block_norm(xs, ys, post_weight=w, kind='rms'), [xs, ys], [xs.detach(), ys.detach()])
+        assert torch.equal(dx[e], want[0]) and torch.equal(dy[e], want[1])
+    del xl, yl, dx, dy, y
+    q = x.detach().view(1, rows, 128, 64)
+    turned, _ = rotary(q, None, torch.arange(rows, device='cuda'))
+    for e in ends:
+        assert torch.equal(turned[:, e], rotary(q[:, e].clone(), None, torch.arange(rows, device='cuda')[e])[0])
+
+
+def test_attention_of_over_2_to_the_31_values(room):
+    from panogrf_amd.attention import diff_attention
+    B, N, M, H, D = 2, 131100, 33, 64, 64
+    q = torch.randn(B, N, H, 2, D, device='cuda', dtype=torch.bfloat16)
+    assert q.numel() > 2 ** 31
+    k, v, lam = torch.randn(B, M, H, 2, D, device='cuda').to(q.dtype), torch.randn(B, M, H, 2 * D, device='cuda').to(q.dtype), torch.rand(H, device='cuda')
+    q.requires_grad_(True)
+    out = diff_attention(q, k, v, lam)
+    dq, = torch.autograd.grad(out, q, q.detach().view(B, N, H, 2 * D))
+    qs = q.detach()[1:, N - 200:].clone().requires_grad_(True)
+    alone = diff_attention(qs, k[1:], v[1:], lam)
+    ds, = torch.autograd.grad(alone, qs, qs.detach().view(1, 200, H, 2 * D))
+    # (which rows share a workgroup does not enter a row's sums)
+    assert torch.equal(out[1:, N - 200:], alone) and torch.equal(dq[1:, N - 200:], ds)
+
+
 class TokenMono(nn.Module):
     """A small mono-depth net over the panorama's patches, behind the renderer's call d_net(erp, cube, dnet=True) -> {'pred_depth', 'mono_feat'}."""
 
