@@ -33,9 +33,12 @@ def _of_sizes(name, *sizes):
 
 def _pack(q, k, v, lam, mask, lengths, causal, scale, out, lse, maps, ws, ws_bytes):
     B, N, H, _, D = q.shape
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
-    return DIFF_ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), ptr(mask), ptr(lengths), ptr(out), ptr(lse), ptr(maps), ptr(ws), ws_bytes,
-                          qs[0], qs[1], qs[2], qs[3], ks[0], ks[1], ks[2], ks[3], vs[0], vs[1], vs[2], 0 if mask is None or B == 1 else mask.stride(0),
+    q0, q1, q2, q3, _ = q.stride()
+    k0, k1, k2, k3, _ = k.stride()
+    v0, v1, v2, _ = v.stride()
+    return DIFF_ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), 0 if mask is None else mask.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
+                          0 if out is None else out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if maps is None else maps.data_ptr(), 0 if ws is None else ws.data_ptr(),
+                          ws_bytes, q0, q1, q2, q3, k0, k1, k2, k3, v0, v1, v2, 0 if mask is None or B == 1 else mask.stride(0),
                           DTYPES[q.dtype], lam.dtype == torch.float32, B, N, k.shape[1], H, k.shape[2], D, causal, scale)
 
 
@@ -84,15 +87,16 @@ class _DiffAttention(torch.autograd.Function):
 
 
 def _check(who, q, k, v, lam, scale):
-    for name, t, axes in (('q', q, 5), ('k', k, 5), ('v', v, 4), ('lam', lam, 1)):
-        if not isinstance(t, torch.Tensor) or t.dim() != axes:
-            refuse(who, f'{name} must be a tensor of {axes} axes (q [B, N, H, 2, d], k [B, M, Hk, 2, d], v [B, M, Hk, 2 d], lam [H])')
+    tensor = torch.Tensor
+    if not (isinstance(q, tensor) and isinstance(k, tensor) and isinstance(v, tensor) and isinstance(lam, tensor) and q.dim() == k.dim() == 5 and v.dim() == 4 and lam.dim() == 1):
+        refuse(who, 'q [B, N, H, 2, d], k [B, M, Hk, 2, d], v [B, M, Hk, 2 d] and lam [H] must be tensors of these axes')
     dtype, device = q.dtype, q.device
     if dtype not in DTYPES:
         refuse(who, f'dtype {dtype} (float32, bfloat16 or float16)')
-    for name, t in (('k', k), ('v', v)):
-        if t.dtype != dtype or t.device != device:
-            alike(who, name, t, dtype, device)
+    if k.dtype != dtype or k.device != device:
+        alike(who, 'k', k, dtype, device)
+    if v.dtype != dtype or v.device != device:
+        alike(who, 'v', v, dtype, device)
     B, N, H, two, d = q.shape
     kB, M, Hk, ktwo, kd = k.shape
     if two != 2 or d not in (32, 64, 128):
@@ -142,9 +146,9 @@ def diff_attention_cached(q, k_cache, v_cache, lam, lengths, *, scale=None):
     tokens at most share a key head, probabilities are not rounded to the tensors' type.  No gradients."""
     who = 'diff_attention_cached'
     scale = _check(who, q, k_cache, v_cache, lam, scale)
-    require(torch.is_tensor(lengths) and lengths.dtype == torch.int32 and lengths.device == q.device and tuple(lengths.shape) == (q.shape[0],), who,
-            f'lengths must be an int32 tensor [{q.shape[0]}] on {q.device}')
-    require(not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_cache, v_cache, lam))), who,
-            'no gradients over a cache: call it under torch.no_grad(), or diff_attention with a key_mask')
+    if not (isinstance(lengths, torch.Tensor) and lengths.dtype == torch.int32 and lengths.device == q.device and lengths.dim() == 1 and lengths.shape[0] == q.shape[0]):
+        refuse(who, f'lengths must be an int32 tensor [{q.shape[0]}] on {q.device}')
+    if (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or lam.requires_grad) and torch.is_grad_enabled():
+        refuse(who, 'no gradients over a cache: call it under torch.no_grad(), or diff_attention with a key_mask')
     on_gpu(q, who)
     return _forward(_aligned(q), _aligned(k_cache), _aligned(v_cache), lam.contiguous(), None, lengths.contiguous(), True, scale, False)[0]

@@ -19,8 +19,8 @@ def _heads(t):
 
 def _launch(q, k, positions, call, backward):
     """-> tensors of the shapes of q and k, contiguous."""
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     B, N = q.shape[:2]
     if B and N:
         rot, interleaved, base, scaling, factor, trained, low, high, magnitude = call
