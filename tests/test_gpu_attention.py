@@ -310,6 +310,93 @@ def test_training_step_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
 
 
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('D', [32, 64, 128])
+@pytest.mark.parametrize('N', [20, 50, 140])
+def test_partial_last_blocks(N, D, dtype):
+    """Workgroups of every size, with a last block of keys that ends at every place of a tile of 64, and what stands behind it not finite."""
+    from panogrf_amd.attention import diff_attention_cached
+    for M in (20, 40, 84, 116, 148, 212, 257, 300, 383, 447, 511):
+        q, k, v, lam, _ = make(2, N, M + 70, 2, 2, D, dtype)
+        k[:, M:], v[:, M:] = float('nan'), float('inf')
+        n = torch.tensor([M, M + 1 - M % 3], dtype=torch.int32, device='cuda')
+        k[1, M:M + 2], v[1, M:M + 2] = 1.0, 1.0
+        behind = torch.arange(M + 70, device='cuda') >= n.view(-1, 1)
+        kz, vz = k.clone(), v.clone()
+        kz[behind], vz[behind] = 0, 0
+        ref = R.diff_attention(q, kz, vz, lam, R.may_see(2, N, M + 70, True, lengths=n), D ** -0.5, None, T[dtype])['out']
+        assert R.worst(diff_attention_cached(q, k, v, lam, n), *ref) <= 1, M
+
+
+# one workgroup for all gradients; shares of rows and keys; both with maps kept; the widest heads
+WAYS = [(64, 64, 64, 4, 4, 32, 'f32'), (1, 2048, 2048, 4, 2, 64, 'bf16'), (2, 700, 1100, 4, 4, 64, 'f16'), (1, 1100, 1100, 2, 1, 128, 'bf16')]
+
+
+@pytest.mark.parametrize('B,N,M,H,Hk,D,dtype', WAYS)
+def test_training_steps_of_every_way_in_graphs(B, N, M, H, Hk, D, dtype):
+    from panogrf_amd.attention import diff_attention
+    ts = [t.clone() for t in make(B, N, M, H, Hk, D, dtype)]
+    for t in ts[:4]:
+        t.requires_grad_(True)
+    mask = torch.ones(B, M, dtype=torch.bool, device='cuda')
+
+    def step():
+        out = diff_attention(*ts[:4], causal=True, key_mask=mask)
+        return (out.detach(),) + torch.autograd.grad(out, ts[:4], ts[4])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in range(3):
+        with torch.no_grad():
+            for t, x in zip(ts, make(B, N, M, H, Hk, D, dtype, seed=seed + 70)):
+                t.copy_(x)
+            mask.copy_(torch.arange(M, device='cuda') < M - 13 * seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in held]
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+def test_calls_beside_each_other():
+    """Every way on a stream of its own, all at once: the results of one after the other."""
+    args = [make(*w[:7], seed=90) for w in WAYS]
+    want = [grads(*a) for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in WAYS]
+    for _ in range(3):
+        got = []
+        for a, s in zip(args, streams):
+            with torch.cuda.stream(s):
+                got.append(grads(*a))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for g, w in zip(got, want) for x, y in zip(g, w))
+
+
+def test_long_caches_of_one_stream_in_a_graph():
+    """The cut of the key axis that a single stream's cache gets, replayed while its length grows."""
+    from panogrf_amd.attention import diff_attention_cached
+    q, k, v, lam, _ = make(1, 1, 5000, 8, 2, 64, 'bf16')
+    n = torch.tensor([4000], dtype=torch.int32, device='cuda')
+    diff_attention_cached(q, k, v, lam, n)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = diff_attention_cached(q, k, v, lam, n)
+    for length in (4000, 1, 0, 4999, 5000, 33):
+        n.fill_(length)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = held.clone()
+        assert torch.equal(got, diff_attention_cached(q, k, v, lam, n))
+        ref = R.diff_attention(q, k, v, lam, R.may_see(1, 1, 5000, True, lengths=n), 64 ** -0.5, None, T['bf16'])['out']
+        assert R.worst(got, *ref) <= 1
+
+
 def test_on_another_stream():
     q, k, v, lam, do = make(2, 100, 100, 2, 2, 64, 'bf16')
     want = grads(q, k, v, lam, do)
