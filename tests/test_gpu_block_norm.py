@@ -88,6 +88,14 @@ def test_without_weights_and_gate(C, kind, dtype):
     check(make((2, 5, C), dtype, kind, 'none', 14, weights=False), kind, 'none', 0.7, dtype)
 
 
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('kind', ['rms', 'layer'])
+@pytest.mark.parametrize('shape,gate', [((1, 1700, 4104), 'channel'), ((2, 850, 8192), 'full'), ((3, 600, 5001), 'sample'), ((1, 1601, 4097), 'none')])
+def test_many_long_rows(shape, gate, kind, dtype):
+    """Several rows to a workgroup, whose column sums stand in LDS."""
+    check(make(shape, dtype, kind, gate, 15), kind, gate, 0.8, dtype)
+
+
 @pytest.mark.parametrize('kind', ['rms', 'layer'])
 def test_norm_alone(kind):
     t = make((4, 6, 5, 64), 'bf16', kind, 'none', 6)
