@@ -37,16 +37,30 @@ __device__ __forceinline__ const void* same_in_all_lanes(const void* p) {
 }
 
 // 16 (or 4) bytes of every lane, from base + its offset, straight into LDS, one lane behind the other from the wave's address `to`.  As assembly, because the compiler lets a
-// transposed read wait for every such load in flight, though it goes to another tile.  Nothing but fetched() waits for these.
+// transposed read wait for every such load in flight, though it goes to another tile.  Nothing but fetched() waits for these.  Nor does the compiler keep the distances inside
+// assembly that the chip asks for: five wait states from a vector instruction that writes a scalar register (the base comes from readfirstlane) to the instruction on memory that
+// reads it, one from a write of m0.  The five stand in front of every load (tests/test_token_isa.py looks them over in the built code).
 __device__ __forceinline__ void fetch16(const void* base, unsigned off, unsigned to) {
   base = same_in_all_lanes(base);
   to = __builtin_amdgcn_readfirstlane(to);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "m0", "memory");
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(to), "v"(off), "s"(base) : "memory");
+}
+// Four of them, to addresses `step` apart, behind one wait
+template <int step>
+__device__ __forceinline__ void fetch16x4(const void* base, const unsigned (&off)[4], unsigned to) {
+  base = same_in_all_lanes(base);
+  to = __builtin_amdgcn_readfirstlane(to);
+  asm volatile(
+      "s_nop 4\n\tglobal_load_lds_dwordx4 %2, %6\n\ts_add_u32 m0, m0, %7\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %6\n\ts_add_u32 m0, m0, %7\n\ts_nop 0\n\t"
+      "global_load_lds_dwordx4 %4, %6\n\ts_add_u32 m0, m0, %7\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %6"
+      : "={m0}"(to)
+      : "0"(to), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "i"(step)
+      : "memory", "scc");
 }
 __device__ __forceinline__ void fetch4(const void* base, unsigned off, unsigned to) {
   base = same_in_all_lanes(base);
   to = __builtin_amdgcn_readfirstlane(to);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(off), "s"(base) : "m0", "memory");
+  asm volatile("s_nop 4\n\tglobal_load_lds_dword %1, %2" ::"{m0}"(to), "v"(off), "s"(base) : "memory");
 }
 // Everything that the workgroup's waves fetched so far is in LDS, and their reads so far are done
 __device__ __forceinline__ void fetched() {
@@ -135,10 +149,18 @@ struct Tile {
     }
     // base: the tile's first row; rows from `rows` on repeat the last one, rows below `from` that one (they are masked)
     __device__ __forceinline__ void operator()(char* t, const T* base, int rows, int tid, int wave, int from = -0x7fffffff - 1) const {
+      unsigned off[kSteps];
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         const int r = row0 + i * kRowsPer, g = max(min(r, rows - 1), from);
-        fetch16(base, (g * sn + val(i)) * (int)sizeof(T), lds(t) + (i * NW + wave) * 1024);
+        off[i] = (g * sn + val(i)) * (int)sizeof(T);
+      }
+      if constexpr (kSteps % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < kSteps; i += 4) fetch16x4<NW * 1024>(base, *(const unsigned(*)[4])(off + i), lds(t) + (i * NW + wave) * 1024);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) fetch16(base, off[i], lds(t) + (i * NW + wave) * 1024);
       }
     }
   };
