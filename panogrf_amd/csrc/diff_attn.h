@@ -62,9 +62,11 @@ __device__ __forceinline__ void fetch4(const void* base, unsigned off, unsigned 
   to = __builtin_amdgcn_readfirstlane(to);
   asm volatile("s_nop 4\n\tglobal_load_lds_dword %1, %2" ::"{m0}"(to), "v"(off), "s"(base) : "memory");
 }
+// What the wave fetched so far is in LDS.  Every kernel ends behind one of these, whatever its loops skipped: a workgroup's LDS may not go to another with loads on their way.
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 // Everything that the workgroup's waves fetched so far is in LDS, and their reads so far are done
 __device__ __forceinline__ void fetched() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  landed();
   __syncthreads();
 }
 
@@ -568,6 +570,7 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
       }
     }
   }
+  landed();
 #pragma unroll
   for (int m = 0; m < MPW; ++m) l[m] += __shfl_xor(l[m], 32, 64);
   const bool live = r < rows;
@@ -969,6 +972,7 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
     }
     add(t1 - 1);
   }
+  landed();
   dlam += __shfl_xor(dlam, 32, 64);
   if (r >= rows) dlam = 0.f;
   if ((a.G & (a.G - 1)) == 0 && a.G <= 32) {                                   // one value for each head of the wave
@@ -1242,6 +1246,7 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D, DK>::kMinWaves)) void diff
       }
     }
   }
+  landed();                                                                    // (without a block to work on, the wave's own values may still be)
   if (key >= a.M) return;
   // (a key nobody sees has gradient 0; what its lanes hold came of values that may be anything, and stayed in their own columns)
   const long long oat = (((long long)b * a.M + key) * a.Hk + hk) * 2 * D + 4 * h;
@@ -1470,7 +1475,7 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_short(DiffArgs a) {
   } else {
     for (int i = tid; i < a.G; i += NW * 64) a.dlam_part[(long long)bh * a.G + i] = 0.f;
   }
-  fetched();                                                                   // (nothing is on its way to LDS when the workgroup ends)
+  landed();                                                                    // (without a block to work on, the keys may still be on their way)
   if (key >= a.M || !a.dk) return;
   const long long oat = (((long long)b * a.M + key) * a.Hk + hk) * 2 * D + 4 * h;
   auto put = [&](T* out, const f32x16& x, float f) {

@@ -1,6 +1,6 @@
 """What the compiler does not look after in the kernels' assembly, checked in the code that was built (no GPU): an instruction on memory that reads a scalar register
-written by a vector instruction needs five wait states in between, and a load straight into LDS one behind the write of m0.  The compiler keeps both for its own instructions,
-not for those of an assembly block."""
+written by a vector instruction needs five wait states in between, and a load straight into LDS one behind the write of m0; and such loads have to be waited for before the
+workgroup ends and its LDS goes to another.  The compiler keeps all that for its own instructions, not for those of an assembly block."""
 import os
 import re
 import struct
@@ -56,6 +56,40 @@ def too_close(lines):
     return bad
 
 
+def ends_with_loads(lines):
+    """-> [(function, end)] of ends of a program that a load straight into LDS (or a call, which may make some) reaches without a wait for all loads, on any path of branches."""
+    bad, functions = [], []
+    for line in lines:
+        head = re.match(r'([0-9a-f]+) <(.*)>:$', line)
+        if head:
+            functions.append((head.group(2), int(head.group(1), 16), []))
+        elif functions and '// ' in line and line.strip():
+            text, _, note = line.partition('//')
+            functions[-1][2].append((int(note.split(':')[0], 16), text.strip(), note))
+    for name, start, code in functions:
+        place = {at: i for i, (at, _, _) in enumerate(code)}
+        todo, seen = [(0, False)] if code else [], set()
+        while todo:
+            i, flying = todo.pop()
+            if (i, flying) in seen or i >= len(code):
+                continue
+            seen.add((i, flying))
+            text, note = code[i][1], code[i][2]
+            if text.startswith('s_endpgm'):
+                if flying:
+                    bad.append((name, hex(code[i][0])))
+                continue
+            if 'load_lds' in text or text.startswith('s_swappc'):
+                flying = True
+            elif text.startswith('s_waitcnt') and 'vmcnt(0)' in text:
+                flying = False
+            if text.startswith(('s_branch', 's_cbranch')):
+                todo.append((place[start + int(re.search(r'\+0x([0-9a-f]+)>', note).group(1), 16)], flying))
+            if not text.startswith(('s_branch', 's_setpc')):
+                todo.append((i + 1, flying))
+    return sorted(set(bad))
+
+
 def code_objects():
     data, mark, at = open(LIB, 'rb').read(), b'__CLANG_OFFLOAD_BUNDLE__', 0
     while (at := data.find(mark, at)) >= 0:
@@ -75,15 +109,20 @@ def test_the_check_itself():
     assert not too_close(['0 <f>:', '  v_readfirstlane_b32 s4, v1', '  s_nop 4', '  global_load_dword v2, v3, s[4:5]'])
     assert not too_close(['0 <f>:', '  v_readfirstlane_b32 s4, v1', '  s_add_u32 s4, s4, 1', '  global_load_dword v2, v3, s[4:5]'])
     assert too_close(['0 <f>:', '  s_mov_b32 m0, s8', '  global_load_lds_dwordx4 v2, s[4:5]'])
+    loads = ['0000 <f>:', ' global_load_lds_dword v2, s[4:5] // 000: 0', ' s_cbranch_scc1 1 // 008: 0 <f+0x10>', ' s_waitcnt vmcnt(0) // 00c: 0', ' s_endpgm // 010: 0']
+    assert ends_with_loads(loads) == [('f', '0x10')]
+    assert not ends_with_loads(loads[:2] + loads[3:]) and not ends_with_loads(loads[:1] + loads[2:])
 
 
 @pytest.mark.skipif(not os.path.exists(OBJDUMP), reason='no llvm-objdump')
 def test_waits_of_memory_instructions(tmp_path):
-    seen = 0
+    seen, flying = 0, []
     for i, code in enumerate(code_objects()):
         path = tmp_path / f'{i}.co'
         path.write_bytes(code)
         listing = subprocess.run([OBJDUMP, '-d', '--no-show-raw-insn', str(path)], check=True, capture_output=True, text=True).stdout.splitlines()
         seen += sum('global_load_lds' in line for line in listing)
         assert too_close(listing) == []
+        flying += ends_with_loads(listing)
     assert seen > 0
+    assert flying == []
