@@ -192,6 +192,8 @@ struct DiffArgs {
   const void* dout;               // [B,N,H,2D] contiguous
   float* delta;                   // [B,H,2,N]: dout . o_i
   float* dlam_part;               // [B*Hk][units][G]: parts of -dlam, by wave of the dq kernel (G a power of two up to 32) or by token, of every share
+  float* sizes;                   // f16: [B*Hk][size_parts][2], the largest |v_j|^2 and |dout_i|^2 of a part of the key head's keys and rows
+  int size_parts;
   void *dq, *dk, *dv, *dlam;
   // a workgroup's blocks cut into shares: partial gradients [shares][...] in float
   int q_shares, kv_shares;
@@ -743,6 +745,108 @@ __global__ __launch_bounds__(S > 1 ? 2 * D * S : 256) void diff_attn_join(DiffAr
 // Two waves or more share a SIMD and run beside each other, but for dq and dk at D = 128 in 16 bits, whose registers leave a SIMD one wave: those weave three blocks as the
 // forward kernel does.  Float does neither, as its products take eight times as long and hide the rest by themselves.  Both pipes are bound as in the forward kernel (2 x 8192,
 // 8 heads, bf16, D = 64: dq 920 us, 896 TFLOP/s; dk and dv 1244 us, 884 TFLOP/s).
+// In f16 the backward pass brings what it rounds into the type's range by powers of two that the float sums' last factor takes out again.  A score gradient a (G - delta) is a
+// probability, about 1 / M, times what is often a mean loss' gradient: rounded as it is, it is lost below 2^-25 where dq and dk are well in range (8192 keys, dout of 1e-4: dq
+// off by 7%), and is infinite above 65504.  |a (G - delta)| is at most 2 |dout_i| |v_j| and |a1 - lam a2| at most 1 + |lam|; with those at 2^14 what is 2^-28 of them still
+// has all its bits.  dq sums over a row, so its factor is the row's; dk and dv sum over the rows of a key head, so theirs is the key head's.  bf16 has float's range.
+template <typename T> constexpr bool kRanged = std::is_same<T, f16>::value;
+
+// The largest over aligned groups of W lanes, every lane gets it (as group_sum)
+template <int W>
+__device__ __forceinline__ float group_max(float v) {
+  auto moved = [](float x, auto ctrl) { return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), decltype(ctrl)::value, 0xf, 0xf, true)); };
+  v = fmaxf(v, moved(v, std::integral_constant<int, 0xB1>{}));
+  v = fmaxf(v, moved(v, std::integral_constant<int, 0x4E>{}));
+  v = fmaxf(v, moved(v, std::integral_constant<int, 0x141>{}));
+  v = fmaxf(v, moved(v, std::integral_constant<int, 0x140>{}));
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  return W == 64 ? with_other_half(v) : v;
+}
+__device__ __forceinline__ float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
+
+template <typename F>
+__device__ __forceinline__ float square(const F& x, float s = 0.f) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s = fmaf((float)x[j], (float)x[j], s);
+  return s;
+}
+
+// The power of two that brings values up to `bound` to at most 2^14 (what is not finite is left as it is)
+__device__ __forceinline__ int to_range(float bound) { return bound > 0.f && bound < INFINITY ? 13 - ilogbf(bound) : 0; }
+
+// For every key head, in parts of its keys and rows: the largest |v_j|^2 of keys that are seen, and |dout_i|^2 of rows that see any
+template <typename T, int D>
+__global__ __launch_bounds__(256) void diff_attn_sizes(DiffArgs a) {
+  using F = typename Frag8<T>::type;
+  constexpr int L = 2 * D / 8, kRows = 256 / L;                                // threads of a row, eight values each; rows at a time, four times
+  __shared__ float2 most[4];
+  const int bh = blockIdx.x / a.size_parts, part = blockIdx.x % a.size_parts, b = bh / a.Hk, hk = bh % a.Hk, tid = threadIdx.x, group = tid / L, e = tid % L * 8;
+  const int keys = (a.M + a.size_parts - 1) / a.size_parts, k0 = part * keys, k1 = min(k0 + keys, a.M);
+  const int all = a.N * a.G, rows = (all + a.size_parts - 1) / a.size_parts, r0 = part * rows, r1 = min(r0 + rows, all);
+  const unsigned char* mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+  const T* v = (const T*)a.v + b * a.v_sb + hk * a.v_sh + e;
+  float v2 = 0.f, g2 = 0.f;
+  for (int k = k0 + group; k < k1; k += 4 * kRows) {
+    F x[4];
+    bool in[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = min(k + j * kRows, k1 - 1);
+      x[j] = load8<T>(v + at * a.v_sn);
+      in[j] = !mask || mask[at];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float s = group_sum<L>(square(x[j]));
+      v2 = in[j] ? fmaxf(v2, s) : v2;
+    }
+  }
+  for (int r = r0 + group; r < r1; r += 4 * kRows) {
+    F x[4];
+    float lse[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = min(r + j * kRows, r1 - 1), n = at / a.G, head = hk * a.G + at % a.G;
+      x[j] = load8<T>((const T*)a.dout + (((long long)b * a.N + n) * a.H + head) * 2 * D + e);
+      lse[j] = a.lse[((long long)b * a.H + head) * 2 * a.N + n];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float s = group_sum<L>(square(x[j]));
+      g2 = lse[j] == INFINITY ? g2 : fmaxf(g2, s);
+    }
+  }
+  v2 = group_max<64>(v2);
+  g2 = group_max<64>(g2);
+  if ((tid & 63) == 0) most[tid >> 6] = make_float2(v2, g2);
+  __syncthreads();
+  if (tid == 0)
+    *(float2*)(a.sizes + 2ll * blockIdx.x) = make_float2(fmaxf(fmaxf(most[0].x, most[1].x), fmaxf(most[2].x, most[3].x)),
+                                                         fmaxf(fmaxf(most[0].y, most[1].y), fmaxf(most[2].y, most[3].y)));
+}
+
+// The largest |lam| of the heads that share a key head
+template <typename T>
+__device__ __forceinline__ float largest_lam(const DiffArgs& a, int hk, int lane) {
+  float lam = 0.f;
+  for (int u = lane; u < a.G; u += 64) lam = fmaxf(lam, fabsf(lam_of<T>(a, hk * a.G + u)));
+  return group_max<64>(lam);
+}
+
+// A key head's largest |v_j|^2, and the powers of two of its score gradients (the second map's with lam) and of a1 - lam a2
+struct Range { float v2; int grad, map; };
+template <typename T>
+__device__ __forceinline__ Range range_of(const DiffArgs& a, int bh, int hk, int lane) {
+  float2 e = make_float2(0.f, 0.f);
+  for (int i = lane; i < a.size_parts; i += 64) {
+    const float2 x = *(const float2*)(a.sizes + ((long long)bh * a.size_parts + i) * 2);
+    e = make_float2(fmaxf(e.x, x.x), fmaxf(e.y, x.y));
+  }
+  const float lam = largest_lam<T>(a, hk, lane), v2 = group_max<64>(e.x), g2 = group_max<64>(e.y);
+  return {uniform(v2), __builtin_amdgcn_readfirstlane(to_range(2.f * sqrtf(v2 * g2) * fmaxf(lam, 1.f))), __builtin_amdgcn_readfirstlane(to_range(1.f + lam))};
+}
+
 template <typename T, int D, bool MORE = true> struct BwdShape {               // MORE: dq or dk is formed
   static constexpr bool kWeave = sizeof(T) == 2 && D == 128 && MORE;
   static constexpr int kMinWaves = sizeof(T) == 2 && !kWeave ? 2 : 1;
@@ -910,10 +1014,23 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
 #pragma unroll
         for (int i = 0; i < 16; ++i) delta[m] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[m][i], a.c, -lse[m])), g[i], delta[m]);
     });
+  int ranged = 0;                                                              // the power of two of the row's score gradients
+  float kept[2] = {1.f, 1.f};                                                  // delta is kept times what the key head's are brought into range by
+  if constexpr (kRanged<T>) {
+    const Range range = range_of<T>(a, bh, hk, lane);
+    kept[0] = ldexpf(1.f, range.grad);
+    kept[1] = ldexpf(1.f, range.grad - range.map);
+    float g2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) g2 = square(gf[i], g2);
+    g2 += __shfl_xor(g2, 32, 64);
+    ranged = to_range(2.f * sqrtf(range.v2 * g2));
+  }
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     delta[m] += __shfl_xor(delta[m], 32, 64);
-    if (h == 0 && r < rows && share == 0) a.delta[st + m * a.N] = delta[m];
+    if (h == 0 && r < rows && share == 0) a.delta[st + m * a.N] = delta[m] * kept[m];
+    if constexpr (kRanged<T>) lse[m] -= (float)ranged;                         // (probabilities, and with them all that follows, times this power of two)
   }
   if constexpr (!kWeave) {
     sweep(t0, t1, [&](int t) {
@@ -973,6 +1090,8 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
     add(t1 - 1);
   }
   landed();
+  const float undo = ldexpf(1.f, -ranged);
+  if constexpr (kRanged<T>) dlam *= undo;
   dlam += __shfl_xor(dlam, 32, 64);
   if (r >= rows) dlam = 0.f;
   if ((a.G & (a.G - 1)) == 0 && a.G <= 32) {                                   // one value for each head of the wave
@@ -984,7 +1103,11 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D>::kMinWaves)) void diff_att
   if (r < rows && a.dq) {
     T* out = (T*)a.dq + oat * 2 * D + 4 * h;
     float* part = a.dq_part + ((long long)share * a.B * a.N * a.H + oat) * 2 * D + 4 * h;
-    const float f[2] = {a.scale, -lam_of<T>(a, head) * a.scale};
+    float f[2] = {a.scale, -lam_of<T>(a, head) * a.scale};
+    if constexpr (kRanged<T>) {
+      f[0] *= undo;
+      f[1] *= undo;
+    }
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -1066,6 +1189,13 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D, DK>::kMinWaves)) void diff
     }
     blind = !any ? a.N : a.causal ? max(0, blind - off) : 0;
   }
+  // f16: what brings the maps' difference (with lam), and each map's score gradients, into range (delta comes times x0 and x1)
+  Range range = {0.f, 0, 0};
+  if constexpr (kRanged<T>) range = range_of<T>(a, bh, hk, lane);
+  const float pk = uniform(ldexpf(1.f, range.map)), x0 = uniform(ldexpf(1.f, range.grad)), x1 = uniform(ldexpf(1.f, range.grad - range.map));
+  auto lam_ranged = [&](int head) { return kRanged<T> ? lam_of<T>(a, head) * pk : lam_of<T>(a, head); };
+  auto apart = [&](float p0, float p1) { return kRanged<T> ? fmaf(p0, pk, -p1) : p0 - p1; };
+  auto above = [&](float g_, float d, float x) { return kRanged<T> ? fmaf(g_, x, -d) : g_ - d; };
   // the blocks: queries that see the workgroup's first key, of each head that shares it
   const int first = max(blind, a.causal ? tile * NW * 32 - off : 0) / QT, nq = blind < a.N ? max((a.N + QT - 1) / QT - first, 0) : 0;
   const int all = nq * a.G, per = (all + a.kv_shares - 1) / a.kv_shares, from = min(share * per, all), total = min(all, from + per) - from;
@@ -1122,16 +1252,16 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D, DK>::kMinWaves)) void diff
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       typedef float f4 __attribute__((ext_vector_type(4)));
-      const int x0 = 8 * u + 4 * h;
-      const f4 e0 = *(const f4*)&e[0][x0], e1 = *(const f4*)&e[1][x0], d0 = *(const f4*)&e[2][x0], d1 = *(const f4*)&e[3][x0];
+      const int at_ = 8 * u + 4 * h;
+      const f4 e0 = *(const f4*)&e[0][at_], e1 = *(const f4*)&e[1][at_], d0 = *(const f4*)&e[2][at_], d1 = *(const f4*)&e[3][at_];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int x = 4 * u + j;
         const float p0 = __builtin_amdgcn_exp2f(fmaf(s[0][x], a.c, -e0[j])), p1 = __builtin_amdgcn_exp2f(fmaf(s[1][x], a.c, -e1[j])) * lam;
-        p[x] = p0 - p1;
+        p[x] = apart(p0, p1);
         if constexpr (DK) {
-          s[0][x] = p0 * (g[x] - d0[j]);
-          s[1][x] = p1 * (g[x] - d1[j]);
+          s[0][x] = p0 * above(g[x], d0[j], x0);
+          s[1][x] = p1 * above(g[x], d1[j], x1);
         }
       }
     }
@@ -1167,10 +1297,10 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D, DK>::kMinWaves)) void diff
     fetched();
     if (total > 1) fetch(1);
     int head = hk * a.G + from_g, n0 = (first + from_n) * QT;
-    float lam = lam_of<T>(a, head);
+    float lam = lam_ranged(head);
     auto step = [&]() {
       n0 += QT;
-      if (n0 >= a.N && head + 1 < (hk + 1) * a.G) { n0 = first * QT; lam = lam_of<T>(a, ++head); }
+      if (n0 >= a.N && head + 1 < (hk + 1) * a.G) { n0 = first * QT; lam = lam_ranged(++head); }
     };
     if constexpr (kWeave) {
       form(s, g, 0);
@@ -1210,10 +1340,10 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D, DK>::kMinWaves)) void diff
 #pragma unroll
                   for (int y = 0; y < (DK ? 4 : 2); ++y) st[y] = *(const f4*)&e[y][2 * x + 4 * h];
                 const float p0 = __builtin_amdgcn_exp2f(fmaf(s[0][x], a.c, -st[0][x % 4])), p1 = __builtin_amdgcn_exp2f(fmaf(s[1][x], a.c, -st[1][x % 4])) * lam_t;
-                if constexpr (DV) pn[x / 8][x % 8] = (T)(p0 - p1);
+                if constexpr (DV) pn[x / 8][x % 8] = (T)apart(p0, p1);
                 if constexpr (DK) {
-                  dn[0][x / 8][x % 8] = (T)(p0 * (g[x] - st[2][x % 4]));
-                  dn[1][x / 8][x % 8] = (T)(p1 * (g[x] - st[3][x % 4]));
+                  dn[0][x / 8][x % 8] = (T)(p0 * above(g[x], st[2][x % 4], x0));
+                  dn[1][x / 8][x % 8] = (T)(p1 * above(g[x], st[3][x % 4], x1));
                 }
               }
             });
@@ -1261,12 +1391,12 @@ __global__ __launch_bounds__(NW * 64, (BwdShape<T, D, DK>::kMinWaves)) void diff
   };
   if constexpr (DV)
 #pragma unroll
-    for (int c = 0; c < ND; ++c) put(a.dv, a.dv_part, 32 * c, dv[c], 1.f);
+    for (int c = 0; c < ND; ++c) put(a.dv, a.dv_part, 32 * c, dv[c], ldexpf(1.f, -range.map));
   if constexpr (DK)
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int c = 0; c < NC; ++c) put(a.dk, a.dk_part, m * D + 32 * c, dk[m][c], m ? -a.scale : a.scale);
+      for (int c = 0; c < NC; ++c) put(a.dk, a.dk_part, m * D + 32 * c, dk[m][c], ldexpf(m ? -a.scale : a.scale, -range.grad));
 }
 
 // Sums over the 32 lanes of a half: lane l gets that of value l & 15 of a (l & 16: of b).  In every step a lane keeps one half of the values it has and gives the other
@@ -1364,12 +1494,28 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_short(DiffArgs a) {
     if (wave == 0)
       fetch4(a.lse + ((long long)b * a.H + head) * 2 * a.N + n0, ((unsigned)h * a.N + min(lane & 31, a.N - 1 - n0)) * 4u, lds_address(&stat[t % R][0][0]));
   };
+  // f16: one power of two for all score gradients of the key head.  It is that of the first block's largest |dout_i|; where a block's is more
+  // than twice as large, what was added up follows
+  float v2 = 0.f, pk = 1.f, most_lam = 1.f;
+  int map = 0, grad = 200;                                                     // (200: none yet)
+  __shared__ float most[NW];
+  if constexpr (kRanged<T>) {
+    const float lam = largest_lam<T>(a, hk, lane);
+    map = __builtin_amdgcn_readfirstlane(to_range(1.f + lam));
+    pk = uniform(ldexpf(1.f, map));
+    most_lam = fmaxf(lam, 1.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v2 = square(vf[i], v2);
+    v2 = group_max<32>(v2 + __shfl_xor(v2, 32, 64));
+    if (lane == 0) most[wave] = v2;
+  }
   if (total > 0) {
     fetch(0);
     int head = hk * a.G, n0 = first * QT;
     float lam = lam_of<T>(a, head);
     for (int t = 0; t < total; ++t) {
       fetched();                                                               // block t has come
+      if (kRanged<T> && t == 0 && NW > 1) v2 = fmaxf(most[0], most[NW - 1]);
       if (t == 0 && seen64 != (NW == 2 ? ~0ull : 0xffffffffull)) {
         TL::template clear<NW * 32, NW * 64>(ktile, seen64, tid);
         __syncthreads();
@@ -1380,7 +1526,30 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_short(DiffArgs a) {
       struct Two { F q, k; };
       weave<Two, 2 * NK, 1>([&](int i) { return Two{TL::row(qb, at, (i & 1) * NK + i / 2), TL::row(ktile + wave * kTile, at, (i & 1) * NK + i / 2)}; },
                             [&](int i, const Two& f) { s[i & 1] = mma(f.q, f.k, s[i & 1]); }, [](int) {});
-      weave<F, NV, 2>([&](int i) { return TL::row(gb, at, i); }, [&](int i, const F& f) { g = mma(f, vf[i], g); }, [](int) {});
+      float g2 = 0.f;
+      weave<F, NV, 2>([&](int i) { return TL::row(gb, at, i); },
+                      [&](int i, const F& f) {
+                        g = mma(f, vf[i], g);
+                        if constexpr (kRanged<T>) g2 = square(f, g2);
+                      },
+                      [](int) {});
+      float x0 = 1.f;
+      if constexpr (kRanged<T>) {
+        g2 = group_max<32>(g2 + __shfl_xor(g2, 32, 64));
+        const int now = __builtin_amdgcn_readfirstlane(to_range(2.f * sqrtf(v2 * g2) * most_lam));
+        if (now < grad - 1 && g2 > 0.f && g2 < INFINITY) {
+          if (grad < 200) {
+            const float down = ldexpf(1.f, now - grad);
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+              for (int c = 0; c < NC; ++c) dk[m][c] *= down;
+            dlam *= down;
+          }
+          grad = now;
+        }
+        x0 = uniform(ldexpf(1.f, grad < 200 ? grad : 0));
+      }
       if (n0 + QT > a.N || seen32 != ~0u || (a.causal && k0 + 31 > n0 + off)) {
         const unsigned ok = seen ? rows_of_lane(a.causal ? key - off - n0 : 0, a.N - 1 - n0, h) : 0u;
 #pragma unroll
@@ -1400,10 +1569,11 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_short(DiffArgs a) {
             const int x = 4 * u + j;
             s[0][x] = __builtin_amdgcn_exp2f(fmaf(s[0][x], a.c, -e0[j]));
             s[1][x] = __builtin_amdgcn_exp2f(fmaf(s[1][x], a.c, -e1[j]));
-            p[x] = fmaf(-lam, s[1][x], s[0][x]);
+            p[x] = kRanged<T> ? fmaf(-lam * pk, s[1][x], s[0][x] * pk) : fmaf(-lam, s[1][x], s[0][x]);
           }
         }
-        sums[wave][(lane >> 4) & 1][row_of(lane & 15, h)] = sums_of_half(s[0] * g, s[1] * g, lane);
+        const float part = sums_of_half(s[0] * g, s[1] * g, lane);
+        sums[wave][(lane >> 4) & 1][row_of(lane & 15, h)] = kRanged<T> ? part * x0 : part;
         pc[0] = pack<T>(p, 0);
         pc[1] = pack<T>(p, 1);
       }
@@ -1422,8 +1592,13 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_short(DiffArgs a) {
         for (int j = 0; j < 4; ++j) {
           const int x = 4 * u + j;
           if (n0 + 8 * u + 4 * h + j < a.N) dlam += d1[j];
-          s[0][x] *= g[x] - d0[j];
-          s[1][x] *= lam * (g[x] - d1[j]);                                     // (without the sign)
+          if constexpr (kRanged<T>) {
+            s[0][x] *= fmaf(g[x], x0, -d0[j]);
+            s[1][x] *= lam * fmaf(g[x], x0, -d1[j]);
+          } else {
+            s[0][x] *= g[x] - d0[j];
+            s[1][x] *= lam * (g[x] - d1[j]);                                   // (without the sign)
+          }
         }
       }
 #pragma unroll
@@ -1454,7 +1629,7 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_short(DiffArgs a) {
             for (int c = 0; c < NC; ++c) dq[c] = mma(TL::col(ktile, at, i, m * NC + c), w, dq[c]);
           }
           const int n = n0 + (lane & 31);
-          const float f = m ? -a.scale : a.scale;
+          const float f = kRanged<T> ? ldexpf(m ? -a.scale : a.scale, grad < 200 ? -grad : 0) : m ? -a.scale : a.scale;
           if (n < a.N) {
             T* out = (T*)a.dq + (((long long)b * a.N + n) * a.H + head) * 2 * D + m * D + 4 * h;
 #pragma unroll
@@ -1466,7 +1641,7 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_short(DiffArgs a) {
       n0 += QT;
       if (n0 >= a.N) {                                                         // the head's last block
         dlam += __shfl_xor(dlam, 32, 64);
-        if (tid == 0) a.dlam_part[(long long)bh * a.G + head - hk * a.G] = dlam;
+        if (tid == 0) a.dlam_part[(long long)bh * a.G + head - hk * a.G] = kRanged<T> ? ldexpf(dlam, grad < 200 ? -grad : 0) : dlam;
         dlam = 0.f;
         n0 = first * QT;
         if (t + 1 < total) lam = lam_of<T>(a, ++head);
@@ -1484,11 +1659,11 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_attn_short(DiffArgs a) {
       store4<T>(out + 8 * u, seen ? x[4 * u] * f : 0.f, seen ? x[4 * u + 1] * f : 0.f, seen ? x[4 * u + 2] * f : 0.f, seen ? x[4 * u + 3] * f : 0.f);
   };
 #pragma unroll
-  for (int c = 0; c < ND; ++c) put((T*)a.dv + oat + 32 * c, dv[c], 1.f);
+  for (int c = 0; c < ND; ++c) put((T*)a.dv + oat + 32 * c, dv[c], ldexpf(1.f, -map));
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int c = 0; c < NC; ++c) put((T*)a.dk + oat + m * D + 32 * c, dk[m][c], m ? -a.scale : a.scale);
+    for (int c = 0; c < NC; ++c) put((T*)a.dk + oat + m * D + 32 * c, dk[m][c], ldexpf(m ? -a.scale : a.scale, grad < 200 ? -grad : 0));
 }
 
 // Adds the shares of a gradient, in order; n a multiple of 4

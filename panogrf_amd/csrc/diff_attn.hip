@@ -64,6 +64,13 @@ static BwdCut cut_bwd(int dtype, int B, int N, int M, int H, int Hk, int D, bool
   return c;
 }
 
+// Workgroups that look for a key head's largest values (f16)
+static int size_parts(int dtype, int N, int M, int G) {
+  if (dtype != PGRF_DTYPE_F16) return 0;
+  const long long most = (long long)N * G > M ? (long long)N * G : M;
+  return most > 256 * 64 ? 256 : (int)((most + 63) / 64);
+}
+
 static int check(const PgrfDiffAttn* p, const char* who, bool backward) {
   if (!p) return set_error(PGRF_ERR_ARG, "%s: null arguments", who);
   if (!dtype_ok(p->dtype)) return set_error(PGRF_ERR_UNSUPPORTED, "%s: dtype %d (PGRF_DTYPE_F32 | BF16 | F16)", who, p->dtype);
@@ -152,6 +159,7 @@ size_t pgrf_diff_attention_backward_workspace_bytes(int dtype, int B, int N, int
   const BwdCut c = cut_bwd(dtype, B, N, M, H, Hk, D, causal != 0);
   size_t n = (size_t)B * H * 2 * N + ((size_t)B * Hk * c.units * (H / Hk) + 3) / 4 * 4;
   n = (n + 3) / 4 * 4;
+  if (c.row_waves) n += ((size_t)B * Hk * size_parts(dtype, N, M, H / Hk) * 2 + 3) / 4 * 4;
   if (c.q_shares > 1) n += (size_t)c.q_shares * B * N * H * 2 * D;
   if (c.kv_shares > 1) n += (size_t)c.kv_shares * B * M * Hk * 4 * D;
   return n * sizeof(float);
@@ -175,6 +183,11 @@ int pgrf_diff_attention_backward(const PgrfDiffAttn* p, const void* dout, void* 
   const size_t sums = (size_t)a.B * a.H * 2 * a.N;
   a.dlam_part = a.delta + sums;
   float* behind = a.delta + (sums + ((size_t)a.B * a.Hk * c.units * a.G + 3) / 4 * 4 + 3) / 4 * 4;
+  if (c.row_waves) {
+    a.size_parts = size_parts(p->dtype, a.N, a.M, a.G);
+    a.sizes = behind;
+    behind += ((size_t)a.B * a.Hk * a.size_parts * 2 + 3) / 4 * 4;
+  }
   if (c.q_shares > 1) { a.dq_part = behind; behind += (size_t)c.q_shares * a.B * a.N * a.H * 2 * p->D; }
   if (c.kv_shares > 1) { a.dk_part = behind; a.dv_part = behind + (size_t)c.kv_shares * a.B * a.M * a.Hk * 2 * p->D; }
   const long long rg = c.row_groups * c.q_shares, kg = c.key_groups * c.kv_shares;

@@ -65,6 +65,10 @@ int PGRF_DA_NAME(launch_da_bwd)(const DiffArgs& a, int row_waves, unsigned row_g
     return PGRF_OK;
   }
 #endif
+#if PGRF_DA_TYPE == 2
+  hipLaunchKernelGGL((diff_attn_sizes<DaT, PGRF_DA_D>), dim3((unsigned)(a.B * a.Hk * a.size_parts)), dim3(256), 0, s, a);
+  PGRF_TOK_LAUNCHED(who);
+#endif
   if (row_waves == 1) hipLaunchKernelGGL((diff_attn_dq<DaT, PGRF_DA_D, 1>), dim3(row_grid), dim3(64), 0, s, a);
   else if (row_waves == 2) hipLaunchKernelGGL((diff_attn_dq<DaT, PGRF_DA_D, 2>), dim3(row_grid), dim3(128), 0, s, a);
   else hipLaunchKernelGGL((diff_attn_dq<DaT, PGRF_DA_D, 4>), dim3(row_grid), dim3(256), 0, s, a);
