@@ -5,6 +5,7 @@ and the device is switched only where the tensors are on another one."""
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import PgrfError, lib
 
@@ -56,6 +57,15 @@ def alike(who, name, t, dtype, device):
         refuse(who, f'{name} is {t.dtype}, expected {dtype}')
 
 
+def no_tangents(who, *tensors):
+    """No tensor carries a tangent of forward-mode differentiation, which the outputs would lose.  (_current_level: -1 outside of it, as nearly always; asking each
+    tensor costs more than all other checks.)"""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                refuse(who, 'no forward-mode derivatives (dual tensors, torch.func.jvp): use backward')
+
+
 def launch(device, name, *args):
     """Calls an entry point with `args` and the current stream of the tensors' device, whatever the current device is."""
     index = device.index
@@ -73,6 +83,7 @@ def first_derivatives_only(backward):
     guarded = torch.autograd.function.once_differentiable(backward)
 
     def call(ctx, *grads):
+        no_tangents('backward', *grads)
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return call
 

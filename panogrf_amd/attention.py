@@ -8,7 +8,7 @@ from functools import lru_cache
 
 import torch
 
-from ._token import DIFF_ATTN, DTYPES, alike, entry, first_derivatives_only, launch, on_gpu, ptr, refuse, require
+from ._token import DIFF_ATTN, DTYPES, alike, entry, first_derivatives_only, launch, no_tangents, on_gpu, ptr, refuse, require
 
 
 def _aligned(t):
@@ -122,13 +122,14 @@ def diff_attention(q, k, v, lam, *, causal=False, key_mask=None, scale=None):
     that do not start at multiples of 16 bytes are copied first).  key_mask [B, M] bool, False: no query sees the key, and what it holds does not matter.
     causal: query i sees keys up to i + M - N, so the last query stands at the last key.  A query that sees no key gives 0 and
     has no part in any gradient, whatever it and its gradient hold.  scale: 1/sqrt(d) unless given.
-    Softmax and sums are float; probabilities and score gradients are rounded to the tensors' type for the products behind them.  Gradients (first derivatives) to
+    Softmax and sums are float; probabilities and score gradients are rounded to the tensors' type for the products behind them.  Gradients (first derivatives, by backward) to
     q, k, v and lam; they do not depend on scheduling."""
     who = 'diff_attention'
     scale = _check(who, q, k, v, lam, scale)
     if key_mask is not None:
         require(torch.is_tensor(key_mask) and key_mask.dtype == torch.bool and key_mask.device == q.device and tuple(key_mask.shape) == tuple(k.shape[:2]), who,
                 f'key_mask must be a bool tensor {list(k.shape[:2])} on {q.device}')
+    no_tangents(who, q, k, v, lam)
     on_gpu(q, who)
     if key_mask is not None:
         key_mask = key_mask if key_mask.stride(-1) == 1 else key_mask.contiguous()
@@ -150,5 +151,6 @@ def diff_attention_cached(q, k_cache, v_cache, lam, lengths, *, scale=None):
         refuse(who, f'lengths must be an int32 tensor [{q.shape[0]}] on {q.device}')
     if (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or lam.requires_grad) and torch.is_grad_enabled():
         refuse(who, 'no gradients over a cache: call it under torch.no_grad(), or diff_attention with a key_mask')
+    no_tangents(who, q, k_cache, v_cache, lam)
     on_gpu(q, who)
     return _forward(_aligned(q), _aligned(k_cache), _aligned(v_cache), lam.contiguous(), None, lengths.contiguous(), True, scale, False)[0]

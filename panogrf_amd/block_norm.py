@@ -8,7 +8,7 @@ in one pass over x and y.  `kind='rms'`: N(a) = a / sqrt(mean(a^2) + eps) * w; `
 form of the aggregation net's ray attention: nn.LayerNorm(16, eps=1e-6), network/ibrnet.py:160-204)."""
 import torch
 
-from ._token import BLOCK_NORM, DTYPES, alike, entry, first_derivatives_only, launch, on_gpu, ptr, refuse, require
+from ._token import BLOCK_NORM, DTYPES, alike, entry, first_derivatives_only, launch, no_tangents, on_gpu, ptr, refuse, require
 
 _LAYER, _POST, _PRE = 1, 2, 4
 _NAMES = ('x', 'y', 'gate', 'post_weight', 'post_bias', 'pre_weight', 'pre_bias')
@@ -74,7 +74,8 @@ def block_norm(x, y=None, gate=None, post_weight=None, post_bias=None, pre_weigh
     block, or of any tensor's last axis).  gate: None (1), [C] (a layer scale), the shape of x, or x's leading axes up to some axis and then C, e.g.
     [B, C] for x [B, N, C] (one gate per sample).  Weights and biases [C] or None (1 and 0); biases with kind='layer' only.  post=False leaves out
     the norm of y, pre=False the norm of x' (z is None then).  Statistics and sums are float; x' is rounded once to its type and z formed from its
-    unrounded value.  All of x, y, gate, weights and biases have gradients (first derivatives; their sums do not depend on scheduling)."""
+    unrounded value.  All of x, y, gate, weights and biases have gradients (first derivatives, by backward;
+    their sums do not depend on scheduling)."""
     who = 'block_norm'
     require(isinstance(x, torch.Tensor) and x.dim() >= 1, who, 'x must be a tensor with a channel axis')
     dtype, device, shape = x.dtype, x.device, x.shape
@@ -118,6 +119,7 @@ def block_norm(x, y=None, gate=None, post_weight=None, post_bias=None, pre_weigh
         gates = gate.numel() // C
         rpg = max(rows // max(gates, 1), 1)
         require(rpg == 1 or gates <= 60000, who, 'over 60000 gate rows that are shared by several rows each')
+    no_tangents(who, *ts)
     on_gpu(x, who)
     flags = (_LAYER if layer else 0) | (_POST if post else 0) | (_PRE if pre else 0)
     if grad and torch.is_grad_enabled():

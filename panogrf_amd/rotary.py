@@ -2,7 +2,7 @@
 difference of their positions.  Positions may be whole (tokens) or continuous (the depths of a ray's samples)."""
 import torch
 
-from ._token import DTYPES, ROTARY, alike, first_derivatives_only, launch, on_gpu, refuse, require
+from ._token import DTYPES, ROTARY, alike, first_derivatives_only, launch, no_tangents, on_gpu, refuse, require
 
 _SCALINGS = {None: 0, 'linear': 1, 'ntk': 2, 'parts': 3}             # PGRF_ROTARY_* of include/panogrf_hip.h
 _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
@@ -70,7 +70,8 @@ def rotary(q, k, positions, *, rotary_dim=None, layout='half', base=10000.0, sca
       'ntk'     with base * factor^(rotary_dim/(rotary_dim-2))
       'parts'   f_i (t + (1-t)/factor), t = clamp((trained_length f_i/2pi - low)/(high - low), 0, 1): pairs of over `high` turns in the trained
                 context stay, those of under `low` are stretched
-    and `magnitude` multiplies every turned pair.  float32, bfloat16 or float16; gradients to q and k (positions have none)."""
+    and `magnitude` multiplies every turned pair.  float32, bfloat16 or float16; gradients to q and k by backward (positions
+    have none)."""
     who = 'rotary'
     require(isinstance(q, torch.Tensor) and q.dim() >= 3, who, 'q must be [B, N, ..., D]')
     dtype, device, shape = q.dtype, q.device, q.shape
@@ -96,6 +97,7 @@ def rotary(q, k, positions, *, rotary_dim=None, layout='half', base=10000.0, sca
     require(q.numel() > 0 or B * N == 0, who, 'q has no heads')
     if positions.requires_grad and torch.is_grad_enabled():
         refuse(who, 'positions have no gradient: detach them')
+    no_tangents(who, q, k, positions)
     on_gpu(q, who)
     call = (rot, int(layout == 'interleaved'), float(base), _SCALINGS[scaling], float(factor), float(trained_length), float(low), float(high),
             float(magnitude))
