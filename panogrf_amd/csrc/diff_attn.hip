@@ -88,9 +88,9 @@ static int check(const PgrfDiffAttn* p, const char* who, bool backward) {
   if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) ||
       (p->q_sb | p->q_sn | p->q_sh | p->q_sm | p->k_sb | p->k_sn | p->k_sh | p->k_sm | p->v_sb | p->v_sn | p->v_sh) % per)
     return set_error(PGRF_ERR_ARG, "%s: q, k, v: addresses and strides must be multiples of 16 bytes", who);
-  // (what a tile's lanes add to its base has to fit 32 bits)
-  if (p->q_sn > (1 << 22) || p->q_sm > (1 << 22) || p->k_sn > (1 << 22) || p->k_sm > (1 << 22) || p->v_sn > (1 << 22) || p->q_sn < 0 || p->q_sm < 0 || p->k_sn < 0 || p->k_sm < 0 ||
-      p->v_sn < 0 || (long long)p->H * 2 * p->D > (1 << 22))
+  // (what a tile's lanes add to its base has to fit 32 bits; nothing is added for an axis of one token)
+  auto far = [](long long stride) { return stride < 0 || stride > (1 << 22); };
+  if ((p->N > 1 && far(p->q_sn)) || far(p->q_sm) || (p->M > 1 && (far(p->k_sn) || far(p->v_sn))) || far(p->k_sm) || (long long)p->H * 2 * p->D > (1 << 22))
     return set_error(PGRF_ERR_UNSUPPORTED, "%s: a stride between tokens or maps is negative or over 2^22 values", who);
   if (backward && !p->lse) return set_error(PGRF_ERR_ARG, "%s: null lse", who);
   if (backward && p->lengths) return set_error(PGRF_ERR_UNSUPPORTED, "%s: lengths have no backward pass (use key_mask)", who);
