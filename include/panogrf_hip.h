@@ -488,8 +488,8 @@ typedef struct PgrfBlockNorm {
   void *x_out, *z_out;
   float* stats;                /* 16-byte aligned */
   /* backward: gradients for upstream dx_out, dz [rows, C] (NULL = zero); x, y, the gate and the weights are the forward's, stats what it wrote.  Any of
-   * dx .. dpre_b may be NULL; those asked for are written, not accumulated (a bias' only with PGRF_NORM_LAYER).  A weight's or a shared gate's gradient
-   * needs `workspace`, 16-byte aligned scratch of the size the function below names. */
+   * dx .. dpre_b may be NULL; those asked for are written, not accumulated (a bias' only with PGRF_NORM_LAYER).  dgate of a gate whose rows are
+   * shared (rows_per_gate > 1) takes up to 60000 of them.  A weight's or a shared gate's gradient needs `workspace`, 16-byte aligned scratch of the size the function below names. */
   const void *dx_out, *dz;
   void *dx, *dy, *dgate, *dpost_w, *dpost_b, *dpre_w, *dpre_b;
   void* workspace;

@@ -58,11 +58,13 @@ class _BlockNorm(torch.autograd.Function):
             dx_out = dx_out.contiguous()
         if dz is not None and not dz.is_contiguous():
             dz = dz.contiguous()
-        n = entry('pgrf_block_norm_backward_workspace_bytes')(rows, C, rpg)
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+        n, ws = 0, None                             # scratch for sums over rows: of the weights, the biases and a shared gate
+        if any(needs[3:7]) or (needs[2] and rpg > 1):
+            n = entry('pgrf_block_norm_backward_workspace_bytes')(rows, C, rpg)
+            ws = torch.empty(n, dtype=torch.uint8, device=x.device)
         launch(x.device, 'pgrf_block_norm_backward',
                BLOCK_NORM.pack(x.data_ptr(), ptr(y), ptr(gate), ptr(pw), ptr(pb), ptr(qw), ptr(qb), 0, 0, stats.data_ptr(), ptr(dx_out), ptr(dz), ptr(dx), ptr(dy),
-                               ptr(dgate), ptr(dpw), ptr(dpb), ptr(dqw), ptr(dqb), ws.data_ptr(), n, rows, rpg, DTYPES[x.dtype], C, flags, scale, 0.0))
+                               ptr(dgate), ptr(dpw), ptr(dpb), ptr(dqw), ptr(dqb), ptr(ws), n, rows, rpg, DTYPES[x.dtype], C, flags, scale, 0.0))
         return dx, dy, dgate, dpw, dpb, dqw, dqb, None, None, None, None
 
 
@@ -72,7 +74,7 @@ def block_norm(x, y=None, gate=None, post_weight=None, post_bias=None, pre_weigh
 
     x [..., C] (C up to 8 192) float32, bfloat16 or float16, y the same shape or None (then x' is x and only z is formed: the norm before the first
     block, or of any tensor's last axis).  gate: None (1), [C] (a layer scale), the shape of x, or x's leading axes up to some axis and then C, e.g.
-    [B, C] for x [B, N, C] (one gate per sample).  Weights and biases [C] or None (1 and 0); biases with kind='layer' only.  post=False leaves out
+    [B, C] for x [B, N, C] (one gate per sample; over 60 000 shared ones have no gradient).  All of x's type.  Weights and biases [C] or None (1 and 0); biases with kind='layer' only.  post=False leaves out
     the norm of y, pre=False the norm of x' (z is None then).  Statistics and sums are float; x' is rounded once to its type and z formed from its
     unrounded value.  All of x, y, gate, weights and biases have gradients (first derivatives, by backward;
     their sums do not depend on scheduling)."""
@@ -118,7 +120,8 @@ def block_norm(x, y=None, gate=None, post_weight=None, post_bias=None, pre_weigh
                 f'gate {tuple(gate.shape)} must be [C], the leading axes of x {tuple(shape)} and C, or the shape of x')
         gates = gate.numel() // C
         rpg = max(rows // max(gates, 1), 1)
-        require(rpg == 1 or gates <= 60000, who, 'over 60000 gate rows that are shared by several rows each')
+        require(rpg == 1 or gates <= 60000 or not (gate.requires_grad and torch.is_grad_enabled()), who,
+                'no gradient of over 60000 gate rows that are shared by several rows each: detach the gate, or expand it to the shape of x')
     no_tangents(who, *ts)
     on_gpu(x, who)
     flags = (_LAYER if layer else 0) | (_POST if post else 0) | (_PRE if pre else 0)

@@ -29,6 +29,7 @@ struct NormArgs {
   float* part;                                     // [chunks][5][C]: dpost_w, dpost_b, dpre_w, dpre_b, dgate
   long long span, rpc;                             // rows that may share a chunk (those of a gate row, or all); rows of a chunk
   int cpg;                                         // chunks of a span
+  int each;                                        // the gate is loaded for every row, not kept for a chunk
   int want;                                        // bit k: quantity k of `part` is wanted
 };
 
@@ -195,7 +196,8 @@ __global__ __launch_bounds__((TPR > 256 ? TPR : 256), 4) void block_norm_kernel(
   }
 }
 
-// One workgroup = one chunk of rows inside one gate row, so the gate is a constant of the chunk (or every row has its own: rpg == 1).
+// One workgroup = one chunk of rows inside one gate row, so the gate is a constant of the chunk, or (`each`: every row has its own, or so many are shared that a chunk
+// for each would be mostly partial sums, and no gradient of theirs is asked for) the gate is one more input of the row.
 template <typename T, int V, int TPR, int NIT, bool LAYER>
 __global__ __launch_bounds__((TPR > 256 ? TPR : 256), (TPR > 512 ? 4 : LAYER ? 2 : 3)) void block_norm_bwd_kernel(NormArgs a) {
   constexpr int WG = TPR > 256 ? TPR : 256, RPB = WG / TPR;
@@ -209,8 +211,8 @@ __global__ __launch_bounds__((TPR > 256 ? TPR : 256), (TPR > 512 ? 4 : LAYER ? 2
   long long last = first + a.rpc;
   if (last > (gr + 1) * a.span) last = (gr + 1) * a.span;
   if (last > a.rows) last = a.rows;
-  const bool per_row = a.gate && a.rpg == 1;       // a gate row of its own per row: its gradient is written in place
-  const bool own_gate = per_row && a.dgate;
+  const bool per_row = a.gate && a.each;
+  const bool own_gate = per_row && a.dgate;        // a gate row of its own per row: its gradient is written in place
   Vec<T, V> pw[NIT], pb[NIT], qw[NIT], gv[NIT];
   if (a.pw) load_row<T, V, TPR, NIT>(a.pw, 0, t, C, pw);
   if (a.pb) load_row<T, V, TPR, NIT>(a.pb, 0, t, C, pb);
@@ -265,7 +267,7 @@ __global__ __launch_bounds__((TPR > 256 ? TPR : 256), (TPR > 512 ? 4 : LAYER ? 2
     }
     if (a.y) load_row<T, V, TPR, NIT>(a.y, at, t, C, r.y);
     if (a.dxo) load_row<T, V, TPR, NIT>(a.dxo, at, t, C, r.dx);
-    if (per_row) load_row<T, V, TPR, NIT>(a.gate, at, t, C, r.g);
+    if (per_row) load_row<T, V, TPR, NIT>(a.gate, a.rpg == 1 ? at : gate_row(a, row) * C, t, C, r.g);
   };
   In in;
   long long row = first + threadIdx.x / TPR;
@@ -466,9 +468,11 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(const float* part, lon
   if (share == 0 && c < C) ((T*)o)[(k < 4 ? 0 : gr * C) + c] = (T)s[x];
 }
 
-// chunks: as many workgroups as the chip holds at a time (three per CU, two for the layer norm's registers), none across a gate row
+constexpr long long kMostGates = 60000;            // shared gate rows whose gradients are formed (a workgroup row of the column sums each)
+
+// chunks: as many workgroups as the chip holds at a time (three per CU, two for the layer norm's registers), none across a gate row that is kept for a chunk
 static long long cut_rows(NormArgs& a, int rpb) {
-  a.span = a.gate && a.rpg > 1 ? a.rpg : a.rows;
+  a.span = a.gate && !a.each ? a.rpg : a.rows;
   const long long gates = a.rows / a.span;         // (check_norm: rows divide into gate rows)
   const long long want = a.layer ? 512 : 768;
   long long cpg = (want + gates - 1) / gates;
@@ -579,9 +583,9 @@ int pgrf_block_norm(const PgrfBlockNorm* p, void* stream) {
 
 size_t pgrf_block_norm_backward_workspace_bytes(long long rows, int C, long long rows_per_gate) {
   if (rows < 1 || C < 1 || rows_per_gate < 1) return 16;
-  // an upper bound of cut_rows' chunks: 768, plus one for each gate row
+  // an upper bound of cut_rows' chunks: 768, plus one for each gate row that is kept for a chunk
   const long long gates = rows_per_gate > 1 ? (rows + rows_per_gate - 1) / rows_per_gate : 1;
-  return (size_t)(768 + gates) * 5 * (size_t)C * sizeof(float);
+  return (size_t)(768 + (gates > kMostGates ? 1 : gates)) * 5 * (size_t)C * sizeof(float);
 }
 
 int pgrf_block_norm_backward(const PgrfBlockNorm* p, void* stream) {
@@ -605,7 +609,8 @@ int pgrf_block_norm_backward(const PgrfBlockNorm* p, void* stream) {
   long long chunks = 0;
   a.cpg = 1;
   const long long gates = (a.want & 16) && p->rows ? p->rows / p->rows_per_gate : 0;
-  if (gates > 60000) return set_error(PGRF_ERR_UNSUPPORTED, "%s: %lld gate rows (at most 60000, or one for each row)", who, gates);
+  if (gates > kMostGates) return set_error(PGRF_ERR_UNSUPPORTED, "%s: gradients of %lld gate rows (at most %lld, or one for each row)", who, gates, kMostGates);
+  a.each = per_row || (p->gate && p->rows / p->rows_per_gate > kMostGates) ? 1 : 0;
   if (p->rows) {
     chunks = cut_rows(a, h.tpr > 256 ? 1 : 256 / h.tpr);
     const size_t need = (size_t)chunks * 5 * C * sizeof(float);

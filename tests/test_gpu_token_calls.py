@@ -5,6 +5,34 @@ import torch
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('kind', ['rms', 'layer'])
+def test_a_gate_for_each_of_many_rays(kind, dtype):
+    """Over 60 000 shared gate rows: what the gate expanded to every row gives, to the last bit, and a gradient of that form."""
+    from panogrf_amd.block_norm import block_norm
+    g = torch.Generator(device='cuda').manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g, device='cuda').to(dtype)
+    for rays, n, C in ((70001, 3, 16), (60001, 2, 33), (60002, 4, 520)):
+        x, y, gate, dx, dz = r(rays, n, C), r(rays, n, C), r(rays, C), r(rays, n, C), r(rays, n, C)
+        w = [r(C) for _ in range(4 if kind == 'layer' else 2)]
+
+        def run(gate):
+            ts = [t.detach().requires_grad_(True) for t in (x, y, *w)]
+            names = ('post_weight', 'pre_weight', 'post_bias', 'pre_bias')
+            outs = block_norm(ts[0], ts[1], gate, kind=kind, scale=0.5, **dict(zip(names, ts[2:])))
+            return tuple(t.detach() for t in outs) + torch.autograd.grad(outs, ts, (dx, dz))
+        got, want = run(gate), run(gate.unsqueeze(1).expand(rays, n, C).contiguous())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        # no weights: no sums over rows, and no scratch for them
+        ts = [t.detach().requires_grad_(True) for t in (x, y)]
+        a, b = block_norm(*ts, gate, kind=kind, scale=0.5), block_norm(*ts, gate.unsqueeze(1).expand(rays, n, C), kind=kind, scale=0.5)
+        assert all(torch.equal(s, t) for s, t in zip(torch.autograd.grad(a, ts, (dx, dz)), torch.autograd.grad(b, ts, (dx, dz))))
+        # the way the refusal names: the expanded gate's gradient, added up outside
+        leaf = gate.detach().requires_grad_(True)
+        full = torch.autograd.grad(block_norm(x, y, leaf.unsqueeze(1).expand(rays, n, C), kind=kind, scale=0.5), leaf, (dx, dz))[0]
+        assert full.shape == gate.shape and torch.isfinite(full).all()
+
+
 def test_one_query_a_stream_in_sequence_first_memory():
     """[1, B, H, 2, d].transpose(0, 1): contiguous, with over 2^22 values from the only token to the next."""
     from panogrf_amd.attention import diff_attention, diff_attention_cached

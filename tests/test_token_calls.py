@@ -2,8 +2,9 @@
 import ctypes as C
 
 import pytest
+import torch
 
-from panogrf_amd._lib import lib
+from panogrf_amd._lib import PgrfBlockNorm, lib
 from tests.test_token_refusals import PTR, attn
 
 FAR = 1 << 23
@@ -19,3 +20,22 @@ def test_strides_of_axes_of_one_token_do_not_matter(kw):
 def test_those_of_others_do(kw):
     a = attn(**kw, lse=PTR)
     assert lib.pgrf_diff_attention_backward(C.byref(a), PTR, PTR, PTR, PTR, PTR, None) == -3 and b'stride' in lib.pgrf_last_error()
+
+
+def test_many_shared_gate_rows():
+    """Only the gate's own gradient has a limit of them; without it they cost no workspace of their own either."""
+    from panogrf_amd._lib import PgrfError
+    from panogrf_amd.block_norm import block_norm
+    x, gate = torch.zeros(60001, 2, 4), torch.ones(60001, 4)
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad), pytest.raises(PgrfError, match='GPU'):         # (as far as CPU tensors go)
+            block_norm(x.requires_grad_(grad), x.detach(), gate)
+    with torch.no_grad(), pytest.raises(PgrfError, match='GPU'):
+        block_norm(x, x, gate.requires_grad_(True))
+    with pytest.raises(PgrfError, match='60000'):
+        block_norm(x, x, gate)
+    assert lib.pgrf_block_norm_backward_workspace_bytes(1 << 20, 64, 2) < 1 << 20
+    assert lib.pgrf_block_norm_backward_workspace_bytes(60000 * 2, 64, 2) >= 60000 * 5 * 64 * 4
+    a = PgrfBlockNorm(x=PTR, y=PTR, gate=PTR, stats=PTR, dx_out=PTR, dz=PTR, dx=PTR, dy=PTR, dpost_w=PTR, dpre_w=PTR, rows=1 << 20, rows_per_gate=2, dtype=0, C=64, flags=6,
+                      scale=1.0, workspace=PTR, workspace_bytes=64)
+    assert lib.pgrf_block_norm_backward(C.byref(a), None) == -1 and b'workspace' in lib.pgrf_last_error()
