@@ -122,6 +122,7 @@ def diff_attention(q, k, v, lam, *, causal=False, key_mask=None, scale=None):
     that do not start at multiples of 16 bytes are copied first).  key_mask [B, M] bool, False: no query sees the key, and what it holds does not matter.
     causal: query i sees keys up to i + M - N, so the last query stands at the last key.  A query that sees no key gives 0 and
     has no part in any gradient, whatever it and its gradient hold.  scale: 1/sqrt(d) unless given.
+    Sizes: B Hk below 2^25, B H N and, with gradients, B Hk M below 2^29 fit the launches; what does not fit is refused.  M up to 2^30, H 2 d up to 2^22.
     Softmax and sums are float; probabilities and score gradients are rounded to the tensors' type for the products behind them.  Gradients (first derivatives, by backward) to
     q, k, v and lam; they do not depend on scheduling."""
     who = 'diff_attention'

@@ -781,49 +781,53 @@ __global__ __launch_bounds__(256) void diff_attn_sizes(DiffArgs a) {
   using F = typename Frag8<T>::type;
   constexpr int L = 2 * D / 8, kRows = 256 / L;                                // threads of a row, eight values each; rows at a time, four times
   __shared__ float2 most[4];
-  const int bh = blockIdx.x / a.size_parts, part = blockIdx.x % a.size_parts, b = bh / a.Hk, hk = bh % a.Hk, tid = threadIdx.x, group = tid / L, e = tid % L * 8;
-  const int keys = (a.M + a.size_parts - 1) / a.size_parts, k0 = part * keys, k1 = min(k0 + keys, a.M);
-  const int all = a.N * a.G, rows = (all + a.size_parts - 1) / a.size_parts, r0 = part * rows, r1 = min(r0 + rows, all);
-  const unsigned char* mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
-  const T* v = (const T*)a.v + b * a.v_sb + hk * a.v_sh + e;
-  float v2 = 0.f, g2 = 0.f;
-  for (int k = k0 + group; k < k1; k += 4 * kRows) {
-    F x[4];
-    bool in[4];
+  const int tid = threadIdx.x, group = tid / L, e = tid % L * 8;
+  for (long long at_part = blockIdx.x; at_part < (long long)a.B * a.Hk * a.size_parts; at_part += gridDim.x) {
+    const int bh = (int)(at_part / a.size_parts), part = (int)(at_part % a.size_parts), b = bh / a.Hk, hk = bh % a.Hk;
+    const int keys = (a.M + a.size_parts - 1) / a.size_parts, k0 = part * keys, k1 = min(k0 + keys, a.M);
+    const int all = a.N * a.G, rows = (all + a.size_parts - 1) / a.size_parts, r0 = part * rows, r1 = min(r0 + rows, all);
+    const unsigned char* mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+    const T* v = (const T*)a.v + b * a.v_sb + hk * a.v_sh + e;
+    float v2 = 0.f, g2 = 0.f;
+    for (int k = k0 + group; k < k1; k += 4 * kRows) {
+      F x[4];
+      bool in[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int at = min(k + j * kRows, k1 - 1);
-      x[j] = load8<T>(v + at * a.v_sn);
-      in[j] = !mask || mask[at];
-    }
+      for (int j = 0; j < 4; ++j) {
+        const int at = min(k + j * kRows, k1 - 1);
+        x[j] = load8<T>(v + at * a.v_sn);
+        in[j] = !mask || mask[at];
+      }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float s = group_sum<L>(square(x[j]));
-      v2 = in[j] ? fmaxf(v2, s) : v2;
+      for (int j = 0; j < 4; ++j) {
+        const float s = group_sum<L>(square(x[j]));
+        v2 = in[j] ? fmaxf(v2, s) : v2;
+      }
     }
+    for (int r = r0 + group; r < r1; r += 4 * kRows) {
+      F x[4];
+      float lse[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = min(r + j * kRows, r1 - 1), n = at / a.G, head = hk * a.G + at % a.G;
+        x[j] = load8<T>((const T*)a.dout + (((long long)b * a.N + n) * a.H + head) * 2 * D + e);
+        lse[j] = a.lse[((long long)b * a.H + head) * 2 * a.N + n];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float s = group_sum<L>(square(x[j]));
+        g2 = lse[j] == INFINITY ? g2 : fmaxf(g2, s);
+      }
+    }
+    v2 = group_max<64>(v2);
+    g2 = group_max<64>(g2);
+    if ((tid & 63) == 0) most[tid >> 6] = make_float2(v2, g2);
+    __syncthreads();
+    if (tid == 0)
+      *(float2*)(a.sizes + 2 * at_part) = make_float2(fmaxf(fmaxf(most[0].x, most[1].x), fmaxf(most[2].x, most[3].x)),
+                                                           fmaxf(fmaxf(most[0].y, most[1].y), fmaxf(most[2].y, most[3].y)));
+    __syncthreads();
   }
-  for (int r = r0 + group; r < r1; r += 4 * kRows) {
-    F x[4];
-    float lse[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int at = min(r + j * kRows, r1 - 1), n = at / a.G, head = hk * a.G + at % a.G;
-      x[j] = load8<T>((const T*)a.dout + (((long long)b * a.N + n) * a.H + head) * 2 * D + e);
-      lse[j] = a.lse[((long long)b * a.H + head) * 2 * a.N + n];
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float s = group_sum<L>(square(x[j]));
-      g2 = lse[j] == INFINITY ? g2 : fmaxf(g2, s);
-    }
-  }
-  v2 = group_max<64>(v2);
-  g2 = group_max<64>(g2);
-  if ((tid & 63) == 0) most[tid >> 6] = make_float2(v2, g2);
-  __syncthreads();
-  if (tid == 0)
-    *(float2*)(a.sizes + 2ll * blockIdx.x) = make_float2(fmaxf(fmaxf(most[0].x, most[1].x), fmaxf(most[2].x, most[3].x)),
-                                                         fmaxf(fmaxf(most[0].y, most[1].y), fmaxf(most[2].y, most[3].y)));
 }
 
 // The largest |lam| of the heads that share a key head

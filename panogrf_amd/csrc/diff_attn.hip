@@ -71,6 +71,10 @@ static int size_parts(int dtype, int N, int M, int G) {
   return most > 256 * 64 ? 256 : (int)((most + 63) / 64);
 }
 
+// Whether a launch has room for so many workgroups: 2^32 - 1 threads.  With B Hk below 2^25, and B H N and (for gradients) B Hk M below 2^29, all launches do: up to 64 rows or
+// keys a key head takes 128 threads, beyond that a row or key less than eight.
+static bool fits(long long workgroups, int threads) { return workgroups <= 0x7fffffffll && workgroups * threads <= 0xffffffffll; }
+
 static int check(const PgrfDiffAttn* p, const char* who, bool backward) {
   if (!p) return set_error(PGRF_ERR_ARG, "%s: null arguments", who);
   if (!dtype_ok(p->dtype)) return set_error(PGRF_ERR_UNSUPPORTED, "%s: dtype %d (PGRF_DTYPE_F32 | BF16 | F16)", who, p->dtype);
@@ -80,8 +84,7 @@ static int check(const PgrfDiffAttn* p, const char* who, bool backward) {
   if (!(p->scale > 0.f) || p->scale > 1e30f) return set_error(PGRF_ERR_ARG, "%s: scale must be positive", who);
   if ((long long)p->N * (p->H / p->Hk) > 0x3fffffff || (long long)p->B * p->N > 0x3fffffff || p->M > 0x3fffffff)
     return set_error(PGRF_ERR_UNSUPPORTED, "%s: over 2^30 rows", who);
-  if ((long long)p->B * p->H * (((long long)p->N + 31) / 32 + 1) > 0xffffff || (long long)p->B * p->Hk * (((long long)p->M + 31) / 32) > 0x7fffffff)
-    return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tiles", who);
+  if ((long long)p->B * p->Hk > (1 << 26)) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tiles", who);   // (what is counted from here on fits 64 bits)
   if ((long long)p->B * p->N == 0) return PGRF_OK;
   if (!p->q || !p->k || !p->v || !p->lam) return set_error(PGRF_ERR_ARG, "%s: null q / k / v / lam", who);
   const long long per = 16 / (long long)dtype_bytes(p->dtype);
@@ -145,7 +148,7 @@ int pgrf_diff_attention(const PgrfDiffAttn* p, void* stream) {
     a.part_ml = a.part_o + (size_t)a.splits * a.B * a.Hk * rows * 4 * p->D;
   }
   const long long grid = (long long)a.B * a.Hk * ((rows + cut.rows - 1) / cut.rows) * a.splits;
-  if (grid > 0x7fffffffll) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tiles", who);
+  if (!fits(grid, cut.waves * 64)) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tiles", who);
 #define PGRF_DA_FWD(T, D_) \
   if (p->dtype == T && p->D == D_) return launch_da_fwd_##T##_##D_(a, cut.waves, (unsigned)grid, (hipStream_t)stream);
   PGRF_DA_ALL(PGRF_DA_FWD)
@@ -172,13 +175,15 @@ int pgrf_diff_attention_backward(const PgrfDiffAttn* p, const void* dout, void* 
   if (!dk != !dv) return set_error(PGRF_ERR_ARG, "%s: dk and dv go together", who);
   if ((long long)p->B * p->N == 0) return set_error(PGRF_ERR_ARG, "%s: no rows: the gradients are 0", who);
   if (!dout || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return set_error(PGRF_ERR_ARG, "%s: dout null, or a tensor not 16-byte aligned", who);
+  const BwdCut c = cut_bwd(p->dtype, p->B, p->N, p->M, p->H, p->Hk, p->D, p->causal != 0);
+  const long long rg = c.row_groups * c.q_shares, kg = c.key_groups * c.kv_shares;
+  if (!fits(rg, c.row_waves * 64) || !fits(kg, c.key_waves * 64)) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tiles", who);
   const size_t need = pgrf_diff_attention_backward_workspace_bytes(p->dtype, p->B, p->N, p->M, p->H, p->Hk, p->D, p->causal);
   if (!p->workspace || !aligned16(p->workspace) || p->workspace_bytes < need)
     return set_error(PGRF_ERR_ARG, "%s: workspace too small or not 16-byte aligned (%zu < %zu bytes)", who, p->workspace_bytes, need);
   DiffArgs a = args_of(p);
   a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv; a.dlam = dlam;
   a.delta = (float*)p->workspace;
-  const BwdCut c = cut_bwd(p->dtype, a.B, a.N, a.M, a.H, a.Hk, p->D, a.causal != 0);
   a.q_shares = c.q_shares; a.kv_shares = c.kv_shares;
   const size_t sums = (size_t)a.B * a.H * 2 * a.N;
   a.dlam_part = a.delta + sums;
@@ -190,8 +195,6 @@ int pgrf_diff_attention_backward(const PgrfDiffAttn* p, const void* dout, void* 
   }
   if (c.q_shares > 1) { a.dq_part = behind; behind += (size_t)c.q_shares * a.B * a.N * a.H * 2 * p->D; }
   if (c.kv_shares > 1) { a.dk_part = behind; a.dv_part = behind + (size_t)c.kv_shares * a.B * a.M * a.Hk * 2 * p->D; }
-  const long long rg = c.row_groups * c.q_shares, kg = c.key_groups * c.kv_shares;
-  if (rg > 0x7fffffffll || kg > 0x7fffffffll) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tiles", who);
 #define PGRF_DA_BWD(T, D_) \
   if (p->dtype == T && p->D == D_) return launch_da_bwd_##T##_##D_(a, c.row_waves, (unsigned)rg, c.units, c.key_waves, (unsigned)kg, (hipStream_t)stream);
   PGRF_DA_ALL(PGRF_DA_BWD)

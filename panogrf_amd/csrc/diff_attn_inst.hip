@@ -66,7 +66,8 @@ int PGRF_DA_NAME(launch_da_bwd)(const DiffArgs& a, int row_waves, unsigned row_g
   }
 #endif
 #if PGRF_DA_TYPE == 2
-  hipLaunchKernelGGL((diff_attn_sizes<DaT, PGRF_DA_D>), dim3((unsigned)(a.B * a.Hk * a.size_parts)), dim3(256), 0, s, a);
+  const long long parts = (long long)a.B * a.Hk * a.size_parts;
+  hipLaunchKernelGGL((diff_attn_sizes<DaT, PGRF_DA_D>), dim3((unsigned)(parts < (1 << 16) ? parts : 1 << 16)), dim3(256), 0, s, a);
   PGRF_TOK_LAUNCHED(who);
 #endif
   if (row_waves == 1) hipLaunchKernelGGL((diff_attn_dq<DaT, PGRF_DA_D, 1>), dim3(row_grid), dim3(64), 0, s, a);

@@ -56,3 +56,26 @@ def test_one_query_a_stream_in_sequence_first_memory():
     far = v1.as_strided(v1.shape, (v1.stride(0), 1 << 23, v1.stride(2), 1))
     n.clamp_(max=1)
     assert all(torch.equal(a, b) for a, b in zip(run(q, k1, far), run(one, k[:, :1].clone(), v1.clone(memory_format=torch.contiguous_format))))
+
+
+@pytest.mark.parametrize('B,H,D,M,dtype', [((1 << 20) + 3, 16, 32, 2, torch.bfloat16), ((1 << 20) + 1, 8, 128, 1, torch.float16)])
+def test_more_than_two_to_the_24_tiles(B, H, D, M, dtype):
+    """What calls of parts of the batch give, to the last bit (parts of over 1280 key heads: fewer are cut otherwise and take other kernels)."""
+    from panogrf_amd.attention import diff_attention
+    g = torch.Generator(device='cuda').manual_seed(2)
+    r = lambda *s: torch.randn(*s, generator=g, device='cuda', dtype=dtype)
+    q, k, v, do, lam = r(B, 1, H, 2, D), r(B, M, H, 2, D), r(B, M, H, 2 * D), r(B, 1, H, 2 * D), torch.rand(H, generator=g, device='cuda')
+
+    def run(*ts):
+        ts, do = [t.detach().requires_grad_(True) for t in ts[:4]], ts[4]
+        out = diff_attention(*ts)
+        return (out.detach(), *torch.autograd.grad(out, ts, do))
+    whole, sums = run(q, k, v, lam, do), torch.zeros(H, dtype=torch.float64, device='cuda')
+    for i in range(0, B, B // 5 + 1):
+        at = slice(i, i + B // 5 + 1)
+        part = run(q[at], k[at], v[at], lam, do[at])
+        assert all(torch.equal(a[at], b) for a, b in zip(whole[:4], part[:4])), i
+        sums += part[4].double()
+    # dlam: a float sum over B rows in 4096 chains, each term a sum of 2 D products, on both sides
+    most = (do.abs().float() * v.abs().float()).sum(-1).amax(1).sum(0).double()
+    assert ((whole[4].double() - sums).abs() <= 2 * 2.0 ** -24 * (B / 4096 + 64 + 2 * D) * most).all()

@@ -39,3 +39,18 @@ def test_many_shared_gate_rows():
     a = PgrfBlockNorm(x=PTR, y=PTR, gate=PTR, stats=PTR, dx_out=PTR, dz=PTR, dx=PTR, dy=PTR, dpost_w=PTR, dpre_w=PTR, rows=1 << 20, rows_per_gate=2, dtype=0, C=64, flags=6,
                       scale=1.0, workspace=PTR, workspace_bytes=64)
     assert lib.pgrf_block_norm_backward(C.byref(a), None) == -1 and b'workspace' in lib.pgrf_last_error()
+
+
+@pytest.mark.parametrize('dtype', [0, 1, 2])
+@pytest.mark.parametrize('kw', [dict(B=524288, N=64, M=64, H=16, Hk=16, D=32), dict(B=1 << 20, N=1, M=3, H=16, Hk=16, D=64), dict(B=(1 << 22) - 1, N=1, M=1, H=8, Hk=8, D=128),
+                                dict(B=(1 << 14) - 1, N=1 << 13, M=1, H=4, Hk=1, D=32), dict(B=1 << 18, N=65, M=33, H=31, Hk=31, D=128)])
+def test_many_workgroups(kw, dtype):
+    """B Hk below 2^25, B H N and B Hk M below 2^29: every launch has room for them."""
+    a = attn(**kw, dtype=dtype, lse=PTR, workspace=PTR, workspace_bytes=16)
+    assert lib.pgrf_diff_attention_backward(C.byref(a), PTR, PTR, PTR, PTR, PTR, None) == -1 and b'workspace' in lib.pgrf_last_error()   # (asked for behind the tiles)
+
+
+def test_too_many_workgroups():
+    a = attn(B=1 << 26, N=1, M=1, H=2, Hk=2, D=64, lse=PTR, workspace=PTR, workspace_bytes=1 << 62)
+    assert lib.pgrf_diff_attention_backward(C.byref(a), PTR, PTR, PTR, PTR, PTR, None) == -3 and b'tiles' in lib.pgrf_last_error()
+    assert lib.pgrf_diff_attention(C.byref(a), None) == -3 and b'tiles' in lib.pgrf_last_error()
