@@ -229,9 +229,11 @@ extern "C" int pgrf_rotary(const PgrfRotary* p, void* stream) {
   if (tile > tokens / 1024) tile = tokens / 1024;
   if (tile > 4096 / (rotary_dim / 2)) tile = 4096 / (rotary_dim / 2);
   if (tile > kMaxTile) tile = kMaxTile;
-  a.tile = tile < 1 ? 1 : (int)tile;
+  const long long least = tokens / 0xffffff + 1;    // a launch holds 2^32 - 1 threads, 256 a workgroup
+  if (tile < least) tile = least;
+  if (tile > kMaxTile || tile * a.items >= (1 << 21) || (tile > 1 && tile * (rotary_dim / 2) > 4096)) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tokens", who);   // (2^21: quick_div)
+  a.tile = (int)tile;
   const long long grid = (tokens + a.tile - 1) / a.tile;
-  if (grid > 0x7fffffffll) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tokens", who);
   const size_t lds = (size_t)a.tile * (rotary_dim / 2) * sizeof(float2);
   if (dtype == PGRF_DTYPE_F32) launch_rotary<float>(a, vec, dim3((unsigned)grid), lds, (hipStream_t)stream);
   else if (dtype == PGRF_DTYPE_BF16) launch_rotary<bf16>(a, vec, dim3((unsigned)grid), lds, (hipStream_t)stream);

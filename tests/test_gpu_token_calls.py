@@ -79,3 +79,15 @@ def test_more_than_two_to_the_24_tiles(B, H, D, M, dtype):
     # dlam: a float sum over B rows in 4096 chains, each term a sum of 2 D products, on both sides
     most = (do.abs().float() * v.abs().float()).sum(-1).amax(1).sum(0).double()
     assert ((whole[4].double() - sums).abs() <= 2 * 2.0 ** -24 * (B / 4096 + 64 + 2 * D) * most).all()
+
+
+def test_rotary_of_more_than_two_to_the_24_wide_tokens():
+    """Heads so wide that a workgroup would take one token, of one panorama's queries seen by many entries."""
+    from panogrf_amd.rotary import rotary
+    g = torch.Generator(device='cuda').manual_seed(3)
+    B, N, H, D = 4096, 4099, 27, 38
+    one = torch.randn(1, N, H, D, generator=g, device='cuda').bfloat16()
+    with torch.no_grad():
+        want = rotary(one, None, torch.arange(N, device='cuda'))[0][0]
+        got = rotary(one.expand(B, N, H, D), None, torch.arange(N, device='cuda'))[0]
+        assert all(torch.equal(got[i], want) for i in (0, 1, 2047, 4001, 4094, 4095))

@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 import torch
 
-from panogrf_amd._lib import PgrfBlockNorm, lib
+from panogrf_amd._lib import PgrfBlockNorm, PgrfRotary, lib
 from tests.test_token_refusals import PTR, attn
 
 FAR = 1 << 23
@@ -54,3 +54,14 @@ def test_too_many_workgroups():
     a = attn(B=1 << 26, N=1, M=1, H=2, Hk=2, D=64, lse=PTR, workspace=PTR, workspace_bytes=1 << 62)
     assert lib.pgrf_diff_attention_backward(C.byref(a), PTR, PTR, PTR, PTR, PTR, None) == -3 and b'tiles' in lib.pgrf_last_error()
     assert lib.pgrf_diff_attention(C.byref(a), None) == -3 and b'tiles' in lib.pgrf_last_error()
+
+
+def rotary(**kw):
+    a = dict(q=PTR, positions=PTR, q_out=PTR, q_sb=0, q_sn=0, q_sh=0, base=1e4, factor=1.0, dtype=1, q_heads=1, rotary_dim=2, magnitude=1.0)
+    return lib.pgrf_rotary(C.byref(PgrfRotary(**{**a, **kw})), None)
+
+
+def test_rotary_tokens():
+    """What no launch holds is refused as such, not by the runtime: 2^30 tokens (less where over 2^21 values and pairs of a workgroup's tokens would have to be counted)."""
+    for kw in (dict(B=1 << 15, N=(1 << 15) + 1, D=2), dict(B=1 << 15, N=1 << 12, D=33, q_heads=31 * 1024)):
+        assert rotary(**kw) == -3 and b'too many tokens' in lib.pgrf_last_error()
