@@ -123,7 +123,9 @@ def diff_attention(q, k, v, lam, *, causal=False, key_mask=None, scale=None):
     causal: query i sees keys up to i + M - N, so the last query stands at the last key.  A query that sees no key gives 0 and
     has no part in any gradient, whatever it and its gradient hold.  scale: 1/sqrt(d) unless given.
     Sizes: B Hk below 2^25, B H N and, with gradients, B Hk M below 2^29 fit the launches; what does not fit is refused.  M up to 2^30, H 2 d up to 2^22.
-    Softmax and sums are float; probabilities and score gradients are rounded to the tensors' type for the products behind them.  Gradients (first derivatives, by backward) to
+    Softmax and sums are float.  Probabilities are not rounded to fewer bits than the output holds where 32 queries or 64 keys at most share a key head, and in bfloat16
+    from 1024 such queries and B H N M d = 2^33 on; elsewhere they are, each map's by itself, to the tensors' type for the product with v, as are the maps' difference and the
+    score gradients in the backward pass (in float16 brought into its range first).  Gradients (first derivatives, by backward) to
     q, k, v and lam; they do not depend on scheduling."""
     who = 'diff_attention'
     scale = _check(who, q, k, v, lam, scale)
@@ -144,8 +146,8 @@ def diff_attention(q, k, v, lam, *, causal=False, key_mask=None, scale=None):
 def diff_attention_cached(q, k_cache, v_cache, lam, lengths, *, scale=None):
     """The same over a cache: k_cache [B, M, Hk, 2, d], v_cache [B, M, Hk, 2 d] of which the first lengths[b] keys count (lengths [B] int32 on the device,
     clamped to [0, M]; the rest may hold anything).  q [B, N, H, 2, d]: the last N tokens of each entry, causal among themselves: query i sees keys up to
-    lengths[b] - N + i.  N = 1 is the step of a served model.  The lengths are read on the device, so a captured step follows them.  Where 32 query heads and
-    tokens at most share a key head, probabilities are not rounded to the tensors' type.  No gradients."""
+    lengths[b] - N + i.  N = 1 is the step of a served model.  The lengths are read on the device, so a captured step follows them.  Probabilities
+    are rounded where diff_attention's are: not where 32 query heads and tokens at most share a key head.  No gradients."""
     who = 'diff_attention_cached'
     scale = _check(who, q, k_cache, v_cache, lam, scale)
     if not (isinstance(lengths, torch.Tensor) and lengths.dtype == torch.int32 and lengths.device == q.device and lengths.dim() == 1 and lengths.shape[0] == q.shape[0]):

@@ -185,6 +185,11 @@ struct DiffArgs {
   void* out;                      // [B,N,H,2D]
   float* lse;                     // [B,H,2,N]: log2 of the sum behind each map, +inf where a row sees nothing
   float* o12;                     // [B,N,H,2,2D]: the two maps' outputs
+  // bf16, where products bound the forward pass: v in f16 [B*Hk][M][2D] times 2^v_exp of the key head (kWide: not), and what v_exp comes from, in parts of the keys
+  void* v16;
+  int* v_exp;                     // [B*Hk]
+  float* v_sizes;                 // [B*Hk][v_parts][2]: the largest |v|, and the smallest among the keys' largest
+  int v_parts;
   // a key axis cut into `splits`: partial [splits][B*Hk][N*G] rows of 2 x 2D values and (m1, l1, m2, l2)
   int splits;
   float *part_o, *part_ml;
@@ -283,7 +288,18 @@ __device__ __forceinline__ unsigned keys_of_lane(unsigned seen32, int last, int 
 // ---------------------------------------------------------------------------------------------------------------- forward
 // MPW: maps of a wave.  Up to D = 64 a wave keeps the sums of both maps of its 32 rows (128 registers), and every fragment of v serves two products.  At
 // D = 128 two waves share 32 rows, one map each, and meet at the end.
-template <typename T, int D, int NW> struct FwdShape {
+// How probabilities go into the product with v (16 bits).  kOne: rounded to the tensors' type.  What the two maps have in common cancels in out and their roundings do not: of
+// independent maps out is off by 0.0026 of its norm in bf16, where 0.0017 is its own rounding, of maps that nearly cancel by that many times more.
+// kTwo: in two pieces, what the type holds and what that leaves: nothing is lost, for 20 products of N M D in place of 12.  Taken where memory bounds the kernel: up to 32 rows
+// (caches as in cut_fwd: 246 us both ways), and up to 64 keys (2048 rays of 64 samples, 4 heads x 64, bf16: 164 us in one piece, 166 in two; x 32: 50, 52).
+// kInF16 (bf16): v goes to f16 first, by a power of two that is exact but for values 2^-13 of their own key's largest, and with it the probabilities, which have 8 times
+// finer steps there at the same rate.  That is two launches over v, and one for key heads whose keys differ too much for f16's range (kWide), which take kTwo: 6 + 7 + 5 us for
+// 8093 keys of 4 heads x 128.  Taken where products bound a long kernel (2 x 8192, 8 heads x 64, training: 2866 us in one piece, 2926 in f16, 3290 in two; 4001 of 8093, 16/4 heads
+// x 128, causal: 615, 651, 870).  All other sizes, and f16 itself beyond 64 keys, keep kOne.
+enum { kOne = 0, kTwo = 1, kInF16 = 2 };
+constexpr int kWide = 1 << 20;
+
+template <typename T, int D, int NW, int HOW> struct FwdShape {
   static_assert(D < 128 || NW > 1, "a pair of waves at D = 128");
   static constexpr int MPW = D == 128 ? 1 : 2, RW = NW * MPW / 2;              // RW: groups of 32 rows in the workgroup
   static constexpr int KT = 32;                                                // keys of a block
@@ -292,9 +308,8 @@ template <typename T, int D, int NW> struct FwdShape {
   static constexpr bool kWeave = sizeof(T) == 4 && D > 32;
   static constexpr int kMinWaves = kWeave || NW == 1 ? 1 : 2;
   static constexpr int kTileKeys = sizeof(T) == 2 && RW == 4 ? 64 : 32;        // keys between barriers: fewer barriers where LDS holds two such tiles
-  // Up to 32 rows (single tokens) memory bounds the kernel, and probabilities go into the product with v in two pieces, what the type holds and what that leaves (the result is
-  // off by 0.0017 of its norm, all from its own rounding to bf16; 0.0026 with one piece.  Caches as in cut_fwd: 246 us both ways).  Elsewhere that would cost half the speed.
-  static constexpr bool kTwoPieces = sizeof(T) == 2 && RW == 1;
+  static constexpr bool kTwoPieces = HOW == kTwo;
+  using V = typename std::conditional<HOW == kInF16, f16, T>::type;            // v and the probabilities in their product
 };
 
 // Scores of a block: S^T of MPW maps
@@ -323,19 +338,21 @@ __device__ __forceinline__ float with_other_half(float t) {                    /
 // products of 32x32x16 (386 ns at its peak) and the vector pipe 96 FMAs and 32 exponentials with their sums and roundings (over 312 ns); side by side the two take 471 ns
 // at best, and here they are busy for 45% and 57% of the time (2 x 8192 rows and keys, 8 heads, bf16: 895 us, 924 TFLOP/s; at D = 128 no exponential is left over, 1000).  With kWeave a wave has three blocks in work: while block j goes through its exponentials, the matrix pipe
 // forms the scores of block j + 1 and adds block j - 1 times its values, in one stretch of code without a branch; masks and a new maximum are dealt with in front of it.
-// P1 and P2 are each rounded to the tensors' type for their product with v (their difference could be rounded once only if both rows' sums were known first); what the two
-// maps have in common cancels in out and their roundings do not, which is where 0.0026 of its norm in bf16 comes from (0.0017 is its own rounding).
-template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff_attn_fwd(DiffArgs a) {
+template <typename T, int D, int NW, int HOW>
+__global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW, HOW>::kMinWaves)) void diff_attn_fwd(DiffArgs a) {
   using TL = Tile<T, D>;
   using F = typename Frag8<T>::type;
-  using Sh = FwdShape<T, D, NW>;
+  using Sh = FwdShape<T, D, NW, HOW>;
+  using VT = typename Sh::V;
+  using TV = Tile<VT, D>;
+  using FV = typename Frag8<VT>::type;
   constexpr int KT = Sh::KT, MPW = Sh::MPW, NK = D / 16, NC = 2 * D / 32, RW = Sh::RW;
   constexpr int kTile = KT * TL::kRow;
   constexpr int BT = Sh::kTileKeys / KT;                                         // blocks between barriers
   __shared__ __attribute__((aligned(1024))) char tiles_lds[4 * BT * kTile];        // two tiles of k, two of v
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const typename TL::Lane at(lane);
+  const typename TV::Lane atv(lane);
   const int group = MPW == 2 ? wave : wave >> 1, map0 = MPW == 2 ? 0 : wave & 1;
   const int rows = a.N * a.G, tiles = (rows + RW * 32 - 1) / (RW * 32);
   // Workgroups side by side: the tiles of rows of one key head, on one XCD, so that they find its keys in its L2 (causal: the longest rows first).  Where there is one tile,
@@ -355,6 +372,11 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
     bh = id / tiles;
   }
   const int b = bh / a.Hk, hk = bh % a.Hk;
+  if constexpr (HOW == kInF16) {
+    if (a.v_exp[bh] == kWide) return;
+  } else if constexpr (HOW == kTwo) {
+    if (a.v_exp && a.v_exp[bh] != kWide) return;
+  }
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.M) : a.M;
   const int r0 = (tile * RW + group) * 32, r = r0 + (lane & 31), rc = min(r, rows - 1);
   const int n = rc / a.G, head = hk * a.G + rc % a.G;
@@ -376,16 +398,18 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
     for (int s = 0; s < NK; ++s) qf[m][s] = load8<T>(q + m * a.q_sm + 16 * s);
 
   const T* k = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
-  const T* v = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
+  const VT* v = HOW == kInF16 ? (const VT*)a.v16 + (long long)bh * a.M * 2 * D : (const VT*)a.v + b * a.v_sb + hk * a.v_sh;
+  const long long v_sn = HOW == kInF16 ? 2 * D : a.v_sn;
   const unsigned char* mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
-  const typename TL::template Loader<KT, NW> lk(a.k_sn, a.k_sm, tid), lv(a.v_sn, D, tid);
+  const typename TL::template Loader<KT, NW> lk(a.k_sn, a.k_sm, tid);
+  const typename TV::template Loader<KT, NW> lv(v_sn, D, tid);
   auto ktile = [&](int t) { return tiles_lds + (t & 1) * kTile; };
   auto vtile = [&](int t) { return tiles_lds + 2 * kTile + (t & 1) * kTile; };
   auto fetch_k = [&](int t) { lk(ktile(t), k + (long long)t * KT * a.k_sn, len - t * KT, tid, wave); };
-  auto fetch_v = [&](int t) { lv(vtile(t), v + (long long)t * KT * a.v_sn, len - t * KT, tid, wave); };
+  auto fetch_v = [&](int t) { lv(vtile(t), v + (long long)t * KT * v_sn, len - t * KT, tid, wave); };
 
   f32x16 o[MPW][NC], s[MPW];
-  F p[MPW][2], rest[Sh::kTwoPieces ? MPW : 1][2];
+  FV p[MPW][2], rest[Sh::kTwoPieces ? MPW : 1][2];
   float mx[MPW], l[MPW], top[MPW];
 #pragma unroll
   for (int m = 0; m < MPW; ++m) {
@@ -396,14 +420,14 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[m][i][j] = (T)0.f;
+      for (int j = 0; j < 8; ++j) p[m][i][j] = (VT)0.f;
   }
   auto add_block = [&](const char* vt) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const F vf = TL::col(vt, at, i, c);
+        const FV vf = TV::col(vt, atv, i, c);
 #pragma unroll
         for (int m = 0; m < MPW; ++m) o[m][c] = mma(vf, p[m][i], o[m][c]);
       }
@@ -436,7 +460,7 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[m][i][j] = (T)((float)p[m][i][j] * f);
+            for (int j = 0; j < 8; ++j) p[m][i][j] = (VT)((float)p[m][i][j] * f);
       }
     }
   };
@@ -516,11 +540,12 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
   } else if (t0 < t1) {
     // two or more waves on a SIMD: one's exponentials run beside another's products, block by block
     constexpr int kB = BT * KT;
-    const typename TL::template Loader<kB, NW> bk(a.k_sn, a.k_sm, tid), bv(a.v_sn, D, tid);
+    const typename TL::template Loader<kB, NW> bk(a.k_sn, a.k_sm, tid);
+    const typename TV::template Loader<kB, NW> bv(v_sn, D, tid);
     auto tile_at = [&](int t) { return tiles_lds + (t & 1) * 2 * BT * kTile; };  // k, then v
     auto fetch = [&](int t) {
       bk(tile_at(t), k + (long long)t * kB * a.k_sn, len - t * kB, tid, wave);
-      bv(tile_at(t) + BT * kTile, v + (long long)t * kB * a.v_sn, len - t * kB, tid, wave);
+      bv(tile_at(t) + BT * kTile, v + (long long)t * kB * v_sn, len - t * kB, tid, wave);
     };
     fetch(t0);
     for (int t = t0; t < t1; ++t) {
@@ -555,13 +580,13 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
           for (int e = 0; e < 16; ++e) {
             const float w = __builtin_amdgcn_exp2f(fmaf(s[m][e], a.c, -base));
             sum += w;
-            p[m][e / 8][e % 8] = (T)w;
-            if constexpr (Sh::kTwoPieces) rest[m][e / 8][e % 8] = (T)(w - (float)(T)w);
+            p[m][e / 8][e % 8] = (VT)w;
+            if constexpr (Sh::kTwoPieces) rest[m][e / 8][e % 8] = (VT)(w - (float)(VT)w);
           }
           l[m] += sum;
         }
-        weave<F, 2 * NC, 2>([&](int i) { return TL::col(vb, at, i / NC, i % NC); },
-                            [&](int i, const F& f) {
+        weave<FV, 2 * NC, 2>([&](int i) { return TV::col(vb, atv, i / NC, i % NC); },
+                            [&](int i, const FV& f) {
 #pragma unroll
                               for (int m = 0; m < MPW; ++m) {
                                 o[m][i % NC] = mma(f, p[m][i / NC], o[m][i % NC]);
@@ -575,6 +600,13 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
   landed();
 #pragma unroll
   for (int m = 0; m < MPW; ++m) l[m] += __shfl_xor(l[m], 32, 64);
+  if constexpr (HOW == kInF16) {
+    const float undo = ldexpf(1.f, -a.v_exp[bh]);
+#pragma unroll
+    for (int m = 0; m < MPW; ++m)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) o[m][c] *= undo;
+  }
   const bool live = r < rows;
   if (a.splits > 1) {
     if (!live) return;
@@ -649,6 +681,92 @@ __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW>::kMinWaves)) void diff
         for (int j = 0; j < 4; ++j) u[j] = o[0][c][4 * g + j] - lam * o[MPW - 1][c][4 * g + j];
         store4<T>(out + 32 * c + 8 * g, u[0], u[1], u[2], u[3]);
       }
+  }
+}
+
+// The largest |v| of keys that are seen, and the smallest of their largest (finite values; keys of zeros aside), in parts
+template <typename T, int D>
+__global__ __launch_bounds__(256) void diff_attn_v_sizes(DiffArgs a) {
+  using F = typename Frag8<T>::type;
+  constexpr int L = 2 * D / 8, kRows = 256 / L;
+  __shared__ float2 both[4];
+  const int tid = threadIdx.x, part = blockIdx.x % a.v_parts, bh = blockIdx.x / a.v_parts, b = bh / a.Hk, hk = bh % a.Hk;
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.M) : a.M;
+  const int keys = (a.M + a.v_parts - 1) / a.v_parts, k1 = min(part * keys + keys, len);
+  const unsigned char* mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+  const T* v = (const T*)a.v + b * a.v_sb + hk * a.v_sh + tid % L * 8;
+  float most = 0.f, least = INFINITY;
+  for (int k = part * keys + tid / L; k < k1; k += 4 * kRows) {
+    F x[4];
+    bool in[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = min(k + j * kRows, k1 - 1);
+      x[j] = load8<T>(v + at * a.v_sn);
+      in[j] = !mask || mask[at];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float u = fabsf((float)x[j][i]);
+        m = u < INFINITY ? fmaxf(m, u) : m;
+      }
+#pragma unroll
+      for (int o = L / 2; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+      most = in[j] ? fmaxf(most, m) : most;
+      least = in[j] && m > 0.f ? fminf(least, m) : least;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    most = fmaxf(most, __shfl_xor(most, o, 64));
+    least = fminf(least, __shfl_xor(least, o, 64));
+  }
+  if ((tid & 63) == 0) both[tid >> 6] = make_float2(most, least);
+  __syncthreads();
+  if (tid == 0)
+    *(float2*)(a.v_sizes + 2ll * blockIdx.x) = make_float2(fmaxf(fmaxf(both[0].x, both[1].x), fmaxf(both[2].x, both[3].x)),
+                                                           fminf(fminf(both[0].y, both[1].y), fminf(both[2].y, both[3].y)));
+}
+
+// v in f16, with the key head's largest value at 2^14: what is 2^-28 of it still has all its bits, and a key whose largest is 2^-15 of it those down to 2^-13 of its own
+template <typename T, int D>
+__global__ __launch_bounds__(256) void diff_attn_v16(DiffArgs a) {
+  using F = typename Frag8<T>::type;
+  constexpr int L = 2 * D / 8, kRows = 256 / L;
+  const int tid = threadIdx.x, lane = tid & 63, part = blockIdx.x % a.v_parts, bh = blockIdx.x / a.v_parts, b = bh / a.Hk, hk = bh % a.Hk;
+  float most = 0.f, least = INFINITY;
+  for (int i = lane; i < a.v_parts; i += 64) {
+    const float2 x = *(const float2*)(a.v_sizes + ((long long)bh * a.v_parts + i) * 2);
+    most = fmaxf(most, x.x);
+    least = fminf(least, x.y);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    most = fmaxf(most, __shfl_xor(most, o, 64));
+    least = fminf(least, __shfl_xor(least, o, 64));
+  }
+  const bool wide = most > 0.f && ilogbf(most) - ilogbf(least) > 15;
+  const int e = most > 0.f ? min(14 - ilogbf(most), 120) : 0;
+  if (part == 0 && tid == 0) a.v_exp[bh] = wide ? kWide : e;
+  if (wide) return;
+  const float f = ldexpf(1.f, e);
+  const int keys = (a.M + a.v_parts - 1) / a.v_parts, k1 = min(part * keys + keys, a.M);
+  const T* v = (const T*)a.v + b * a.v_sb + hk * a.v_sh + tid % L * 8;
+  f16* out = (f16*)a.v16 + (long long)bh * a.M * 2 * D + tid % L * 8;
+  for (int k = part * keys + tid / L; k < k1; k += 4 * kRows) {
+    F x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = load8<T>(v + min(k + j * kRows, k1 - 1) * a.v_sn);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      Frag8<f16>::type y;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = (f16)((float)x[j][i] * f);
+      if (k + j * kRows < k1) *(Frag8<f16>::type*)(out + (long long)(k + j * kRows) * 2 * D) = y;
+    }
   }
 }
 

@@ -6,7 +6,7 @@ namespace pgrf {
 namespace tok {
 
 #define PGRF_DA_DECL(T, D)                                                                       \
-  int launch_da_fwd_##T##_##D(const DiffArgs& a, int waves, unsigned grid, hipStream_t s);       \
+  int launch_da_fwd_##T##_##D(const DiffArgs& a, int waves, unsigned grid, int how, hipStream_t s); \
   int launch_da_bwd_##T##_##D(const DiffArgs& a, int row_waves, unsigned row_grid, int units, int key_waves, unsigned key_grid, hipStream_t s);
 #define PGRF_DA_ALL(X) X(0, 32) X(0, 64) X(0, 128) X(1, 32) X(1, 64) X(1, 128) X(2, 32) X(2, 64) X(2, 128)
 PGRF_DA_ALL(PGRF_DA_DECL)
@@ -14,9 +14,13 @@ PGRF_DA_ALL(PGRF_DA_DECL)
 static int waves_for(long long rows) { return rows > 64 ? 4 : rows > 32 ? 2 : 1; }
 
 // The forward kernel's waves and their rows: at D = 128 two waves share 32 rows (and float's values leave no room for eight)
-struct FwdCut { int waves, rows, splits; };
+struct FwdCut { int waves, rows, splits, how, v_parts; };
 static FwdCut cut_fwd(int dtype, int B, int Hk, long long rows, int M, int D) {
   FwdCut f;
+  // (kTwo, kInF16 and what they cost stand at their names.  v in f16 from 2^33 products of a score and 1024 rows on: a forward pass there takes 100-180 us and 12-20 more with the
+  // launches over v, at 2^34 11 or 23 more on 220, at 2^32 17 on 67 and 12 on 101; 64 x 512 rows and keys, 2^33: 45 more on 176.)
+  f.how = dtype == PGRF_DTYPE_F32 ? kOne : rows <= 32 || M <= 64 ? kTwo : dtype == PGRF_DTYPE_BF16 && rows >= 1024 && (double)B * Hk * rows * M * D >= 8589934592.0 ? kInF16 : kOne;
+  f.v_parts = f.how != kInF16 ? 0 : M > 256 * 64 ? 256 : (M + 63) / 64;
   f.waves = waves_for(rows);
   if (D == 128) f.waves = f.waves == 4 && dtype == PGRF_DTYPE_F32 ? 4 : 2 * f.waves;
   f.rows = D == 128 ? f.waves * 16 : f.waves * 32;
@@ -127,8 +131,10 @@ extern "C" {
 size_t pgrf_diff_attention_workspace_bytes(int dtype, int B, int N, int M, int H, int Hk, int D) {
   if (B < 1 || N < 1 || M < 1 || H < 1 || Hk < 1 || H % Hk || D < 1) return 0;
   const long long rows = (long long)N * (H / Hk);
-  const int s = cut_fwd(dtype, B, Hk, rows, M, D).splits;
-  return s > 1 ? (size_t)s * B * Hk * rows * (4 * D + 4) * sizeof(float) : 0;
+  const FwdCut c = cut_fwd(dtype, B, Hk, rows, M, D);
+  size_t n = c.splits > 1 ? (size_t)c.splits * B * Hk * rows * (4 * D + 4) * sizeof(float) : 0;
+  if (c.how == kInF16) n += (size_t)B * Hk * M * 2 * D * 2 + ((size_t)B * Hk * c.v_parts * 8 + 15) / 16 * 16 + ((size_t)B * Hk * 4 + 15) / 16 * 16;
+  return n;
 }
 
 int pgrf_diff_attention(const PgrfDiffAttn* p, void* stream) {
@@ -140,17 +146,27 @@ int pgrf_diff_attention(const PgrfDiffAttn* p, void* stream) {
   const long long rows = (long long)a.N * a.G;
   const FwdCut cut = cut_fwd(p->dtype, a.B, a.Hk, rows, a.M, p->D);
   a.splits = cut.splits;
+  const size_t need = pgrf_diff_attention_workspace_bytes(p->dtype, p->B, p->N, p->M, p->H, p->Hk, p->D);
+  if (need && (!p->workspace || !aligned16(p->workspace) || p->workspace_bytes < need))
+    return set_error(PGRF_ERR_ARG, "%s: workspace too small or not 16-byte aligned (%zu < %zu bytes)", who, p->workspace_bytes, need);
+  char* room = (char*)p->workspace;
   if (a.splits > 1) {
-    const size_t need = pgrf_diff_attention_workspace_bytes(p->dtype, p->B, p->N, p->M, p->H, p->Hk, p->D);
-    if (!p->workspace || !aligned16(p->workspace) || p->workspace_bytes < need)
-      return set_error(PGRF_ERR_ARG, "%s: workspace too small or not 16-byte aligned (%zu < %zu bytes)", who, p->workspace_bytes, need);
-    a.part_o = (float*)p->workspace;
-    a.part_ml = a.part_o + (size_t)a.splits * a.B * a.Hk * rows * 4 * p->D;
+    const size_t n = (size_t)a.splits * a.B * a.Hk * rows;
+    a.part_o = (float*)room;
+    a.part_ml = a.part_o + n * 4 * p->D;
+    room += n * (4 * p->D + 4) * sizeof(float);
+  }
+  if (cut.how == kInF16) {
+    a.v_parts = cut.v_parts;
+    a.v16 = room;
+    room += (size_t)a.B * a.Hk * a.M * 2 * p->D * 2;
+    a.v_sizes = (float*)room;
+    a.v_exp = (int*)(room + ((size_t)a.B * a.Hk * a.v_parts * 8 + 15) / 16 * 16);
   }
   const long long grid = (long long)a.B * a.Hk * ((rows + cut.rows - 1) / cut.rows) * a.splits;
-  if (!fits(grid, cut.waves * 64)) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tiles", who);
+  if (!fits(grid, cut.waves * 64) || !fits((long long)a.B * a.Hk * cut.v_parts, 256)) return set_error(PGRF_ERR_UNSUPPORTED, "%s: too many tiles", who);
 #define PGRF_DA_FWD(T, D_) \
-  if (p->dtype == T && p->D == D_) return launch_da_fwd_##T##_##D_(a, cut.waves, (unsigned)grid, (hipStream_t)stream);
+  if (p->dtype == T && p->D == D_) return launch_da_fwd_##T##_##D_(a, cut.waves, (unsigned)grid, cut.how, (hipStream_t)stream);
   PGRF_DA_ALL(PGRF_DA_FWD)
   return set_error(PGRF_ERR_UNSUPPORTED, "%s: no kernel", who);
 }

@@ -18,15 +18,43 @@ using DaT = f16;
 #define PGRF_DA_NAME(f) PGRF_DA_NAME1(f, PGRF_DA_TYPE, PGRF_DA_D)
 
 #if !PGRF_DA_BWD
-int PGRF_DA_NAME(launch_da_fwd)(const DiffArgs& a, int waves, unsigned grid, hipStream_t s) {
+template <int HOW>
+static void launch_fwd(const DiffArgs& a, int waves, unsigned grid, hipStream_t s) {
+  // (16 bits: up to 32 rows, one wave or a pair of them, are kTwo; kInF16 is for whole workgroups of rows)
+  constexpr int D = PGRF_DA_D;
+  constexpr bool few = (HOW == kTwo) == (PGRF_DA_TYPE != 0), whole = HOW == kInF16;
+  if constexpr (D < 128 && few) {
+    if (waves == 1) hipLaunchKernelGGL((diff_attn_fwd<DaT, D, 1, HOW>), dim3(grid), dim3(64), 0, s, a);
+  }
+  if constexpr ((D < 128 && !whole) || few) {
+    if (waves == 2) hipLaunchKernelGGL((diff_attn_fwd<DaT, D, 2, HOW>), dim3(grid), dim3(128), 0, s, a);
+  }
+  if constexpr (D < 128 || !whole) {
+    if (waves == 4) hipLaunchKernelGGL((diff_attn_fwd<DaT, D, 4, HOW>), dim3(grid), dim3(256), 0, s, a);
+  }
+  if constexpr (D == 128 && PGRF_DA_TYPE != 0) {
+    if (waves == 8) hipLaunchKernelGGL((diff_attn_fwd<DaT, D, 8, HOW>), dim3(grid), dim3(512), 0, s, a);
+  }
+}
+
+int PGRF_DA_NAME(launch_da_fwd)(const DiffArgs& a, int waves, unsigned grid, int how, hipStream_t s) {
   const char* who = "pgrf_diff_attention";
-#if PGRF_DA_D < 128
-  if (waves == 1) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 1>), dim3(grid), dim3(64), 0, s, a);
+#if PGRF_DA_TYPE == 0
+  launch_fwd<kOne>(a, waves, grid, s);
+#else
+  if (how == kOne) launch_fwd<kOne>(a, waves, grid, s);
+#if PGRF_DA_TYPE == 1
+  if (how == kInF16) {
+    const dim3 parts((unsigned)(a.B * a.Hk * a.v_parts));
+    hipLaunchKernelGGL((diff_attn_v_sizes<DaT, PGRF_DA_D>), parts, dim3(256), 0, s, a);
+    PGRF_TOK_LAUNCHED(who);
+    hipLaunchKernelGGL((diff_attn_v16<DaT, PGRF_DA_D>), parts, dim3(256), 0, s, a);
+    PGRF_TOK_LAUNCHED(who);
+    launch_fwd<kInF16>(a, waves, grid, s);
+    PGRF_TOK_LAUNCHED(who);
+  }
 #endif
-  if (waves == 2) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 2>), dim3(grid), dim3(128), 0, s, a);
-  if (waves == 4) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 4>), dim3(grid), dim3(256), 0, s, a);
-#if PGRF_DA_D == 128 && PGRF_DA_TYPE != 0
-  if (waves == 8) hipLaunchKernelGGL((diff_attn_fwd<DaT, PGRF_DA_D, 8>), dim3(grid), dim3(512), 0, s, a);
+  if (how != kOne) launch_fwd<kTwo>(a, waves, grid, s);                        // (behind kInF16: the key heads that it left)
 #endif
   PGRF_TOK_LAUNCHED(who);
   if (a.splits > 1) {
