@@ -289,7 +289,8 @@ __device__ __forceinline__ unsigned keys_of_lane(unsigned seen32, int last, int 
 // MPW: maps of a wave.  Up to D = 64 a wave keeps the sums of both maps of its 32 rows (128 registers), and every fragment of v serves two products.  At
 // D = 128 two waves share 32 rows, one map each, and meet at the end.
 // How probabilities go into the product with v (16 bits).  kOne: rounded to the tensors' type.  What the two maps have in common cancels in out and their roundings do not: of
-// independent maps out is off by 0.0026 of its norm in bf16, where 0.0017 is its own rounding, of maps that nearly cancel by that many times more.
+// independent maps out is off by 0.0026 of its norm in bf16, where 0.0017 is its own rounding, of sharp maps that nearly cancel by
+// 0.0068 (scores of 3, nearly equal, 0.9 of the second taken off; 0.0018 in f16).
 // kTwo: in two pieces, what the type holds and what that leaves: nothing is lost, for 20 products of N M D in place of 12.  Taken where memory bounds the kernel: up to 32 rows
 // (caches as in cut_fwd: 246 us both ways), and up to 64 keys (2048 rays of 64 samples, 4 heads x 64, bf16: 164 us in one piece, 166 in two; x 32: 50, 52).
 // kInF16 (bf16): v goes to f16 first, by a power of two that is exact but for values 2^-13 of their own key's largest, and with it the probabilities, which have 8 times
@@ -336,7 +337,7 @@ __device__ __forceinline__ float with_other_half(float t) {                    /
 
 // One pass over the keys in blocks of 32 with the running maximum and sum of each row's softmax.  What bounds it: per block and wave at D = 64 the matrix pipe has 24
 // products of 32x32x16 (386 ns at its peak) and the vector pipe 96 FMAs and 32 exponentials with their sums and roundings (over 312 ns); side by side the two take 471 ns
-// at best, and here they are busy for 45% and 57% of the time (2 x 8192 rows and keys, 8 heads, bf16: 895 us, 924 TFLOP/s; at D = 128 no exponential is left over, 1000).  With kWeave a wave has three blocks in work: while block j goes through its exponentials, the matrix pipe
+// at best, and here they are busy for 45% and 57% of the time (2 x 8192 rows and keys, 8 heads, bf16: 820-855 us, 960-1000 TFLOP/s, as at D = 128, where no exponential is left over; the first calls on an idle card take 13% longer).  With kWeave a wave has three blocks in work: while block j goes through its exponentials, the matrix pipe
 // forms the scores of block j + 1 and adds block j - 1 times its values, in one stretch of code without a branch; masks and a new maximum are dealt with in front of it.
 template <typename T, int D, int NW, int HOW>
 __global__ __launch_bounds__(NW * 64, (FwdShape<T, D, NW, HOW>::kMinWaves)) void diff_attn_fwd(DiffArgs a) {
@@ -862,7 +863,7 @@ __global__ __launch_bounds__(S > 1 ? 2 * D * S : 256) void diff_attn_join(DiffAr
 //
 // Two waves or more share a SIMD and run beside each other, but for dq and dk at D = 128 in 16 bits, whose registers leave a SIMD one wave: those weave three blocks as the
 // forward kernel does.  Float does neither, as its products take eight times as long and hide the rest by themselves.  Both pipes are bound as in the forward kernel (2 x 8192,
-// 8 heads, bf16, D = 64: dq 920 us, 896 TFLOP/s; dk and dv 1244 us, 884 TFLOP/s).
+// 8 heads, bf16, D = 64: dq 850-885 us, dk and dv 1130-1180 us, both 930-970 TFLOP/s).
 // In f16 the backward pass brings what it rounds into the type's range by powers of two that the float sums' last factor takes out again.  A score gradient a (G - delta) is a
 // probability, about 1 / M, times what is often a mean loss' gradient: rounded as it is, it is lost below 2^-25 where dq and dk are well in range (8192 keys, dout of 1e-4: dq
 // off by 7%), and is infinite above 65504.  |a (G - delta)| is at most 2 |dout_i| |v_j| and |a1 - lam a2| at most 1 + |lam|; with those at 2^14 what is 2^-28 of them still
@@ -1548,7 +1549,7 @@ __device__ __forceinline__ float sums_of_half(const f32x16& a, const f32x16& b, 
 // All gradients of a key head with up to 64 keys in one go: a workgroup holds the keys, a wave 32 of them, and the queries of the head pass by once, so that scores, maps and
 // the products with v are formed once (10 products of N M D where the two kernels above have 14, or 20 with delta's sweep) and every input is read once.  delta is the sum of
 // a row's A G over the lanes and waves that hold its keys; score gradients go through LDS, turned round, to the sum over keys that is dq.  Bound by its chain of loads, products
-// and stores with a wave on a SIMD (2048 rays x 4 heads x 64 samples, float, D = 32: 351 us, the matrix pipe busy for 41%; three workgroups to a CU, or starts apart from each
+// and stores with a wave on a SIMD (2048 rays x 4 heads x 64 samples, float, D = 32: 326 us, on an idle card 350, the matrix pipe busy for 40%; three workgroups to a CU, or starts apart from each
 // other, were no quicker).
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, 1) void diff_attn_short(DiffArgs a) {

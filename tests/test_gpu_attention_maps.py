@@ -110,7 +110,7 @@ def test_values_in_f16(B, N, M, H, Hk, D, causal):
 @pytest.mark.parametrize('B,N,M,H,Hk,D', LONG)
 @pytest.mark.parametrize('causal', [False, True])
 def test_sharp_maps(B, N, M, H, Hk, D, causal):
-    """Maps of a few keys, nearly alike, with nearly all of the one taken off: 13 times the maps' roundings in bf16 would be left."""
+    """Maps of a few keys, nearly alike, with nearly all of the one taken off: roundings to bf16 are four times the output's own there."""
     q, k, v, lam = make(B, N, M, H, Hk, D, torch.bfloat16)
     check(q * 4, k, v, lam, causal, way='f16', rows=some(N, 6), chance=True)
 
