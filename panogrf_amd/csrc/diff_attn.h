@@ -37,7 +37,7 @@ __device__ __forceinline__ const void* same_in_all_lanes(const void* p) {
 }
 
 // 16 (or 4) bytes of every lane, from base + its offset, straight into LDS, one lane behind the other from the wave's address `to`.  As assembly, because the compiler lets a
-// transposed read wait for every such load in flight, though it goes to another tile.  Nothing but fetched() waits for these.  Nor does the compiler keep the distances inside
+// transposed read wait for every such load in flight, though it goes to another tile.  Nothing but landed() waits for these.  Nor does the compiler keep the distances inside
 // assembly that the chip asks for: five wait states from a vector instruction that writes a scalar register (the base comes from readfirstlane) to the instruction on memory that
 // reads it, one from a write of m0.  The five stand in front of every load (tests/test_token_isa.py looks them over in the built code).
 __device__ __forceinline__ void fetch16(const void* base, unsigned off, unsigned to) {
@@ -292,7 +292,8 @@ __device__ __forceinline__ unsigned keys_of_lane(unsigned seen32, int last, int 
 // independent maps out is off by 0.0026 of its norm in bf16, where 0.0017 is its own rounding, of sharp maps that nearly cancel by
 // 0.0068 (scores of 3, nearly equal, 0.9 of the second taken off; 0.0018 in f16).
 // kTwo: in two pieces, what the type holds and what that leaves: nothing is lost, for 20 products of N M D in place of 12.  Taken where memory bounds the kernel: up to 32 rows
-// (caches as in cut_fwd: 246 us both ways), and up to 64 keys (2048 rays of 64 samples, 4 heads x 64, bf16: 164 us in one piece, 166 in two; x 32: 50, 52).
+// (caches as in cut_fwd: 246 us both ways), and up to 64 keys (2048 rays of 64 samples, 4 heads x 64, bf16: 164 us in one piece, 166 in two; x 32: 50, 52; 1024 rows
+// on 64 keys, 64 x 8 heads x 32: 40, 45; x 128: 268, 283).
 // kInF16 (bf16): v goes to f16 first, by a power of two that is exact but for values 2^-13 of their own key's largest, and with it the probabilities, which have 8 times
 // finer steps there at the same rate.  That is two launches over v, and one for key heads whose keys differ too much for f16's range (kWide), which take kTwo: 6 + 7 + 5 us for
 // 8093 keys of 4 heads x 128.  Taken where products bound a long kernel (2 x 8192, 8 heads x 64, training: 2866 us in one piece, 2926 in f16, 3290 in two; 4001 of 8093, 16/4 heads
